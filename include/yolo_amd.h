@@ -317,6 +317,150 @@ int yolo_amd_conv_query(const yolo_amd_conv_desc* desc, yolo_amd_conv_choice* ou
 int yolo_amd_conv_forward(const yolo_amd_conv_desc* descs, int n, const void* zero_page,
                           void* stream);
 
+/* ---------------------------------------------------------------- matrix product with epilogue
+ * y = act(x weight^T + bias) + residual, and its gradients.  No counterpart in the reference, whose
+ * only matrix products are 1x1 convolutions (yolo_amd_conv_forward runs those, on packed weights); these
+ * take plain row-major matrices of any size: a transformer block's layers, a classifier's, a prompt's
+ * thousands of rows or one token's.
+ *
+ * x is [m][k], weight [n][k], both of `type`; bias [n], residual [m][n] and y [m][n] are of `type`, or
+ * fp32 where their flag says so.  Row strides (ld*) are in elements and at least the row's length; any
+ * alignment to the element is accepted (rows that start on 16-byte boundaries with k a multiple of 8 are
+ * read in place, others are copied into the workspace by the call).  Sums are fp32, in an order that
+ * depends on the sizes only; y is rounded once.  m == 0 and n == 0 do nothing; k == 0 sums nothing. */
+#define YOLO_AMD_TYPE_F32 0
+#define YOLO_AMD_TYPE_BF16 1
+#define YOLO_AMD_TYPE_F16 2
+
+#define YOLO_AMD_ACT_NONE 0
+#define YOLO_AMD_ACT_LEAKY 1     /* max(v, 0.1 v), the network's own                    */
+#define YOLO_AMD_ACT_RELU 2
+#define YOLO_AMD_ACT_GELU 3      /* v (1 + erf(v / sqrt 2)) / 2                         */
+#define YOLO_AMD_ACT_GELU_TANH 4 /* v (1 + tanh(sqrt(2 / pi) (v + 0.044715 v^3))) / 2   */
+#define YOLO_AMD_ACT_SILU 5      /* v / (1 + exp(-v))                                   */
+
+typedef struct {
+    const void* x;
+    const void* weight;
+    const void* bias;     /* or NULL                                                    */
+    const void* residual; /* or NULL; may be y itself (same stride and type)            */
+    void* y;
+    void* pre;            /* or NULL: x weight^T + bias [m][n] (no gaps between rows),   */
+                          /* rounded to `type`: what yolo_amd_linear_backward wants      */
+    int64_t m, n, k;
+    int64_t ldx, ldw, ldr, ldy;
+    int type;             /* YOLO_AMD_TYPE_BF16 or YOLO_AMD_TYPE_F16                     */
+    int bias_f32, residual_f32, y_f32;
+    int activation;       /* YOLO_AMD_ACT_*                                             */
+    void* workspace;      /* 256-byte aligned, yolo_amd_linear_workspace_bytes bytes     */
+    size_t workspace_bytes;
+} yolo_amd_linear_desc;
+
+/* Bytes of scratch this call wants (0: none).  Reads the shapes, strides and the alignment of the
+ * pointers; 0 as well for a descriptor that yolo_amd_linear_forward would refuse. */
+size_t yolo_amd_linear_workspace_bytes(const yolo_amd_linear_desc* desc);
+int yolo_amd_linear_forward(const yolo_amd_linear_desc* desc, void* stream);
+
+/* Which kernel yolo_amd_linear_forward runs for a descriptor, and with what tiling (for tests and tuning). */
+#define YOLO_AMD_LINEAR_ROWS 1 /* few rows: reads the weights once, straight into the matrix units */
+#define YOLO_AMD_LINEAR_TILE 2 /* tiles through LDS                                              */
+typedef struct {
+    int kernel;      /* YOLO_AMD_LINEAR_*                                */
+    int bm, bn;      /* rows x columns of y per workgroup                */
+    int k_slices;    /* > 1: split reduction + finishing launch          */
+    int copies_x, copies_weight; /* 1: the operand is copied into the workspace first */
+} yolo_amd_linear_choice;
+int yolo_amd_linear_query(const yolo_amd_linear_desc* desc, yolo_amd_linear_choice* out);
+
+/* Gradients of yolo_amd_linear_forward for dy = d(loss)/dy (the residual's gradient is dy itself).
+ * With dp = dy * act'(pre): dx = dp weight, dweight = dp^T x, dbias = column sums of dp.  dp is rounded
+ * to `type` as the operand of both products (as pre was when it was kept); the column sums take it unrounded.
+ * dx [m][k], dweight [n][k] of `type` without gaps between rows; each of dx, dweight, dbias may be NULL.
+ * weight is read for dx only, x for dweight only, pre unless the activation is YOLO_AMD_ACT_NONE.
+ * All sums have a fixed order. */
+typedef struct {
+    const void* dy;       /* [m][n], stride lddy, of `type` or fp32 (dy_f32)             */
+    const void* x;
+    const void* weight;
+    const void* pre;      /* as written by yolo_amd_linear_forward                       */
+    void* dx;
+    void* dweight;
+    void* dbias;          /* [n] of `type` or fp32 (dbias_f32)                           */
+    int64_t m, n, k;
+    int64_t lddy, ldx, ldw;
+    int type;
+    int dy_f32, dbias_f32;
+    int activation;
+    void* workspace;      /* 256-byte aligned                                            */
+    size_t workspace_bytes;
+} yolo_amd_linear_backward_desc;
+
+size_t yolo_amd_linear_backward_workspace_bytes(const yolo_amd_linear_backward_desc* desc);
+int yolo_amd_linear_backward(const yolo_amd_linear_backward_desc* desc, void* stream);
+
+/* ---------------------------------------------------------------- norms around a residual add
+ * What lies between two blocks of a residual network, in one pass over memory.  Per row of d values:
+ *
+ *     p      = after ? norm(x) * after_weight + after_bias : x
+ *     stream = residual + scale * gate * p
+ *     normed = norm(stream) * before_weight + before_bias           (with `before`)
+ *
+ * norm(v) = v / sqrt(mean(v^2) + eps) (YOLO_AMD_NORM_RMS, which takes no biases) or (v - mean(v)) /
+ * sqrt(var(v) + eps), biased variance (YOLO_AMD_NORM_LAYER).  No counterpart in the reference, whose only
+ * norm is BatchNorm2d (yolo_amd_bn_train).  x and normed are of `type` (fp32, bf16 or fp16); residual and
+ * stream are of `type`, or fp32 with stream_f32.  The gate is of `type` or fp32: row i of x takes row
+ * i / rows_per_gate of it (1: a gate for each row; the rows of a sequence: one for each sequence; >= rows:
+ * one for all).  Weights and biases are of `type` or fp32, one flag per norm.  NULL stands for: no residual
+ * (0), no gate (1), no weight (1), no bias (0).  Statistics are fp32; stream is rounded once, and normed is
+ * taken from the unrounded stream.  Rows are independent of each other; 1 <= d <= 16384. */
+#define YOLO_AMD_NORM_RMS 0
+#define YOLO_AMD_NORM_LAYER 1
+
+typedef struct {
+    const void* x;            /* [rows][d], row stride ldx                                */
+    const void* residual;     /* [rows][d], row stride ldr, or NULL                       */
+    const void* gate;         /* [ceil(rows / rows_per_gate)][d] without gaps, or NULL    */
+    const void* after_weight; /* [d] or NULL, as the three below                          */
+    const void* after_bias;
+    const void* before_weight;
+    const void* before_bias;
+    void* stream;             /* [rows][d] without gaps, or NULL: not wanted              */
+    void* normed;             /* [rows][d] without gaps; NULL without `before`            */
+    int64_t rows, d;
+    int64_t ldx, ldr;         /* in elements                                              */
+    int64_t rows_per_gate;
+    int type;                 /* YOLO_AMD_TYPE_*                                          */
+    int norm;                 /* YOLO_AMD_NORM_*                                          */
+    int after, before;        /* which of the two norms are there                         */
+    int stream_f32, gate_f32, after_f32, before_f32;
+    float eps, scale;
+} yolo_amd_block_norm_desc;
+
+int yolo_amd_block_norm_forward(const yolo_amd_block_norm_desc* desc, void* stream);
+
+/* Gradients of yolo_amd_block_norm_forward.  `forward` is its descriptor (the outputs in it are not used;
+ * everything is recomputed from x and residual).  dnormed and dstream: gradients of the two outputs, [rows][d]
+ * without gaps, of `type` and of the stream's type; NULL: zero.  Of the gradients below each may be NULL:
+ * dx and dresidual [rows][d] of x's and the stream's type, the others shaped and typed like what they belong
+ * to.  With a gate, rows must be whole runs of rows_per_gate (or one run).  All sums have a fixed order. */
+typedef struct {
+    yolo_amd_block_norm_desc forward;
+    const void* dnormed;
+    const void* dstream;
+    void* dx;
+    void* dresidual;
+    void* dgate;
+    void* dafter_weight;
+    void* dafter_bias;
+    void* dbefore_weight;
+    void* dbefore_bias;
+    void* workspace;          /* 256-byte aligned                                         */
+    size_t workspace_bytes;
+} yolo_amd_block_norm_backward_desc;
+
+size_t yolo_amd_block_norm_backward_workspace_bytes(const yolo_amd_block_norm_backward_desc* desc);
+int yolo_amd_block_norm_backward(const yolo_amd_block_norm_backward_desc* desc, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -94,6 +94,71 @@ KERNEL_FIRST, KERNEL_STEM, KERNEL_THIN, KERNEL_PATCH, KERNEL_IGEMM = 1, 2, 3, 4,
 KERNEL_NAMES = {1: "first", 2: "stem", 3: "thin", 4: "patch", 5: "igemm", 6: "block"}
 
 
+TYPE_F32, TYPE_BF16, TYPE_F16 = 0, 1, 2
+ACT_CODES = {None: 0, "leaky": 1, "relu": 2, "gelu": 3, "gelu_tanh": 4, "silu": 5}
+NORM_CODES = {"rms": 0, "layer": 1}
+LINEAR_KERNEL_NAMES = {0: "none", 1: "rows", 2: "tile"}
+
+
+class LinearDesc(ctypes.Structure):
+    """yolo_amd_linear_desc of include/yolo_amd.h."""
+    _fields_ = [
+        ("x", ctypes.c_void_p), ("weight", ctypes.c_void_p), ("bias", ctypes.c_void_p),
+        ("residual", ctypes.c_void_p), ("y", ctypes.c_void_p), ("pre", ctypes.c_void_p),
+        ("m", ctypes.c_int64), ("n", ctypes.c_int64), ("k", ctypes.c_int64),
+        ("ldx", ctypes.c_int64), ("ldw", ctypes.c_int64), ("ldr", ctypes.c_int64), ("ldy", ctypes.c_int64),
+        ("type", ctypes.c_int),
+        ("bias_f32", ctypes.c_int), ("residual_f32", ctypes.c_int), ("y_f32", ctypes.c_int),
+        ("activation", ctypes.c_int),
+        ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_size_t),
+    ]
+
+
+class LinearChoice(ctypes.Structure):
+    """yolo_amd_linear_choice of include/yolo_amd.h."""
+    _fields_ = [("kernel", ctypes.c_int), ("bm", ctypes.c_int), ("bn", ctypes.c_int), ("k_slices", ctypes.c_int),
+                ("copies_x", ctypes.c_int), ("copies_weight", ctypes.c_int)]
+
+
+class LinearBackwardDesc(ctypes.Structure):
+    """yolo_amd_linear_backward_desc of include/yolo_amd.h."""
+    _fields_ = [
+        ("dy", ctypes.c_void_p), ("x", ctypes.c_void_p), ("weight", ctypes.c_void_p), ("pre", ctypes.c_void_p),
+        ("dx", ctypes.c_void_p), ("dweight", ctypes.c_void_p), ("dbias", ctypes.c_void_p),
+        ("m", ctypes.c_int64), ("n", ctypes.c_int64), ("k", ctypes.c_int64),
+        ("lddy", ctypes.c_int64), ("ldx", ctypes.c_int64), ("ldw", ctypes.c_int64),
+        ("type", ctypes.c_int), ("dy_f32", ctypes.c_int), ("dbias_f32", ctypes.c_int), ("activation", ctypes.c_int),
+        ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_size_t),
+    ]
+
+
+class BlockNormDesc(ctypes.Structure):
+    """yolo_amd_block_norm_desc of include/yolo_amd.h."""
+    _fields_ = [
+        ("x", ctypes.c_void_p), ("residual", ctypes.c_void_p), ("gate", ctypes.c_void_p),
+        ("after_weight", ctypes.c_void_p), ("after_bias", ctypes.c_void_p),
+        ("before_weight", ctypes.c_void_p), ("before_bias", ctypes.c_void_p),
+        ("stream", ctypes.c_void_p), ("normed", ctypes.c_void_p),
+        ("rows", ctypes.c_int64), ("d", ctypes.c_int64), ("ldx", ctypes.c_int64), ("ldr", ctypes.c_int64),
+        ("rows_per_gate", ctypes.c_int64),
+        ("type", ctypes.c_int), ("norm", ctypes.c_int), ("after", ctypes.c_int), ("before", ctypes.c_int),
+        ("stream_f32", ctypes.c_int), ("gate_f32", ctypes.c_int), ("after_f32", ctypes.c_int),
+        ("before_f32", ctypes.c_int),
+        ("eps", ctypes.c_float), ("scale", ctypes.c_float),
+    ]
+
+
+class BlockNormBackwardDesc(ctypes.Structure):
+    """yolo_amd_block_norm_backward_desc of include/yolo_amd.h."""
+    _fields_ = [
+        ("forward", BlockNormDesc),
+        ("dnormed", ctypes.c_void_p), ("dstream", ctypes.c_void_p), ("dx", ctypes.c_void_p),
+        ("dresidual", ctypes.c_void_p), ("dgate", ctypes.c_void_p), ("dafter_weight", ctypes.c_void_p),
+        ("dafter_bias", ctypes.c_void_p), ("dbefore_weight", ctypes.c_void_p), ("dbefore_bias", ctypes.c_void_p),
+        ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_size_t),
+    ]
+
+
 # name -> (restype, argtypes); every symbol include/yolo_amd.h declares
 SYMBOLS = {
     "yolo_amd_last_error": (ctypes.c_char_p, []),
@@ -131,6 +196,14 @@ SYMBOLS = {
     "yolo_amd_conv_query": (ctypes.c_int, [ctypes.POINTER(ConvDesc), ctypes.POINTER(ConvChoice)]),
     "yolo_amd_conv_forward": (ctypes.c_int, [ctypes.POINTER(ConvDesc), ctypes.c_int,
                                               ctypes.c_void_p, ctypes.c_void_p]),
+    "yolo_amd_linear_workspace_bytes": (ctypes.c_size_t, [ctypes.POINTER(LinearDesc)]),
+    "yolo_amd_linear_forward": (ctypes.c_int, [ctypes.POINTER(LinearDesc), ctypes.c_void_p]),
+    "yolo_amd_linear_query": (ctypes.c_int, [ctypes.POINTER(LinearDesc), ctypes.POINTER(LinearChoice)]),
+    "yolo_amd_linear_backward_workspace_bytes": (ctypes.c_size_t, [ctypes.POINTER(LinearBackwardDesc)]),
+    "yolo_amd_linear_backward": (ctypes.c_int, [ctypes.POINTER(LinearBackwardDesc), ctypes.c_void_p]),
+    "yolo_amd_block_norm_forward": (ctypes.c_int, [ctypes.POINTER(BlockNormDesc), ctypes.c_void_p]),
+    "yolo_amd_block_norm_backward_workspace_bytes": (ctypes.c_size_t, [ctypes.POINTER(BlockNormBackwardDesc)]),
+    "yolo_amd_block_norm_backward": (ctypes.c_int, [ctypes.POINTER(BlockNormBackwardDesc), ctypes.c_void_p]),
 }
 
 

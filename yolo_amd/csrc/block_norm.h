@@ -1,0 +1,477 @@
+// Norms after and before a block, fused with the block's gate, residual scale and residual add; forward and
+// backward, for gfx950.  Per row of D values:
+//
+//   p = after ? norm(u) * wa + ba : u        norm(v) = v / sqrt(mean(v^2) + eps)                  (rms)
+//   h = r + s * g * p                                  (v - mean(v)) / sqrt(var(v) + eps)         (layer)
+//   y = norm(h) * wb + bb
+//
+//   q  = dy * wb;  dH = dh + f_h (q - [mean(q)] - h^ mean(q h^))       h^ = norm(h), f_h its factor
+//   dr = dH;  dg = s p dH (summed over the rows that share the gate);  dp = s g dH
+//   q' = dp * wa;  du = after ? f_u (q' - [mean(q')] - u^ mean(q' u^)) : dp
+//   dwb = sum dy h^;  dbb = sum dy;  dwa = sum dp u^;  dba = sum dp    over all rows
+//
+// Memory bound: a row is read once, held in registers (a group of TPR threads, 8 * CH values each) through
+// every statistic, and written once.  The backward kernel recomputes p and h from u and r instead of reading a
+// stored h: the same bytes, and no rounding of h enters the gradients.  Statistics and sums are fp32; a variance
+// is taken around its mean in a second sweep over the registers.
+#pragma once
+#include <algorithm>
+
+#include "common.h"
+#include "../../include/yolo_amd.h"
+
+namespace yolo_amd {
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+
+struct NormArgs {
+    const void *x, *res, *gate, *aw, *ab, *bw, *bb;
+    long long ldx, ldr;
+    void *h, *y;
+    long long rows;
+    int D;
+    int gate_f32, after_f32, before_f32;
+    long long rows_per_gate;       // rows that share a row of the gate
+    int after, before, layer;
+    float eps, scale, inv_d;
+    // backward
+    const void *dy, *dh;
+    void *dx, *dres, *dgate;       // dgate here: a gate row per token, written directly
+    float* part;                   // [block][vector][D] column sums of this launch's blocks
+    int vectors;                   // vectors per block, in the order wb, wa, gate, bb, ba (those that are wanted)
+    int at_wb, at_wa, at_g, at_bb, at_ba;   // position among them, or -1
+    // rows are walked as `sequences` runs of `length` rows; block (i, c): runs i * seq_per_block .., chunk c of `chunks`
+    long long sequences, length, chunk_rows;
+    int seq_per_block, chunks;
+    float* gate_part;              // [sequence][chunk][D]: gate sums where a run of rows shares a gate row
+};
+
+// 8 consecutive values, 16-byte aligned
+__device__ __forceinline__ void get8(const float* p, float* v) {
+    const f32x4 a = *reinterpret_cast<const f32x4*>(p), b = *reinterpret_cast<const f32x4*>(p + 4);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) { v[i] = a[i]; v[4 + i] = b[i]; }
+}
+template <typename T>
+__device__ __forceinline__ void get8(const T* p, float* v) {
+    typedef T t8 __attribute__((ext_vector_type(8)));
+    const t8 a = *reinterpret_cast<const t8*>(p);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = (float)a[i];
+}
+__device__ __forceinline__ void put8(float* p, const float* v) {
+    f32x4 a, b;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) { a[i] = v[i]; b[i] = v[4 + i]; }
+    *reinterpret_cast<f32x4*>(p) = a;
+    *reinterpret_cast<f32x4*>(p + 4) = b;
+}
+template <typename T>
+__device__ __forceinline__ void put8(T* p, const float* v) {
+    typedef T t8 __attribute__((ext_vector_type(8)));
+    t8 a;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) a[i] = (T)v[i];
+    *reinterpret_cast<t8*>(p) = a;
+}
+
+// The columns thread t of a group owns: with VEC runs of 8 (D % 8 == 0, rows 16-byte aligned), else single
+// columns TPR apart, which keeps element-wise accesses coalesced.
+template <int TPR, int CH, bool VEC>
+struct Cols {
+    static constexpr int E = CH * 8;
+    __device__ static __forceinline__ int col(int t, int e) { return VEC ? ((e >> 3) * TPR + t) * 8 + (e & 7) : e * TPR + t; }
+    // columns past D read as 0 (from an address inside the row)
+    template <typename S>
+    __device__ static __forceinline__ void load(const S* row, int D, int t, float (&v)[E]) {
+        if constexpr (VEC) {
+#pragma unroll
+            for (int c = 0; c < CH; ++c) {
+                const int at = (c * TPR + t) * 8;
+                get8(row + min(at, D - 8), v + c * 8);
+                if (at >= D) {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) v[c * 8 + i] = 0.f;
+                }
+            }
+        } else {
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+                const int at = e * TPR + t;
+                const float x = (float)row[min(at, D - 1)];
+                v[e] = at < D ? x : 0.f;
+            }
+        }
+    }
+    template <typename S>
+    __device__ static __forceinline__ void store(S* row, int D, int t, const float (&v)[E]) {
+        if constexpr (VEC) {
+#pragma unroll
+            for (int c = 0; c < CH; ++c) {
+                const int at = (c * TPR + t) * 8;
+                if (at < D) put8(row + at, v + c * 8);
+            }
+        } else {
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+                const int at = e * TPR + t;
+                if (at < D) row[at] = (S)v[e];
+            }
+        }
+    }
+    // a parameter vector, fp32 or T
+    template <typename T>
+    __device__ static __forceinline__ void param(const void* p, int f32, long long at, int D, int t, float (&v)[E]) {
+        if (f32) load((const float*)p + at, D, t, v);
+        else load((const T*)p + at, D, t, v);
+    }
+};
+
+// sum over the 64 lanes, the same bits in every lane
+__device__ __forceinline__ float wave_sum(float v) {
+    // lanes 1, 2 (quad_perm), 4 (row_half_mirror) and 8 (row_mirror) apart, then the four rows of 16
+#define YA_DPP_ADD(ctrl) v += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), ctrl, 0xF, 0xF, true))
+    YA_DPP_ADD(0xB1);
+    YA_DPP_ADD(0x4E);
+    YA_DPP_ADD(0x141);
+    YA_DPP_ADD(0x140);
+#undef YA_DPP_ADD
+    const int b = __float_as_int(v);
+    return (__int_as_float(__builtin_amdgcn_readlane(b, 0)) + __int_as_float(__builtin_amdgcn_readlane(b, 16))) +
+           (__int_as_float(__builtin_amdgcn_readlane(b, 32)) + __int_as_float(__builtin_amdgcn_readlane(b, 48)));
+}
+
+// Sums over a group of TPR threads; every thread of the workgroup makes the same calls.  Two slot sets in turn:
+// a set is written again only after the barrier of the call in between, which its readers reach after reading.
+template <int TPR, int NT>
+struct GroupSum {
+    float (*slots)[2][NT / 64];
+    int parity;
+    __device__ __forceinline__ void two(float& a, float& b) {
+        a = wave_sum(a);
+        b = wave_sum(b);
+        if constexpr (TPR > 64) {
+            const int w = threadIdx.x >> 6;
+            if ((threadIdx.x & 63) == 0) {
+                slots[parity][0][w] = a;
+                slots[parity][1][w] = b;
+            }
+            __syncthreads();
+            const int w0 = w / (TPR / 64) * (TPR / 64);
+            a = slots[parity][0][w0];
+            b = slots[parity][1][w0];
+#pragma unroll
+            for (int i = 1; i < TPR / 64; ++i) {
+                a += slots[parity][0][w0 + i];
+                b += slots[parity][1][w0 + i];
+            }
+            parity ^= 1;
+        }
+    }
+    __device__ __forceinline__ float one(float a) {
+        a = wave_sum(a);
+        if constexpr (TPR > 64) {
+            const int w = threadIdx.x >> 6;
+            if ((threadIdx.x & 63) == 0) slots[parity][0][w] = a;
+            __syncthreads();
+            const int w0 = w / (TPR / 64) * (TPR / 64);
+            a = slots[parity][0][w0];
+#pragma unroll
+            for (int i = 1; i < TPR / 64; ++i) a += slots[parity][0][w0 + i];
+            parity ^= 1;
+        }
+        return a;
+    }
+};
+
+// mean (0 for rms) and factor of a row; columns past D hold 0
+template <typename C, typename G>
+__device__ __forceinline__ void row_stats(const float (&v)[C::E], const NormArgs& a, int t, G& sum, float& mean, float& f) {
+    mean = 0.f;
+    if (a.layer) {
+        float s = 0.f;
+#pragma unroll
+        for (int e = 0; e < C::E; ++e) s += v[e];
+        mean = sum.one(s) * a.inv_d;
+    }
+    float q = 0.f;
+#pragma unroll
+    for (int e = 0; e < C::E; ++e) {
+        const float d = C::col(t, e) < a.D ? v[e] - mean : 0.f;
+        q = fmaf(d, d, q);
+    }
+    f = rsqrtf(sum.one(q) * a.inv_d + a.eps);
+}
+
+template <typename T, typename R, int TPR, int CH, bool VEC>
+__global__ void __launch_bounds__(TPR < 256 ? 256 : TPR)
+block_norm_forward_kernel(const NormArgs a) {
+    constexpr int NT = TPR < 256 ? 256 : TPR, GROUPS = NT / TPR, E = CH * 8;
+    typedef Cols<TPR, CH, VEC> C;
+    __shared__ float slots[2][2][NT / 64];
+    GroupSum<TPR, NT> sum{slots, 0};
+    const int t = threadIdx.x % TPR, group = threadIdx.x / TPR;
+    for (long long base = (long long)blockIdx.x * GROUPS; base < a.rows; base += (long long)gridDim.x * GROUPS) {
+        const bool valid = base + group < a.rows;
+        const long long row = valid ? base + group : a.rows - 1;
+        float u[E], h[E], w[E];
+        C::load((const T*)a.x + row * a.ldx, a.D, t, u);
+        if (a.res) C::load((const R*)a.res + row * a.ldr, a.D, t, h);
+        if (a.after) {
+            float mean, f;
+            row_stats<C>(u, a, t, sum, mean, f);
+#pragma unroll
+            for (int e = 0; e < E; ++e) u[e] = C::col(t, e) < a.D ? (u[e] - mean) * f : 0.f;
+            if (a.aw) {
+                C::template param<T>(a.aw, a.after_f32, 0, a.D, t, w);
+#pragma unroll
+                for (int e = 0; e < E; ++e) u[e] *= w[e];
+            }
+            if (a.ab) {
+                C::template param<T>(a.ab, a.after_f32, 0, a.D, t, w);
+#pragma unroll
+                for (int e = 0; e < E; ++e) u[e] += w[e];
+            }
+        }
+        if (a.gate) {
+            C::template param<T>(a.gate, a.gate_f32, row / a.rows_per_gate * a.D, a.D, t, w);
+#pragma unroll
+            for (int e = 0; e < E; ++e) u[e] *= w[e];
+        }
+        if (a.res) {
+#pragma unroll
+            for (int e = 0; e < E; ++e) h[e] = fmaf(a.scale, u[e], h[e]);
+        } else {
+#pragma unroll
+            for (int e = 0; e < E; ++e) h[e] = a.scale * u[e];
+        }
+        if (a.h && valid) C::store((R*)a.h + row * a.D, a.D, t, h);
+        if (a.before) {
+            float mean, f;
+            row_stats<C>(h, a, t, sum, mean, f);
+#pragma unroll
+            for (int e = 0; e < E; ++e) h[e] = (h[e] - mean) * f;
+            if (a.bw) {
+                C::template param<T>(a.bw, a.before_f32, 0, a.D, t, w);
+#pragma unroll
+                for (int e = 0; e < E; ++e) h[e] *= w[e];
+            }
+            if (a.bb) {
+                C::template param<T>(a.bb, a.before_f32, 0, a.D, t, w);
+#pragma unroll
+                for (int e = 0; e < E; ++e) h[e] += w[e];
+            }
+            if (valid) C::store((T*)a.y + row * a.D, a.D, t, h);
+        }
+    }
+}
+
+// Adds the column sums v of a workgroup's groups in group order and writes them to out[0 .. D).
+template <typename C, int TPR, int GROUPS>
+__device__ __forceinline__ void write_sums(float* lds, const float (&v)[C::E], int t, int group, int D, float* out) {
+    if constexpr (GROUPS == 1) {
+#pragma unroll
+        for (int e = 0; e < C::E; ++e)
+            if (C::col(t, e) < D) out[C::col(t, e)] = v[e];
+    } else {
+        // [group][e][t]: conflict free both ways
+        __syncthreads();
+#pragma unroll
+        for (int e = 0; e < C::E; ++e) lds[(group * C::E + e) * TPR + t] = v[e];
+        __syncthreads();
+        for (int i = threadIdx.x; i < C::E * TPR; i += GROUPS * TPR) {
+            float s = lds[i];
+#pragma unroll
+            for (int g = 1; g < GROUPS; ++g) s += lds[g * C::E * TPR + i];
+            const int c = C::col(i % TPR, i / TPR);
+            if (c < D) out[c] = s;
+        }
+    }
+}
+
+template <typename T, typename R, int TPR, int CH, bool VEC, bool LAYER>
+__global__ void __launch_bounds__(TPR < 512 ? 512 : TPR)
+block_norm_backward_kernel(const NormArgs a) {
+    constexpr int NT = TPR < 512 ? 512 : TPR, GROUPS = NT / TPR, E = CH * 8;
+    typedef Cols<TPR, CH, VEC> C;
+    __shared__ float slots[2][2][NT / 64];
+    __shared__ float lds[GROUPS > 1 ? GROUPS * E * TPR : 1];
+    GroupSum<TPR, NT> sum{slots, 0};
+    const int t = threadIdx.x % TPR, group = threadIdx.x / TPR;
+    const int chunk = blockIdx.x % a.chunks;
+    const long long s0 = (long long)(blockIdx.x / a.chunks) * a.seq_per_block;
+    const long long s1 = min(a.sequences, s0 + a.seq_per_block);
+    float wb[E], wa[E], wg[E], bb[E], ba[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) wb[e] = wa[e] = wg[e] = bb[e] = ba[e] = 0.f;
+    for (long long seq = s0; seq < s1; ++seq) {
+        const long long r0 = seq * a.length + chunk * a.chunk_rows;
+        const long long r1 = min(seq * a.length + a.length, r0 + a.chunk_rows);
+        for (long long base = r0; base < r1; base += GROUPS) {
+            const bool valid = base + group < r1;
+            const long long row = valid ? base + group : r1 - 1;
+            float u[E], h[E], d[E], dy[E], w[E];
+            C::load((const T*)a.x + row * a.ldx, a.D, t, u);
+            if (a.res) C::load((const R*)a.res + row * a.ldr, a.D, t, h);
+            if (a.dy) C::load((const T*)a.dy + row * a.D, a.D, t, dy);
+            if (a.dh) C::load((const R*)a.dh + row * a.D, a.D, t, d);
+            if (!a.res) {
+#pragma unroll
+                for (int e = 0; e < E; ++e) h[e] = 0.f;
+            }
+            if (!a.dh) {
+#pragma unroll
+                for (int e = 0; e < E; ++e) d[e] = 0.f;
+            }
+            // forward again: u becomes u^ (its norm without weights), h the stream
+            float fu = 1.f;
+            if (a.after) {
+                float mean;
+                row_stats<C>(u, a, t, sum, mean, fu);
+#pragma unroll
+                for (int e = 0; e < E; ++e) u[e] = C::col(t, e) < a.D ? (u[e] - mean) * fu : 0.f;
+            }
+            float p[E];
+#pragma unroll
+            for (int e = 0; e < E; ++e) p[e] = u[e];
+            if (a.aw) {
+                C::template param<T>(a.aw, a.after_f32, 0, a.D, t, w);
+#pragma unroll
+                for (int e = 0; e < E; ++e) p[e] *= w[e];
+            }
+            if (a.ab) {
+                C::template param<T>(a.ab, a.after_f32, 0, a.D, t, w);
+#pragma unroll
+                for (int e = 0; e < E; ++e) p[e] += w[e];
+            }
+            float g[E];
+            if (a.gate) {
+                C::template param<T>(a.gate, a.gate_f32, row / a.rows_per_gate * a.D, a.D, t, g);
+            } else {
+#pragma unroll
+                for (int e = 0; e < E; ++e) g[e] = 1.f;
+            }
+            if (a.dy) {
+                float mean, f;
+#pragma unroll
+                for (int e = 0; e < E; ++e) h[e] = fmaf(a.scale, g[e] * p[e], h[e]);
+                row_stats<C>(h, a, t, sum, mean, f);
+#pragma unroll
+                for (int e = 0; e < E; ++e) h[e] = C::col(t, e) < a.D ? (h[e] - mean) * f : 0.f;
+                if (valid) {
+#pragma unroll
+                    for (int e = 0; e < E; ++e) {
+                        wb[e] = fmaf(dy[e], h[e], wb[e]);
+                        if (LAYER) bb[e] += dy[e];
+                    }
+                }
+                if (a.bw) {
+                    C::template param<T>(a.bw, a.before_f32, 0, a.D, t, w);
+#pragma unroll
+                    for (int e = 0; e < E; ++e) dy[e] *= w[e];
+                }
+                float c0 = 0.f, c1 = 0.f;
+#pragma unroll
+                for (int e = 0; e < E; ++e) {
+                    c0 += dy[e];
+                    c1 = fmaf(dy[e], h[e], c1);
+                }
+                if (LAYER) sum.two(c0, c1);
+                else { c1 = sum.one(c1); c0 = 0.f; }
+                c0 *= a.inv_d;
+                c1 *= a.inv_d;
+#pragma unroll
+                for (int e = 0; e < E; ++e) d[e] += f * (dy[e] - c0 - h[e] * c1);
+            }
+            if (a.dres && valid) C::store((R*)a.dres + row * a.D, a.D, t, d);
+            // gate
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+                p[e] *= a.scale * d[e];
+                d[e] *= a.scale * g[e];
+            }
+            if (a.dgate && valid) {
+                if (a.gate_f32) C::store((float*)a.dgate + row * a.D, a.D, t, p);
+                else C::store((T*)a.dgate + row * a.D, a.D, t, p);
+            }
+            if (valid) {
+#pragma unroll
+                for (int e = 0; e < E; ++e) {
+                    if (C::col(t, e) < a.D) wg[e] += p[e];
+                    wa[e] = fmaf(d[e], u[e], wa[e]);
+                    if (LAYER) ba[e] += d[e];
+                }
+            }
+            if (a.after && a.dx) {
+                if (a.aw) {
+                    C::template param<T>(a.aw, a.after_f32, 0, a.D, t, w);
+#pragma unroll
+                    for (int e = 0; e < E; ++e) d[e] *= w[e];
+                }
+                float c0 = 0.f, c1 = 0.f;
+#pragma unroll
+                for (int e = 0; e < E; ++e) {
+                    c0 += C::col(t, e) < a.D ? d[e] : 0.f;
+                    c1 = fmaf(d[e], u[e], c1);
+                }
+                if (LAYER) sum.two(c0, c1);
+                else { c1 = sum.one(c1); c0 = 0.f; }
+                c0 *= a.inv_d;
+                c1 *= a.inv_d;
+#pragma unroll
+                for (int e = 0; e < E; ++e) d[e] = fu * (d[e] - c0 - u[e] * c1);
+            }
+            if (a.dx && valid) C::store((T*)a.dx + row * a.D, a.D, t, d);
+        }
+        if (a.gate_part) {
+            write_sums<C, TPR, GROUPS>(lds, wg, t, group, a.D, a.gate_part + (seq * a.chunks + chunk) * a.D);
+#pragma unroll
+            for (int e = 0; e < E; ++e) wg[e] = 0.f;
+        }
+    }
+    float* out = a.part + (long long)blockIdx.x * a.vectors * a.D;
+    if (a.at_wb >= 0) write_sums<C, TPR, GROUPS>(lds, wb, t, group, a.D, out + (long long)a.at_wb * a.D);
+    if (a.at_wa >= 0) write_sums<C, TPR, GROUPS>(lds, wa, t, group, a.D, out + (long long)a.at_wa * a.D);
+    if (a.at_g >= 0) write_sums<C, TPR, GROUPS>(lds, wg, t, group, a.D, out + (long long)a.at_g * a.D);
+    if (LAYER && a.at_bb >= 0) write_sums<C, TPR, GROUPS>(lds, bb, t, group, a.D, out + (long long)a.at_bb * a.D);
+    if (LAYER && a.at_ba >= 0) write_sums<C, TPR, GROUPS>(lds, ba, t, group, a.D, out + (long long)a.at_ba * a.D);
+}
+
+// ---------------------------------------------------------------- launch, one translation unit per element type
+// Groups by row length: up to 16 values per thread, so that the backward kernel's row (four tensors) and its
+// column sums (up to five) stay in registers.
+template <typename T, typename R, bool VEC, int TPR, int CH>
+static void norm_launch_shape(const NormArgs& a, int blocks, bool backward, hipStream_t s) {
+    if (!backward) {
+        constexpr int NT = TPR < 256 ? 256 : TPR;
+        hipLaunchKernelGGL((block_norm_forward_kernel<T, R, TPR, CH, VEC>), dim3(blocks), dim3(NT), 0, s, a);
+    } else {
+        constexpr int NT = TPR < 512 ? 512 : TPR;
+        if (a.layer) hipLaunchKernelGGL((block_norm_backward_kernel<T, R, TPR, CH, VEC, true>), dim3(blocks), dim3(NT), 0, s, a);
+        else hipLaunchKernelGGL((block_norm_backward_kernel<T, R, TPR, CH, VEC, false>), dim3(blocks), dim3(NT), 0, s, a);
+    }
+}
+
+static inline int norm_tpr(int D) { return D <= 1024 ? 64 : D <= 2048 ? 128 : D <= 4096 ? 256 : D <= 8192 ? 512 : 1024; }
+
+template <typename T, typename R, bool VEC>
+static void norm_launch_width(const NormArgs& a, int blocks, bool backward, hipStream_t s) {
+    if (a.D <= 512) norm_launch_shape<T, R, VEC, 64, 1>(a, blocks, backward, s);
+    else if (a.D <= 1024) norm_launch_shape<T, R, VEC, 64, 2>(a, blocks, backward, s);
+    else if (a.D <= 2048) norm_launch_shape<T, R, VEC, 128, 2>(a, blocks, backward, s);
+    else if (a.D <= 4096) norm_launch_shape<T, R, VEC, 256, 2>(a, blocks, backward, s);
+    else if (a.D <= 8192) norm_launch_shape<T, R, VEC, 512, 2>(a, blocks, backward, s);
+    else norm_launch_shape<T, R, VEC, 1024, 2>(a, blocks, backward, s);
+}
+
+template <typename T, typename R>
+static void norm_launch(const NormArgs& a, bool vec, int blocks, bool backward, hipStream_t s) {
+    if (vec) norm_launch_width<T, R, true>(a, blocks, backward, s);
+    else norm_launch_width<T, R, false>(a, blocks, backward, s);
+}
+
+void block_norm_launch_bf16(const NormArgs& a, bool stream_f32, bool vec, int blocks, bool backward, hipStream_t s);
+void block_norm_launch_f16(const NormArgs& a, bool stream_f32, bool vec, int blocks, bool backward, hipStream_t s);
+void block_norm_launch_f32(const NormArgs& a, bool vec, int blocks, bool backward, hipStream_t s);
+
+}  // namespace yolo_amd

@@ -39,6 +39,13 @@ void set_error(const char* fmt, ...);
         }                                          \
     } while (0)
 
+// hand an error code of another checked function on
+#define YA_TRY(expr)                     \
+    do {                                 \
+        const int _rc = (expr);          \
+        if (_rc != yolo_amd::YA_OK) return _rc;    \
+    } while (0)
+
 static inline size_t align_up(size_t x, size_t a) { return (x + a - 1) / a * a; }
 
 static inline uint32_t next_pow2(uint32_t x) {

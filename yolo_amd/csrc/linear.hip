@@ -1,0 +1,902 @@
+// Matrix product with bias, activation and residual in its epilogue, and its gradients, for gfx950.
+//
+//   P = x W^T + b          x [M][K], W [N][K], bf16 or fp16, fp32 accumulation on the matrix units
+//   Y = act(P) + r
+//   dP = dY * act'(P);  dX = dP W;  dW = dP^T x;  db = sum over rows of dP;  dr = dY
+//
+// All three products are D[m][n] = sum_k A(m, k) B(n, k) with operands that are contiguous either along k
+// (x and W in the forward product) or along their own rows' index (W in dX, dP and x in dW): one tile kernel
+// takes both, the second kind through the transposing LDS read (ds_read_b64_tr_b16).
+#include <algorithm>
+
+#include "common.h"
+#include "lds_dma.h"
+#include "../../include/yolo_amd.h"
+
+namespace yolo_amd {
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+template <typename T> struct Vec;
+template <> struct Vec<__bf16> { typedef __bf16 v8 __attribute__((ext_vector_type(8))); };
+template <> struct Vec<_Float16> { typedef _Float16 v8 __attribute__((ext_vector_type(8))); };
+template <typename T> using v8 = typename Vec<T>::v8;
+
+__device__ __forceinline__ f32x4 mfma(v8<__bf16> a, v8<__bf16> b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x4 mfma(v8<_Float16> a, v8<_Float16> b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+}
+
+// ---------------------------------------------------------------- activations
+constexpr float kGeluC = 0.7978845608028654f, kGeluA = 0.044715f, kRsqrt2 = 0.7071067811865476f;
+constexpr float kRsqrt2Pi = 0.3989422804014327f;
+
+// 1 / (1 + exp(-x)); exp overflows to +inf for x < -88 and the reciprocal is then 0, as it should be
+__device__ __forceinline__ float sigmoid(float x) { return sigmoid_fast(x); }
+
+__device__ __forceinline__ float act_value(float p, int act) {
+    switch (act) {
+        case YOLO_AMD_ACT_LEAKY: return p > 0.f ? p : 0.1f * p;
+        case YOLO_AMD_ACT_RELU: return p > 0.f ? p : (p != p ? p : 0.f);
+        case YOLO_AMD_ACT_GELU: return 0.5f * p * (1.f + erff(p * kRsqrt2));
+        // 0.5 (1 + tanh z) = sigmoid(2 z)
+        case YOLO_AMD_ACT_GELU_TANH: return p * sigmoid(2.f * kGeluC * (p + kGeluA * p * p * p));
+        case YOLO_AMD_ACT_SILU: return p * sigmoid(p);
+        default: return p;
+    }
+}
+
+__device__ __forceinline__ float act_slope(float p, int act) {
+    switch (act) {
+        case YOLO_AMD_ACT_LEAKY: return p > 0.f ? 1.f : 0.1f;
+        case YOLO_AMD_ACT_RELU: return p > 0.f ? 1.f : 0.f;
+        case YOLO_AMD_ACT_GELU:
+            return 0.5f * (1.f + erff(p * kRsqrt2)) + p * kRsqrt2Pi * exp_fast(-0.5f * p * p);
+        case YOLO_AMD_ACT_GELU_TANH: {
+            const float z = sigmoid(2.f * kGeluC * (p + kGeluA * p * p * p));
+            return z + p * z * (1.f - z) * 2.f * kGeluC * (1.f + 3.f * kGeluA * p * p);
+        }
+        case YOLO_AMD_ACT_SILU: {
+            const float z = sigmoid(p);
+            return z * (1.f + p * (1.f - z));
+        }
+        default: return 1.f;
+    }
+}
+
+// ---------------------------------------------------------------- epilogue
+struct Epilogue {
+    const void* bias;      // [N] or null
+    const void* res;       // [M][ldr] or null
+    void* y;               // [M][ldy]
+    void* pre;             // [M][ldp] or null: P, rounded to T, for the backward pass
+    long long ldr, ldy, ldp;
+    int bias_f32, res_f32, y_f32, act;
+    int vec;               // every row of every tensor above starts on a 16-byte boundary and N % 8 == 0
+    float* part;           // not null: the raw sums of one K slice go to [slice][M][ld_part] instead
+    long long ld_part, slice_stride;
+};
+
+template <typename T>
+__device__ __forceinline__ void load8(const void* p, long long at, int f32, float (&v)[8]) {
+    if (f32) {
+        const f32x4 a = *reinterpret_cast<const f32x4*>((const float*)p + at);
+        const f32x4 b = *reinterpret_cast<const f32x4*>((const float*)p + at + 4);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) { v[i] = a[i]; v[4 + i] = b[i]; }
+    } else {
+        const v8<T> a = *reinterpret_cast<const v8<T>*>((const T*)p + at);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = (float)a[i];
+    }
+}
+template <typename T>
+__device__ __forceinline__ void store8(void* p, long long at, int f32, const float (&v)[8]) {
+    if (f32) {
+        f32x4 a, b;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) { a[i] = v[i]; b[i] = v[4 + i]; }
+        *reinterpret_cast<f32x4*>((float*)p + at) = a;
+        *reinterpret_cast<f32x4*>((float*)p + at + 4) = b;
+    } else {
+        v8<T> a;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) a[i] = (T)v[i];
+        *reinterpret_cast<v8<T>*>((T*)p + at) = a;
+    }
+}
+template <typename T>
+__device__ __forceinline__ float load1(const void* p, long long at, int f32) {
+    return f32 ? ((const float*)p)[at] : (float)((const T*)p)[at];
+}
+template <typename T>
+__device__ __forceinline__ void store1(void* p, long long at, int f32, float v) {
+    if (f32) ((float*)p)[at] = v;
+    else ((T*)p)[at] = (T)v;
+}
+
+// Eight sums of row m, columns n .. n + 7 (n a multiple of 8, n < N): bias, activation, residual, one
+// rounding, store.
+template <typename T>
+__device__ __forceinline__ void finish8(const Epilogue& e, long long m, int n, int N, float (&v)[8]) {
+    if (e.vec) {
+        if (e.bias) {
+            float b[8];
+            load8<T>(e.bias, n, e.bias_f32, b);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] += b[i];
+        }
+        if (e.pre) store8<T>(e.pre, m * e.ldp + n, 0, v);
+        if (e.act) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = act_value(v[i], e.act);
+        }
+        if (e.res) {
+            float r[8];
+            load8<T>(e.res, m * e.ldr + n, e.res_f32, r);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] += r[i];
+        }
+        store8<T>(e.y, m * e.ldy + n, e.y_f32, v);
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        if (n + i < N) {
+            float s = v[i];
+            if (e.bias) s += load1<T>(e.bias, n + i, e.bias_f32);
+            if (e.pre) store1<T>(e.pre, m * e.ldp + n + i, 0, s);
+            s = act_value(s, e.act);
+            if (e.res) s += load1<T>(e.res, m * e.ldr + n + i, e.res_f32);
+            store1<T>(e.y, m * e.ldy + n + i, e.y_f32, s);
+        }
+    }
+}
+
+// ---------------------------------------------------------------- tile kernel
+struct TileArgs {
+    const void *A, *B;
+    long long lda, ldb;     // elements
+    int M, N, K;
+    int tiles_m, tiles_n;
+    int ksteps;             // K-steps of 64 per slice (blockIdx.y = slice)
+    Epilogue e;
+};
+
+constexpr int kBK = 64;
+constexpr uint32_t kBufferBytes = 0x80000000u;   // descriptor size: offsets built below stay under it
+
+// One operand's tile of R rows (its own index) x 64 reduction indices in LDS, filled by W waves.
+//   TR = false: contiguous along k in memory.  Image: R rows of 128 bytes, 16-byte chunk c of row r at
+//     position c ^ (r & 7): the 16 lanes of a fragment read then hit 8 different bank groups.
+//   TR = true: contiguous along R.  Image: 64 rows (k) of 2R bytes, 16-byte chunk c of row k at position
+//     c ^ 2 f(k), f(k) = (k & 3) | (k >> 3 & 1) << 2: the 32 lanes that one transposing read serves at a time
+//     (4 k-rows x 2 groups of 8 k apart, 32 bytes each) then cover all 64 banks once.
+// Rows past the operand's end and reduction indices past K are read as zero through the buffer
+// descriptor's range check, so no tile reads outside its matrix.
+template <int R, int W, bool TR>
+struct Operand {
+    static constexpr int NI = R / 8 / W;          // LDS-DMA instructions (1 KiB each) per wave and K-step
+    static constexpr int BYTES = R * kBK * 2;
+    uint32_t voff[NI];
+    int kfirst, kstride;                          // reduction index of this lane's first chunk, and per instruction
+    const char* base;                             // wave-uniform: this tile at the current K-step
+    long long step;                               // bytes from one K-step to the next
+
+    __device__ __forceinline__ void init(const void* p, long long ld, int row0, int extent, int kbeg, int lane, int w) {
+        if constexpr (!TR) {
+            const int r = lane >> 3, c = (lane & 7) ^ r;
+            kfirst = c * 8;
+            kstride = 0;
+#pragma unroll
+            for (int j = 0; j < NI; ++j) {
+                const int row = (j * W + w) * 8 + r;
+                voff[j] = row0 + row < extent ? (uint32_t)(row * (uint32_t)ld * 2u) + c * 16u : kBufferNowhere;
+            }
+            base = (const char*)p + ((long long)row0 * ld + kbeg) * 2;
+            step = kBK * 2;
+        } else {
+            constexpr int CPR = R / 8, RPI = 64 / CPR;     // chunks per row, rows per instruction
+            static_assert((W * RPI) % 16 == 0, "f(k) is the same for all of a lane's instructions");
+            const int k = w * RPI + lane / CPR;
+            const int f = (k & 3) | ((k >> 3 & 1) << 2);
+            const int c = (lane % CPR) ^ (f << 1);
+            kfirst = k;
+            kstride = W * RPI;
+#pragma unroll
+            for (int j = 0; j < NI; ++j)
+                voff[j] = row0 + c * 8 < extent ? (uint32_t)((k + j * W * RPI) * (uint32_t)ld * 2u) + c * 16u : kBufferNowhere;
+            base = (const char*)p + ((long long)kbeg * ld + row0) * 2;
+            step = kBK * ld * 2;
+        }
+    }
+    // issue the K-step at `base`, whose reduction indices below `left` are valid, and move on
+    __device__ __forceinline__ void issue(char* buf, int w, int left) {
+        const __amdgpu_buffer_rsrc_t rs =
+            __builtin_amdgcn_make_buffer_rsrc((void*)base, 0, (int)kBufferBytes, (int)kRawBufferWord3);
+#pragma unroll
+        for (int j = 0; j < NI; ++j) {
+            uint32_t v = voff[j];
+            if (left < kBK) v = kfirst + j * kstride < left ? v : kBufferNowhere;
+            lds_dma16_buf(rs, v, 0, buf + (j * W + w) * 1024);
+        }
+        base += step;
+    }
+};
+
+// fragment reads: 16 rows x 32 reduction indices; lane l holds row (l & 15), indices (l >> 4) * 8 ..
+template <typename T, int R, bool TR>
+struct Fragments {
+    uint32_t at0;
+    __device__ __forceinline__ void init(int row0, int lane) {
+        if constexpr (!TR) {
+            at0 = (row0 + (lane & 15)) * 128 + (((lane >> 4) ^ (lane & 7)) << 4);
+        } else {
+            const int g = lane >> 4, j = lane & 15;
+            const int f = (j >> 2) | ((g & 1) << 2);
+            at0 = (uint32_t)((g * 8 + (j >> 2)) * (R * 2) + (((row0 >> 4) ^ f) << 5) + ((j & 3) << 3));
+        }
+    }
+    __device__ __forceinline__ v8<T> get(const char* buf, int i, int s) const {
+        if constexpr (!TR) {
+            return *reinterpret_cast<const v8<T>*>(buf + ((at0 ^ (s << 6)) + i * 2048));
+        } else {
+            const char* p = buf + ((at0 ^ (i << 5)) + s * (32 * R * 2));
+            typedef __attribute__((address_space(3))) s16x4* lds_p;
+            union { s16x4 h[2]; v8<T> v; } u;
+            u.h[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_p)p);
+            u.h[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_p)(p + 4 * R * 2));
+            return u.v;
+        }
+    }
+};
+
+template <typename T, int BM, int BN, int WM, int WN, bool AT, bool BT>
+__global__ void __launch_bounds__(WM * WN * 64)
+linear_tile_kernel(const TileArgs a) {
+    constexpr int W = WM * WN, NT = W * 64;
+    constexpr int WTM = BM / WM, WTN = BN / WN, TM = WTM / 16, TN = WTN / 16;
+    typedef Operand<BM, W, AT> OpA;
+    typedef Operand<BN, W, BT> OpB;
+    constexpr int STAGE = OpA::BYTES + OpB::BYTES;
+    constexpr int CROWS = WM * 32, CLD = BN + 4;       // epilogue chunk: 32 rows per wave row, fp32
+    constexpr int LDS = 2 * STAGE > CROWS * CLD * 4 ? 2 * STAGE : CROWS * CLD * 4;
+    __shared__ __attribute__((aligned(1024))) char lds[LDS];
+
+    const int lane = threadIdx.x & 63;
+    const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wm = w % WM, wn = w / WM;
+    // XCD-aware order: the blocks of one XCD (blockIdx % 8) take a contiguous run of tiles, and a run walks
+    // groups of 8 tile rows column by column, so that the tiles an XCD works on at a time share rows and columns.
+    int tile_m, tile_n;
+    {
+        const int T_ = a.tiles_m * a.tiles_n, q = T_ >> 3, r = T_ & 7;
+        const int xcd = blockIdx.x & 7, loc = blockIdx.x >> 3;
+        const int t = (xcd < r ? xcd * (q + 1) : r * (q + 1) + (xcd - r) * q) + loc;
+        const int per = 8 * a.tiles_n, g = t / per, in = t - g * per;
+        const int gm = min(8, a.tiles_m - g * 8);
+        tile_n = in / gm;
+        tile_m = g * 8 + (in - tile_n * gm);
+    }
+    const int m0 = tile_m * BM, n0 = tile_n * BN;
+    const int kbeg = (int)blockIdx.y * a.ksteps * kBK;
+    const int kend = min(a.K, kbeg + a.ksteps * kBK);
+    const int nt = kend > kbeg ? (kend - kbeg + kBK - 1) / kBK : 0;
+
+    OpA opa;
+    OpB opb;
+    opa.init(a.A, a.lda, m0, a.M, kbeg, lane, w);
+    opb.init(a.B, a.ldb, n0, a.N, kbeg, lane, w);
+    Fragments<T, BM, AT> fa;
+    Fragments<T, BN, BT> fb;
+    fa.init(wm * WTM, lane);
+    fb.init(wn * WTN, lane);
+
+    f32x4 acc[TM][TN];
+#pragma unroll
+    for (int i = 0; i < TM; ++i)
+#pragma unroll
+        for (int j = 0; j < TN; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+
+    auto issue = [&](int t) {
+        char* buf = lds + (t & 1) * STAGE;
+        const int left = kend - kbeg - t * kBK;
+        opa.issue(buf, w, left);
+        opb.issue(buf + OpA::BYTES, w, left);
+    };
+    if (nt > 0) issue(0);
+    for (int t = 0; t < nt; ++t) {
+        // this wave's loads have landed and its reads of the other buffer have returned; then everybody's
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        if (t + 1 < nt) issue(t + 1);
+        const char* buf = lds + (t & 1) * STAGE;
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+            v8<T> av[TM], bv[TN];
+#pragma unroll
+            for (int j = 0; j < TN; ++j) bv[j] = fb.get(buf + OpA::BYTES, j, s);
+#pragma unroll
+            for (int i = 0; i < TM; ++i) av[i] = fa.get(buf, i, s);
+#pragma unroll
+            for (int i = 0; i < TM; ++i)
+#pragma unroll
+                for (int j = 0; j < TN; ++j) acc[i][j] = mfma(bv[j], av[i], acc[i][j]);
+        }
+    }
+
+    // The accumulators (lane: row l & 15, four columns (l >> 4) * 4 ..) go through LDS in fp32, 32 rows of every
+    // wave row at a time, so that every access to memory behind it is 16 bytes per lane and coalesced.
+    float* out = reinterpret_cast<float*>(lds);
+#pragma unroll
+    for (int c = 0; c < WTM / 32; ++c) {
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int j = 0; j < TN; ++j)
+                *reinterpret_cast<f32x4*>(out + (wm * 32 + i * 16 + (lane & 15)) * CLD + wn * WTN + j * 16 + (lane >> 4) * 4) =
+                    acc[c * 2 + i][j];
+        __syncthreads();
+        for (int it = threadIdx.x; it < CROWS * (BN / 8); it += NT) {
+            const int lr = it / (BN / 8), n = n0 + (it % (BN / 8)) * 8;
+            const long long m = m0 + (lr >> 5) * WTM + c * 32 + (lr & 31);
+            if (m < a.M && n < a.N) {
+                float v[8];
+                load8<T>(out, lr * CLD + (n - n0), 1, v);
+                if (a.e.part) store8<T>(a.e.part, blockIdx.y * a.e.slice_stride + m * a.e.ld_part + n, 1, v);
+                else finish8<T>(a.e, m, n, a.N, v);
+            }
+        }
+    }
+}
+
+// Adds the K slices in ascending order and finishes: one thread per eight columns.
+template <typename T>
+__global__ void __launch_bounds__(256)
+linear_finish_kernel(const Epilogue e, const float* part, int slices, int M, int N, int n8) {
+    const long long total = (long long)M * n8;
+    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < total; i += (long long)gridDim.x * 256) {
+        const long long m = i / n8;
+        const int n = (int)(i - m * n8) * 8;
+        float v[8];
+        load8<T>(part, m * e.ld_part + n, 1, v);
+        for (int s = 1; s < slices; ++s) {
+            float u[8];
+            load8<T>(part, s * e.slice_stride + m * e.ld_part + n, 1, u);
+#pragma unroll
+            for (int k = 0; k < 8; ++k) v[k] += u[k];
+        }
+        finish8<T>(e, m, n, N, v);
+    }
+}
+
+// ---------------------------------------------------------------- few rows
+// M <= 16 * MT rows of x: the product is a read of W.  A workgroup owns 16 * NT rows of W (columns of Y) and
+// its eight waves take 64 reduction indices each in turn, straight from memory into matrix-instruction fragments;
+// the eight partial sums meet in LDS in a fixed order.  No second launch, no atomics.
+template <typename T, int MT, int NT>
+__global__ void __launch_bounds__(512)
+linear_rows_kernel(const TileArgs a) {
+    __shared__ __attribute__((aligned(16))) f32x4 red[8][MT][NT][64];
+    const int lane = threadIdx.x & 63;
+    const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int n0 = blockIdx.x * (16 * NT);
+    const int kl = (lane >> 4) * 8;
+    const T* xp[MT];
+    const T* wp[NT];
+#pragma unroll
+    for (int i = 0; i < MT; ++i) xp[i] = (const T*)a.A + (long long)min(i * 16 + (lane & 15), a.M - 1) * a.lda + kl;
+#pragma unroll
+    for (int j = 0; j < NT; ++j) wp[j] = (const T*)a.B + (long long)min(n0 + j * 16 + (lane & 15), a.N - 1) * a.ldb + kl;
+    f32x4 acc[MT][NT];
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int j = 0; j < NT; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    int k = w * 64;
+#pragma unroll 4
+    for (; k + 64 <= a.K; k += 512) {
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+            v8<T> xv[MT], wv[NT];
+#pragma unroll
+            for (int j = 0; j < NT; ++j) wv[j] = *reinterpret_cast<const v8<T>*>(wp[j] + k + s * 32);
+#pragma unroll
+            for (int i = 0; i < MT; ++i) xv[i] = *reinterpret_cast<const v8<T>*>(xp[i] + k + s * 32);
+#pragma unroll
+            for (int i = 0; i < MT; ++i)
+#pragma unroll
+                for (int j = 0; j < NT; ++j) acc[i][j] = mfma(wv[j], xv[i], acc[i][j]);
+        }
+    }
+    if (k < a.K) {                                  // one wave has the last, partial step
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+            const bool in = k + s * 32 + kl < a.K;  // whole chunks: K is a multiple of 8
+            v8<T> xv[MT], wv[NT];
+#pragma unroll
+            for (int j = 0; j < NT; ++j) wv[j] = in ? *reinterpret_cast<const v8<T>*>(wp[j] + k + s * 32) : v8<T>{};
+#pragma unroll
+            for (int i = 0; i < MT; ++i) xv[i] = in ? *reinterpret_cast<const v8<T>*>(xp[i] + k + s * 32) : v8<T>{};
+#pragma unroll
+            for (int i = 0; i < MT; ++i)
+#pragma unroll
+                for (int j = 0; j < NT; ++j) acc[i][j] = mfma(wv[j], xv[i], acc[i][j]);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int j = 0; j < NT; ++j) red[w][i][j][lane] = acc[i][j];
+    __syncthreads();
+    for (int it = threadIdx.x; it < MT * 16 * NT * 2; it += 512) {
+        const int mr = it / (NT * 2), n8 = it % (NT * 2);
+        const int n = n0 + n8 * 8;
+        if (mr < a.M && n < a.N) {
+            const int l0 = (n8 & 1) * 32 + (mr & 15);
+            f32x4 lo = f32x4{0.f, 0.f, 0.f, 0.f}, hi = lo;
+#pragma unroll
+            for (int q = 0; q < 8; ++q) {
+                lo += red[q][mr >> 4][n8 >> 1][l0];
+                hi += red[q][mr >> 4][n8 >> 1][l0 + 16];
+            }
+            float v[8];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) { v[i] = lo[i]; v[4 + i] = hi[i]; }
+            finish8<T>(a.e, mr, n, a.N, v);
+        }
+    }
+}
+
+// ---------------------------------------------------------------- operand copies
+// Rows of C elements at any stride and alignment -> rows of C rounded up to 8, zero filled: what the kernels
+// above need (16-byte chunks that never straddle a row's end).  One thread per chunk.
+template <typename T>
+__global__ void __launch_bounds__(256)
+linear_pack_kernel(const T* src, long long ld, long long rows, int C, T* dst, int c8) {
+    const long long total = rows * c8;
+    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < total; i += (long long)gridDim.x * 256) {
+        const long long r = i / c8;
+        const int c = (int)(i - r * c8) * 8;
+        v8<T> v;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) v[k] = c + k < C ? src[r * ld + c + k] : (T)0.f;
+        *reinterpret_cast<v8<T>*>(dst + i * 8) = v;
+    }
+}
+
+// ---------------------------------------------------------------- backward: dP and the bias gradient
+struct DpreArgs {
+    const void *dy, *pre;
+    long long lddy, ldpre;
+    int dy_f32, act, vec;
+    void* dp;               // [M][ldp], zero filled past N; null: only the column sums are wanted
+    long long ldp;
+    float* part;            // [row block][N] column sums, or null
+    int M, N, rows;         // rows per block
+};
+
+// Thread = eight columns of a run of rows; column sums in fp32 over that run, added over the runs by
+// linear_dbias_kernel in ascending order.
+template <typename T>
+__global__ void __launch_bounds__(256)
+linear_dpre_kernel(const DpreArgs a) {
+    const int lane_c = threadIdx.x & 31, lane_r = threadIdx.x >> 5;      // 32 chunks x 8 rows
+    const int n = (blockIdx.x * 32 + lane_c) * 8;
+    __shared__ float red[8][32 * 8 + 1];
+    const long long r0 = (long long)blockIdx.y * a.rows;
+    const long long r1 = min((long long)a.M, r0 + a.rows);
+    float sum[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    if (n < a.N) {
+        for (long long m = r0 + lane_r; m < r1; m += 8) {
+            float d[8], p[8];
+            if (a.vec) {
+                load8<T>(a.dy, m * a.lddy + n, a.dy_f32, d);
+                if (a.pre) load8<T>(a.pre, m * a.ldpre + n, 0, p);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    d[i] = n + i < a.N ? load1<T>(a.dy, m * a.lddy + n + i, a.dy_f32) : 0.f;
+                    p[i] = a.pre && n + i < a.N ? load1<T>(a.pre, m * a.ldpre + n + i, 0) : 0.f;
+                }
+            }
+            if (a.pre) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) d[i] *= act_slope(p[i], a.act);
+            }
+            if (a.dp) store8<T>(a.dp, m * a.ldp + n, 0, d);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) sum[i] += d[i];
+        }
+    }
+    if (!a.part) return;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) red[lane_r][lane_c * 8 + i] = sum[i];
+    __syncthreads();
+    const int c = blockIdx.x * 256 + threadIdx.x;
+    if (c < a.N) {
+        float s = 0.f;
+#pragma unroll
+        for (int r = 0; r < 8; ++r) s += red[r][threadIdx.x];
+        a.part[(long long)blockIdx.y * a.N + c] = s;
+    }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(256)
+linear_dbias_kernel(const float* part, int blocks, int N, void* db, int db_f32) {
+    const int n = blockIdx.x * 256 + threadIdx.x;
+    if (n >= N) return;
+    float s = 0.f;
+    for (int b = 0; b < blocks; ++b) s += part[(long long)b * N + n];
+    store1<T>(db, n, db_f32, s);
+}
+
+// ---------------------------------------------------------------- host side
+struct Matrix {
+    const void* p;
+    long long ld;
+    long long rows;
+    int cols;
+};
+
+static bool packed_ok(const Matrix& m) {
+    return ((uintptr_t)m.p & 15) == 0 && m.cols % 8 == 0 && (m.ld % 8 == 0 || m.rows <= 1);
+}
+static size_t packed_bytes(const Matrix& m) {
+    return packed_ok(m) ? 0 : align_up((size_t)m.rows * align_up(m.cols, 8) * 2, 256);
+}
+
+// Which kernel a product D[M][N] over K runs on.
+struct TilePlan {
+    int kernel, bm, bn, slices, ksteps;
+};
+
+static TilePlan plan_product(long long M, int N, long long K, bool kc_operands) {
+    TilePlan p{};
+    const long long steps = std::max<long long>(1, (K + kBK - 1) / kBK);
+    if (kc_operands && M <= 32) {
+        p.kernel = YOLO_AMD_LINEAR_ROWS;
+        p.bm = M <= 16 ? 16 : 32;
+        p.bn = N >= 16384 ? 32 : 16;
+        p.slices = 1;
+        p.ksteps = (int)steps;
+        return p;
+    }
+    double best = 0;
+    for (int cfg = 0; cfg < 2; ++cfg) {
+        const int bt = cfg ? 128 : 256;
+        const long long tiles = ((M + bt - 1) / bt) * ((N + bt - 1) / bt);
+        const double slots = cfg ? 512 : 256, cyc = cfg ? 1700 : 2700;
+        for (int s = 1; s <= 64 && s <= steps; ++s) {
+            const long long per = (steps + s - 1) / s;
+            if ((steps + per - 1) / per != s) continue;
+            const double rounds = (double)((tiles * s + (long long)slots - 1) / (long long)slots);
+            double t = rounds * (per * cyc + 6000);
+            if (s > 1) t += 8000 + (double)s * M * N * 8 / 2000;    // partial sums out and back at about 4.5 TB/s
+            if (p.kernel == 0 || t < best) {
+                best = t;
+                p.kernel = YOLO_AMD_LINEAR_TILE;
+                p.bm = p.bn = bt;
+                p.slices = s;
+                p.ksteps = (int)per;
+            }
+        }
+    }
+    return p;
+}
+
+static size_t partial_bytes(const TilePlan& p, long long M, int N) {
+    return p.slices > 1 ? align_up((size_t)p.slices * M * align_up(N, 8) * 4, 256) : 0;
+}
+
+template <typename T>
+static void launch_pack(const Matrix& m, void* dst, hipStream_t s) {
+    const int c8 = (int)(align_up(m.cols, 8) / 8);
+    const long long total = m.rows * c8;
+    const unsigned blocks = (unsigned)std::min<long long>((total + 255) / 256, 1 << 16);
+    hipLaunchKernelGGL((linear_pack_kernel<T>), dim3(blocks), dim3(256), 0, s, (const T*)m.p, m.ld, m.rows, m.cols, (T*)dst, c8);
+}
+
+template <typename T, bool AT, bool BT>
+static int launch_product(const TilePlan& p, TileArgs a, void* partial, hipStream_t s) {
+    if (p.kernel == YOLO_AMD_LINEAR_ROWS) {
+        if constexpr (!AT && !BT) {
+            const int nt = p.bn / 16;
+            const dim3 grid((a.N + p.bn - 1) / p.bn);
+            if (p.bm == 16 && nt == 1) hipLaunchKernelGGL((linear_rows_kernel<T, 1, 1>), grid, dim3(512), 0, s, a);
+            else if (p.bm == 16) hipLaunchKernelGGL((linear_rows_kernel<T, 1, 2>), grid, dim3(512), 0, s, a);
+            else if (nt == 1) hipLaunchKernelGGL((linear_rows_kernel<T, 2, 1>), grid, dim3(512), 0, s, a);
+            else hipLaunchKernelGGL((linear_rows_kernel<T, 2, 2>), grid, dim3(512), 0, s, a);
+        }
+        YA_CHECK_HIP(hipGetLastError());
+        return YA_OK;
+    }
+    a.tiles_m = (a.M + p.bm - 1) / p.bm;
+    a.tiles_n = (a.N + p.bn - 1) / p.bn;
+    a.ksteps = p.ksteps;
+    const Epilogue e = a.e;
+    if (p.slices > 1) {
+        a.e.part = (float*)partial;
+        a.e.ld_part = (long long)align_up(a.N, 8);
+        a.e.slice_stride = a.e.ld_part * a.M;
+    }
+    const dim3 grid((unsigned)((long long)a.tiles_m * a.tiles_n), (unsigned)p.slices);
+    if (p.bm == 256) hipLaunchKernelGGL((linear_tile_kernel<T, 256, 256, 2, 4, AT, BT>), grid, dim3(512), 0, s, a);
+    else hipLaunchKernelGGL((linear_tile_kernel<T, 128, 128, 2, 2, AT, BT>), grid, dim3(256), 0, s, a);
+    if (p.slices > 1) {
+        Epilogue f = e;
+        f.ld_part = a.e.ld_part;
+        f.slice_stride = a.e.slice_stride;
+        const long long total = (long long)a.M * (a.e.ld_part / 8);
+        hipLaunchKernelGGL((linear_finish_kernel<T>), dim3((unsigned)std::min<long long>((total + 255) / 256, 8192)), dim3(256), 0, s,
+                           f, (const float*)partial, p.slices, a.M, a.N, (int)(a.e.ld_part / 8));
+    }
+    YA_CHECK_HIP(hipGetLastError());
+    return YA_OK;
+}
+
+static bool rows16(const void* p, long long ld, int esize) {
+    return p == nullptr || (((uintptr_t)p & 15) == 0 && (ld * esize) % 16 == 0);
+}
+
+constexpr long long kMaxLd = (1ll << 22) - 1, kMaxRows = (1ll << 31) - 1024;
+
+static int check_common(const char* what, int64_t m, int64_t n, int64_t k, int type, int act) {
+    YA_REQUIRE(m >= 0 && n >= 0 && k >= 0 && m <= kMaxRows && n <= kMaxLd && k <= kMaxLd,
+               "%s: m=%lld n=%lld k=%lld (m up to %lld, n and k up to %lld)", what, (long long)m, (long long)n, (long long)k,
+               kMaxRows, kMaxLd);
+    YA_REQUIRE(type == YOLO_AMD_TYPE_BF16 || type == YOLO_AMD_TYPE_F16, "%s: type %d (bf16 or fp16)", what, type);
+    YA_REQUIRE(act >= YOLO_AMD_ACT_NONE && act <= YOLO_AMD_ACT_SILU, "%s: activation %d", what, act);
+    return YA_OK;
+}
+
+static int check_matrix(const char* what, const char* name, const void* p, long long ld, long long rows, int cols, int esize) {
+    if (rows == 0 || cols == 0) return YA_OK;
+    YA_REQUIRE(p, "%s: %s is null", what, name);
+    YA_REQUIRE(((uintptr_t)p & (esize - 1)) == 0, "%s: %s is not aligned to its elements", what, name);
+    YA_REQUIRE(rows <= 1 || (ld >= cols && ld <= kMaxLd), "%s: %s has row stride %lld for %d columns (at most %lld)", what, name, ld,
+               cols, kMaxLd);
+    return YA_OK;
+}
+static int check_forward(const yolo_amd_linear_desc* d) {
+    YA_REQUIRE(d, "linear_forward: null descriptor");
+    YA_TRY(check_common("linear_forward", d->m, d->n, d->k, d->type, d->activation));
+    YA_TRY(check_matrix("linear_forward", "x", d->x, d->ldx, d->m, (int)d->k, 2));
+    YA_TRY(check_matrix("linear_forward", "weight", d->weight, d->ldw, d->n, (int)d->k, 2));
+    YA_TRY(check_matrix("linear_forward", "y", d->y, d->ldy, d->m, (int)d->n, d->y_f32 ? 4 : 2));
+    if (d->residual) YA_TRY(check_matrix("linear_forward", "residual", d->residual, d->ldr, d->m, (int)d->n, d->residual_f32 ? 4 : 2));
+    if (d->bias) YA_TRY(check_matrix("linear_forward", "bias", d->bias, d->n, 1, (int)d->n, d->bias_f32 ? 4 : 2));
+    if (d->pre) YA_TRY(check_matrix("linear_forward", "pre", d->pre, d->n, d->m, (int)d->n, 2));
+    return YA_OK;
+}
+
+struct ForwardPlan {
+    TilePlan tile;
+    Matrix x, w;
+    size_t x_bytes, w_bytes, part_bytes;
+    size_t bytes() const { return x_bytes + w_bytes + part_bytes; }
+};
+
+static ForwardPlan plan_forward(const yolo_amd_linear_desc* d) {
+    ForwardPlan f{};
+    f.x = Matrix{d->x, d->ldx, d->m, (int)d->k};
+    f.w = Matrix{d->weight, d->ldw, d->n, (int)d->k};
+    if (d->m == 0 || d->n == 0) return f;
+    f.tile = plan_product(d->m, (int)d->n, d->k, true);
+    f.x_bytes = packed_bytes(f.x);
+    f.w_bytes = packed_bytes(f.w);
+    f.part_bytes = partial_bytes(f.tile, d->m, (int)d->n);
+    return f;
+}
+
+// Scratch of a call, handed out front to back.
+struct Scratch {
+    char* p;
+    void* take(size_t bytes) {
+        void* r = p;
+        p += bytes;
+        return r;
+    }
+};
+
+static int check_workspace(const char* what, const void* ws, size_t have, size_t need) {
+    if (need == 0) return YA_OK;
+    YA_REQUIRE(ws && ((uintptr_t)ws & 255) == 0, "%s: the workspace is null or not 256-byte aligned", what);
+    if (have < need) {
+        set_error("%s: workspace of %zu bytes, %zu needed", what, have, need);
+        return YA_ERR_WORKSPACE;
+    }
+    return YA_OK;
+}
+
+template <typename T>
+static Matrix packed(const Matrix& m, size_t bytes, Scratch& sc, hipStream_t s) {
+    if (bytes == 0) return m;
+    void* dst = sc.take(bytes);
+    launch_pack<T>(m, dst, s);
+    const int c8 = (int)align_up(m.cols, 8);
+    return Matrix{dst, c8, m.rows, c8};
+}
+
+template <typename T>
+static int forward(const yolo_amd_linear_desc* d, const ForwardPlan& f, hipStream_t s) {
+    Scratch sc{(char*)d->workspace};
+    const Matrix x = packed<T>(f.x, f.x_bytes, sc, s), w = packed<T>(f.w, f.w_bytes, sc, s);
+    TileArgs a{};
+    a.A = x.p; a.lda = x.ld;
+    a.B = w.p; a.ldb = w.ld;
+    a.M = (int)d->m; a.N = (int)d->n; a.K = std::min(x.cols, w.cols) ;
+    Epilogue& e = a.e;
+    e.bias = d->bias; e.res = d->residual; e.y = d->y; e.pre = d->pre;
+    e.ldr = d->ldr; e.ldy = d->ldy; e.ldp = d->n;
+    e.bias_f32 = d->bias_f32; e.res_f32 = d->residual_f32; e.y_f32 = d->y_f32; e.act = d->activation;
+    e.vec = d->n % 8 == 0 && rows16(e.bias, 0, 2) && rows16(e.res, e.ldr, e.res_f32 ? 4 : 2) &&
+            rows16(e.y, e.ldy, e.y_f32 ? 4 : 2) && rows16(e.pre, e.ldp, 2);
+    return launch_product<T, false, false>(f.tile, a, sc.take(f.part_bytes), s);
+}
+
+// ---- backward
+static int check_backward(const yolo_amd_linear_backward_desc* d) {
+    const char* me = "linear_backward";
+    YA_REQUIRE(d, "%s: null descriptor", me);
+    YA_TRY(check_common(me, d->m, d->n, d->k, d->type, d->activation));
+    YA_TRY(check_matrix(me, "dy", d->dy, d->lddy, d->m, (int)d->n, d->dy_f32 ? 4 : 2));
+    if (d->dweight) YA_TRY(check_matrix(me, "x", d->x, d->ldx, d->m, (int)d->k, 2));
+    if (d->dx) YA_TRY(check_matrix(me, "weight", d->weight, d->ldw, d->n, (int)d->k, 2));
+    if (d->activation != YOLO_AMD_ACT_NONE) YA_TRY(check_matrix(me, "pre", d->pre, d->n, d->m, (int)d->n, 2));
+    if (d->dx) YA_TRY(check_matrix(me, "dx", d->dx, d->k, d->m, (int)d->k, 2));
+    if (d->dweight) YA_TRY(check_matrix(me, "dweight", d->dweight, d->k, d->n, (int)d->k, 2));
+    if (d->dbias) YA_TRY(check_matrix(me, "dbias", d->dbias, d->n, 1, (int)d->n, d->dbias_f32 ? 4 : 2));
+    return YA_OK;
+}
+
+struct BackwardPlan {
+    TilePlan dx, dw;
+    Matrix x, w;
+    bool own_dp;            // dP is a tensor of its own (else dY is dP)
+    int blocks, rows;       // row blocks of the column sums
+    size_t dp_bytes, db_bytes, x_bytes, w_bytes, part_bytes;
+    size_t bytes() const { return dp_bytes + db_bytes + x_bytes + w_bytes + part_bytes; }
+};
+
+static BackwardPlan plan_backward(const yolo_amd_linear_backward_desc* d) {
+    BackwardPlan b{};
+    const bool empty = d->m == 0 || d->n == 0;
+    const Matrix dy{d->dy, d->lddy, d->m, (int)d->n};
+    b.x = Matrix{d->x, d->ldx, d->m, (int)d->k};
+    b.w = Matrix{d->weight, d->ldw, d->n, (int)d->k};
+    const bool products = (d->dx || d->dweight) && d->k > 0 && !empty;
+    b.own_dp = products && (d->activation != YOLO_AMD_ACT_NONE || d->dy_f32 || !packed_ok(dy));
+    if (b.own_dp) b.dp_bytes = align_up((size_t)d->m * align_up(d->n, 8) * 2, 256);
+    if (d->dbias && !empty) {
+        // enough blocks of rows to fill the chip, at least 32 rows each
+        const long long cols = (d->n + 255) / 256;
+        long long want = std::max<long long>(1, 2048 / cols);
+        b.rows = (int)std::max<long long>(32, (d->m + want - 1) / want);
+        b.db_bytes = align_up((size_t)((d->m + b.rows - 1) / b.rows) * d->n * 4, 256);
+    } else {
+        b.rows = 64;
+    }
+    b.blocks = (int)((d->m + b.rows - 1) / b.rows);
+    if (!products) return b;
+    if (d->dx) {
+        b.dx = plan_product(d->m, (int)d->k, d->n, false);
+        b.w_bytes = packed_bytes(b.w);
+        b.part_bytes = partial_bytes(b.dx, d->m, (int)d->k);
+    }
+    if (d->dweight) {
+        b.dw = plan_product(d->n, (int)d->k, d->m, false);
+        b.x_bytes = packed_bytes(b.x);
+        b.part_bytes = std::max(b.part_bytes, partial_bytes(b.dw, d->n, (int)d->k));
+    }
+    return b;
+}
+
+template <typename T>
+__global__ void __launch_bounds__(256) linear_zero_kernel(T* p, long long n) {
+    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n; i += (long long)gridDim.x * 256) p[i] = (T)0.f;
+}
+template <typename T>
+static void launch_zero(T* p, long long n, hipStream_t s) {
+    if (n > 0) hipLaunchKernelGGL((linear_zero_kernel<T>), dim3((unsigned)std::min<long long>((n + 255) / 256, 4096)), dim3(256), 0, s, p, n);
+}
+
+template <typename T>
+static int backward(const yolo_amd_linear_backward_desc* d, const BackwardPlan& b, hipStream_t s) {
+    const int M = (int)d->m, N = (int)d->n, K = (int)d->k;
+    if (M == 0 || N == 0) {                       // sums over nothing are zero
+        if (d->dx) launch_zero((T*)d->dx, (long long)M * K, s);
+        if (d->dweight) launch_zero((T*)d->dweight, (long long)N * K, s);
+        if (d->dbias && d->dbias_f32) launch_zero((float*)d->dbias, N, s);
+        else if (d->dbias) launch_zero((T*)d->dbias, N, s);
+        YA_CHECK_HIP(hipGetLastError());
+        return YA_OK;
+    }
+    Scratch sc{(char*)d->workspace};
+    void* dp = sc.take(b.dp_bytes);
+    float* db = (float*)sc.take(b.db_bytes);
+    if (b.own_dp || d->dbias) {
+        DpreArgs g{};
+        g.dy = d->dy; g.lddy = d->lddy; g.dy_f32 = d->dy_f32;
+        g.act = d->activation;
+        g.pre = g.act == YOLO_AMD_ACT_NONE ? nullptr : d->pre;
+        g.ldpre = N;
+        g.vec = N % 8 == 0 && rows16(g.dy, M > 1 ? g.lddy : 0, g.dy_f32 ? 4 : 2) && rows16(g.pre, N, 2);
+        g.dp = b.own_dp ? dp : nullptr;
+        g.ldp = (long long)align_up(N, 8);
+        g.part = d->dbias ? db : nullptr;
+        g.M = M; g.N = N; g.rows = b.rows;
+        hipLaunchKernelGGL((linear_dpre_kernel<T>), dim3((N + 255) / 256, b.blocks), dim3(256), 0, s, g);
+        if (d->dbias)
+            hipLaunchKernelGGL((linear_dbias_kernel<T>), dim3((N + 255) / 256), dim3(256), 0, s, db, b.blocks, N, d->dbias, d->dbias_f32);
+    }
+    const void* P = b.own_dp ? dp : d->dy;
+    const long long ldP = b.own_dp ? (long long)align_up(N, 8) : d->lddy;
+    if (K > 0) {
+        TileArgs a{};
+        a.e.act = YOLO_AMD_ACT_NONE;
+        a.e.vec = K % 8 == 0;
+        a.e.ldy = K;
+        const Matrix w = d->dx ? packed<T>(b.w, b.w_bytes, sc, s) : Matrix{};
+        const Matrix x = d->dweight ? packed<T>(b.x, b.x_bytes, sc, s) : Matrix{};
+        void* part = sc.take(b.part_bytes);
+        if (d->dx) {
+            a.A = P; a.lda = ldP;
+            a.B = w.p; a.ldb = w.ld;
+            a.M = M; a.N = K; a.K = N;
+            a.e.y = d->dx;
+            a.e.vec = K % 8 == 0 && ((uintptr_t)d->dx & 15) == 0;
+            YA_TRY((launch_product<T, false, true>(b.dx, a, part, s)));
+        }
+        if (d->dweight) {
+            a.A = P; a.lda = ldP;
+            a.B = x.p; a.ldb = x.ld;
+            a.M = N; a.N = K; a.K = M;
+            a.e.y = d->dweight;
+            a.e.vec = K % 8 == 0 && ((uintptr_t)d->dweight & 15) == 0;
+            YA_TRY((launch_product<T, true, true>(b.dw, a, part, s)));
+        }
+    }
+    YA_CHECK_HIP(hipGetLastError());
+    return YA_OK;
+}
+
+}  // namespace yolo_amd
+
+using namespace yolo_amd;
+
+extern "C" size_t yolo_amd_linear_workspace_bytes(const yolo_amd_linear_desc* d) {
+    return check_forward(d) == YA_OK ? plan_forward(d).bytes() : 0;
+}
+
+extern "C" int yolo_amd_linear_query(const yolo_amd_linear_desc* d, yolo_amd_linear_choice* out) {
+    YA_REQUIRE(out, "linear_query: null output");
+    YA_TRY(check_forward(d));
+    const ForwardPlan f = plan_forward(d);
+    *out = yolo_amd_linear_choice{f.tile.kernel, f.tile.bm, f.tile.bn, f.tile.slices, f.x_bytes != 0, f.w_bytes != 0};
+    return YA_OK;
+}
+
+extern "C" int yolo_amd_linear_forward(const yolo_amd_linear_desc* d, void* stream) {
+    YA_TRY(check_forward(d));
+    const ForwardPlan f = plan_forward(d);
+    if (d->m == 0 || d->n == 0) return YA_OK;
+    YA_TRY(check_workspace("linear_forward", d->workspace, d->workspace_bytes, f.bytes()));
+    return d->type == YOLO_AMD_TYPE_BF16 ? forward<__bf16>(d, f, (hipStream_t)stream) : forward<_Float16>(d, f, (hipStream_t)stream);
+}
+
+extern "C" size_t yolo_amd_linear_backward_workspace_bytes(const yolo_amd_linear_backward_desc* d) {
+    return check_backward(d) == YA_OK ? plan_backward(d).bytes() : 0;
+}
+
+extern "C" int yolo_amd_linear_backward(const yolo_amd_linear_backward_desc* d, void* stream) {
+    YA_TRY(check_backward(d));
+    const BackwardPlan b = plan_backward(d);
+    YA_TRY(check_workspace("linear_backward", d->workspace, d->workspace_bytes, b.bytes()));
+    return d->type == YOLO_AMD_TYPE_BF16 ? backward<__bf16>(d, b, (hipStream_t)stream) : backward<_Float16>(d, b, (hipStream_t)stream);
+}
