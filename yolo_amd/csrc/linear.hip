@@ -29,21 +29,59 @@ __device__ __forceinline__ f32x4 mfma(v8<_Float16> a, v8<_Float16> b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
 }
 
+// The same in place on accumulators held in accumulation registers: with 64 of them (all 256 registers) the
+// compiler's own allocation rotates them through copies at every turn of a loop.  The compiler does not see that a
+// matrix instruction is in flight: a kernel waits (mfma_drain) before it reads its accumulators otherwise.
+__device__ __forceinline__ void mfma_in_place(v8<__bf16> a, v8<__bf16> b, f32x4& c) {
+    asm volatile("v_mfma_f32_16x16x32_bf16 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b));
+}
+__device__ __forceinline__ void mfma_in_place(v8<_Float16> a, v8<_Float16> b, f32x4& c) {
+    asm volatile("v_mfma_f32_16x16x32_f16 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b));
+}
+// more wait states than any matrix instruction's result takes (16 passes at most)
+__device__ __forceinline__ void mfma_drain() { asm volatile("s_nop 15\n\ts_nop 15" ::: "memory"); }
+
 // ---------------------------------------------------------------- activations
-constexpr float kGeluC = 0.7978845608028654f, kGeluA = 0.044715f, kRsqrt2 = 0.7071067811865476f;
-constexpr float kRsqrt2Pi = 0.3989422804014327f;
+// exp2, reciprocal: the hardware's (1 ulp each).  erfc(x) for x >= 0 after Abramowitz and Stegun, Handbook of
+// Mathematical Functions, 7.1.26 (error at most 1.5e-7 absolute): a fifth of erff's instructions, and an epilogue of
+// one activation per matrix-unit column is bound by them.
+constexpr float kLog2e = 1.44269504088896340736f;
+constexpr float kGeluC = 0.7978845608028654f, kGeluA = 0.044715f;
 
-// 1 / (1 + exp(-x)); exp overflows to +inf for x < -88 and the reciprocal is then 0, as it should be
-__device__ __forceinline__ float sigmoid(float x) { return sigmoid_fast(x); }
+// erfc(|p| / sqrt 2) and exp(-p^2 / 2); NaN for NaN, 0 and 0 for infinities
+__device__ __forceinline__ float erfc_scaled(float p, float& e) {
+    const float t = __builtin_amdgcn_rcpf(fmaf(fabsf(p), 0.3275911f * 0.70710678118654752f, 1.f));
+    e = __builtin_amdgcn_exp2f(p * p * (-0.5f * kLog2e));
+    float q = fmaf(t, 1.061405429f, -1.453152027f);
+    q = fmaf(q, t, 1.421413741f);
+    q = fmaf(q, t, -0.284496736f);
+    q = fmaf(q, t, 0.254829592f);
+    return q * t * e;
+}
 
+template <int ACT>
+__device__ __forceinline__ float act_value(float p) {
+    if constexpr (ACT == YOLO_AMD_ACT_LEAKY) return p > 0.f ? p : 0.1f * p;
+    if constexpr (ACT == YOLO_AMD_ACT_RELU) return p < 0.f ? 0.f : p;
+    if constexpr (ACT == YOLO_AMD_ACT_GELU) {
+        // max(p, 0) - |p| erfc(|p| / sqrt 2) / 2; the clamp keeps inf * 0 out (erfc is 0 from 15 on)
+        float e;
+        const float q = erfc_scaled(p, e);
+        return fmaf(fminf(fabsf(p), 100.f) * -0.5f, q, p < 0.f ? 0.f : p);
+    }
+    // (1 + tanh z) / 2 = 1 / (1 + exp(-2 z))
+    if constexpr (ACT == YOLO_AMD_ACT_GELU_TANH)
+        return p * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(p * fmaf(p * p, -2.f * kLog2e * kGeluC * kGeluA, -2.f * kLog2e * kGeluC)));
+    if constexpr (ACT == YOLO_AMD_ACT_SILU) return p * sigmoid_fast(p);
+    return p;
+}
 __device__ __forceinline__ float act_value(float p, int act) {
     switch (act) {
-        case YOLO_AMD_ACT_LEAKY: return p > 0.f ? p : 0.1f * p;
-        case YOLO_AMD_ACT_RELU: return p > 0.f ? p : (p != p ? p : 0.f);
-        case YOLO_AMD_ACT_GELU: return 0.5f * p * (1.f + erff(p * kRsqrt2));
-        // 0.5 (1 + tanh z) = sigmoid(2 z)
-        case YOLO_AMD_ACT_GELU_TANH: return p * sigmoid(2.f * kGeluC * (p + kGeluA * p * p * p));
-        case YOLO_AMD_ACT_SILU: return p * sigmoid(p);
+        case YOLO_AMD_ACT_LEAKY: return act_value<YOLO_AMD_ACT_LEAKY>(p);
+        case YOLO_AMD_ACT_RELU: return act_value<YOLO_AMD_ACT_RELU>(p);
+        case YOLO_AMD_ACT_GELU: return act_value<YOLO_AMD_ACT_GELU>(p);
+        case YOLO_AMD_ACT_GELU_TANH: return act_value<YOLO_AMD_ACT_GELU_TANH>(p);
+        case YOLO_AMD_ACT_SILU: return act_value<YOLO_AMD_ACT_SILU>(p);
         default: return p;
     }
 }
@@ -52,14 +90,17 @@ __device__ __forceinline__ float act_slope(float p, int act) {
     switch (act) {
         case YOLO_AMD_ACT_LEAKY: return p > 0.f ? 1.f : 0.1f;
         case YOLO_AMD_ACT_RELU: return p > 0.f ? 1.f : 0.f;
-        case YOLO_AMD_ACT_GELU:
-            return 0.5f * (1.f + erff(p * kRsqrt2)) + p * kRsqrt2Pi * exp_fast(-0.5f * p * p);
+        case YOLO_AMD_ACT_GELU: {
+            float e;
+            const float q = 0.5f * erfc_scaled(p, e);
+            return fmaf(p * 0.3989422804014327f, e, p < 0.f ? q : 1.f - q);
+        }
         case YOLO_AMD_ACT_GELU_TANH: {
-            const float z = sigmoid(2.f * kGeluC * (p + kGeluA * p * p * p));
+            const float z = sigmoid_fast(2.f * kGeluC * (p + kGeluA * p * p * p));
             return z + p * z * (1.f - z) * 2.f * kGeluC * (1.f + 3.f * kGeluA * p * p);
         }
         case YOLO_AMD_ACT_SILU: {
-            const float z = sigmoid(p);
+            const float z = sigmoid_fast(p);
             return z * (1.f + p * (1.f - z));
         }
         default: return 1.f;
@@ -155,17 +196,161 @@ __device__ __forceinline__ void finish8(const Epilogue& e, long long m, int n, i
     }
 }
 
+// ---- from the accumulators of a wave, without LDS
+// A wave's accumulator tile has lane l's row l & 15 and four columns (l >> 4) * 4 ..  Two neighbouring tiles, rounded
+// and packed to two registers each, change lanes so that a lane holds eight consecutive columns: a 16-byte store of
+// each lane then fills 64 contiguous bytes of 16 rows.  Swapping lane halves, then odd and even rows of 16 lanes, does
+// it; the two swaps in the other order undo it.
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ void swap32(uint32_t& x, uint32_t& y) {
+    const auto r = __builtin_amdgcn_permlane32_swap(x, y, false, false);
+    x = r[0];
+    y = r[1];
+}
+__device__ __forceinline__ void swap16(uint32_t& x, uint32_t& y) {
+    const auto r = __builtin_amdgcn_permlane16_swap(x, y, false, false);
+    x = r[0];
+    y = r[1];
+}
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+    typedef T t2 __attribute__((ext_vector_type(2)));
+    const t2 v = {(T)a, (T)b};
+    return __builtin_bit_cast(uint32_t, v);
+}
+template <typename T>
+__device__ __forceinline__ void unpack2(uint32_t u, float& a, float& b) {
+    typedef T t2 __attribute__((ext_vector_type(2)));
+    const t2 v = __builtin_bit_cast(t2, u);
+    a = (float)v[0];
+    b = (float)v[1];
+}
+// v: columns of two tiles -> the lane's 16 bytes
+template <typename T>
+__device__ __forceinline__ u32x4 pair_out(const float (&v)[2][4]) {
+    uint32_t a0 = pack2<T>(v[0][0], v[0][1]), a1 = pack2<T>(v[0][2], v[0][3]);
+    uint32_t b0 = pack2<T>(v[1][0], v[1][1]), b1 = pack2<T>(v[1][2], v[1][3]);
+    swap32(a0, b0);
+    swap32(a1, b1);
+    swap16(a0, b0);
+    swap16(a1, b1);
+    return u32x4{a0, a1, b0, b1};
+}
+template <typename T>
+__device__ __forceinline__ void pair_in(u32x4 u, float (&v)[2][4]) {
+    uint32_t a0 = u[0], a1 = u[1], b0 = u[2], b1 = u[3];
+    swap16(a0, b0);
+    swap16(a1, b1);
+    swap32(a0, b0);
+    swap32(a1, b1);
+    unpack2<T>(a0, v[0][0], v[0][1]);
+    unpack2<T>(a1, v[0][2], v[0][3]);
+    unpack2<T>(b0, v[1][0], v[1][1]);
+    unpack2<T>(b1, v[1][2], v[1][3]);
+}
+
+// Four accumulators, read where they are used (IN_PLACE: see mfma_in_place; the compiler would fetch all 256 at once)
+template <bool IN_PLACE>
+__device__ __forceinline__ void acc_read(f32x4& c, float (&v)[4]) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        if constexpr (IN_PLACE) asm volatile("v_accvgpr_read_b32 %0, %1" : "=v"(v[k]) : "a"(c[k]));
+        else v[k] = c[k];
+    }
+}
+
+// The wave's rows m0 .. and columns n0 .. (e.vec holds).
+template <typename T, int ACT, bool IN_PLACE, int TM, int TN>
+__device__ __forceinline__ void finish_direct(const Epilogue& e, f32x4 (&acc)[TM][TN], int m0, int n0, int M, int N, int lane) {
+    const int row = lane & 15, c4 = (lane >> 4) * 4, c8 = (lane >> 4) * 8;
+    float bias[TN][4];
+#pragma unroll
+    for (int j = 0; j < TN; ++j) {
+        const int n = n0 + j * 16 + c4;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) bias[j][k] = 0.f;
+        if (e.bias && n < N) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) bias[j][k] = load1<T>(e.bias, n + k, e.bias_f32);
+        }
+    }
+    u32x4 ahead[TN / 2];                               // the next rows' residual, if it has T's size
+    auto fetch = [&](int i) {
+        const long long m = (long long)m0 + i * 16 + row;
+#pragma unroll
+        for (int p = 0; p < TN / 2; ++p) {
+            const int n = n0 + p * 32 + c8;
+            if (m < M && n < N) ahead[p] = *reinterpret_cast<const u32x4*>((const T*)e.res + m * e.ldr + n);
+        }
+    };
+    const bool res_t = e.res && !e.res_f32;
+    if (res_t) fetch(0);
+#pragma unroll
+    for (int i = 0; i < TM; ++i) {
+        const long long m = (long long)m0 + i * 16 + row;
+        u32x4 now[TN / 2];
+#pragma unroll
+        for (int p = 0; p < TN / 2; ++p) now[p] = ahead[p];
+        if (res_t && i + 1 < TM) fetch(i + 1);
+#pragma unroll
+        for (int p = 0; p < TN / 2; ++p) {
+            const int n = n0 + p * 32;
+            const bool in8 = m < M && n + c8 < N;
+            float v[2][4];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                acc_read<IN_PLACE>(acc[i][p * 2 + h], v[h]);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) v[h][k] += bias[p * 2 + h][k];
+            }
+            if (e.pre) {
+                const u32x4 o = pair_out<T>(v);
+                if (in8) *reinterpret_cast<u32x4*>((T*)e.pre + m * e.ldp + n + c8) = o;
+            }
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) v[h][k] = act_value<ACT>(v[h][k]);
+            if (res_t) {
+                float r[2][4];
+                pair_in<T>(now[p], r);
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) v[h][k] += r[h][k];
+            } else if (e.res) {
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+                    if (m < M && n + h * 16 + c4 < N) {
+                        const f32x4 r = *reinterpret_cast<const f32x4*>((const float*)e.res + m * e.ldr + n + h * 16 + c4);
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) v[h][k] += r[k];
+                    }
+            }
+            if (e.y_f32) {
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+                    if (m < M && n + h * 16 + c4 < N)
+                        *reinterpret_cast<f32x4*>((float*)e.y + m * e.ldy + n + h * 16 + c4) = f32x4{v[h][0], v[h][1], v[h][2], v[h][3]};
+            } else {
+                const u32x4 o = pair_out<T>(v);
+                if (in8) *reinterpret_cast<u32x4*>((T*)e.y + m * e.ldy + n + c8) = o;
+            }
+        }
+    }
+}
+
 // ---------------------------------------------------------------- tile kernel
 struct TileArgs {
     const void *A, *B;
     long long lda, ldb;     // elements
     int M, N, K;
     int tiles_m, tiles_n;
-    int ksteps;             // K-steps of 64 per slice (blockIdx.y = slice)
+    int ksteps;             // units of 64 reduction indices per slice (blockIdx.y = slice)
     Epilogue e;
 };
 
-constexpr int kBK = 64;
+constexpr int kBK = 64;         // reduction indices per step: whole 128-byte lines of a row
 constexpr uint32_t kBufferBytes = 0x80000000u;   // descriptor size: offsets built below stay under it
 
 // One operand's tile of R rows (its own index) x 64 reduction indices in LDS, filled by W waves.
@@ -178,12 +363,12 @@ constexpr uint32_t kBufferBytes = 0x80000000u;   // descriptor size: offsets bui
 // descriptor's range check, so no tile reads outside its matrix.
 template <int R, int W, bool TR>
 struct Operand {
-    static constexpr int NI = R / 8 / W;          // LDS-DMA instructions (1 KiB each) per wave and K-step
+    static constexpr int NI = R / 8 / W;          // LDS-DMA instructions (1 KiB each) per wave and step
     static constexpr int BYTES = R * kBK * 2;
     uint32_t voff[NI];
     int kfirst, kstride;                          // reduction index of this lane's first chunk, and per instruction
-    const char* base;                             // wave-uniform: this tile at the current K-step
-    long long step;                               // bytes from one K-step to the next
+    const char* base;                             // wave-uniform: this tile at the current step
+    long long step;                               // bytes from one step to the next
 
     __device__ __forceinline__ void init(const void* p, long long ld, int row0, int extent, int kbeg, int lane, int w) {
         if constexpr (!TR) {
@@ -199,30 +384,32 @@ struct Operand {
             step = kBK * 2;
         } else {
             constexpr int CPR = R / 8, RPI = 64 / CPR;     // chunks per row, rows per instruction
-            static_assert((W * RPI) % 16 == 0, "f(k) is the same for all of a lane's instructions");
+            // f(k) of instruction j: k advances by W * RPI, a multiple of 8; where it is an odd one, bit 3 changes
+            static_assert((W * RPI) % 8 == 0, "only bit 2 of f(k) differs between a lane's instructions");
             const int k = w * RPI + lane / CPR;
-            const int f = (k & 3) | ((k >> 3 & 1) << 2);
-            const int c = (lane % CPR) ^ (f << 1);
             kfirst = k;
             kstride = W * RPI;
 #pragma unroll
-            for (int j = 0; j < NI; ++j)
-                voff[j] = row0 + c * 8 < extent ? (uint32_t)((k + j * W * RPI) * (uint32_t)ld * 2u) + c * 16u : kBufferNowhere;
+            for (int j = 0; j < NI; ++j) {
+                const int kj = k + j * W * RPI;
+                const int c = (lane % CPR) ^ (((kj & 3) | ((kj >> 3 & 1) << 2)) << 1);
+                voff[j] = row0 + c * 8 < extent ? (uint32_t)(kj * (uint32_t)ld * 2u) + c * 16u : kBufferNowhere;
+            }
             base = (const char*)p + ((long long)kbeg * ld + row0) * 2;
             step = kBK * ld * 2;
         }
     }
-    // issue the K-step at `base`, whose reduction indices below `left` are valid, and move on
-    __device__ __forceinline__ void issue(char* buf, int w, int left) {
+    // from here on only reduction indices below `left` of the step at `base` are valid (left <= 0: none; the loads
+    // then write zeros and touch no memory)
+    __device__ __forceinline__ void limit(int left) {
+#pragma unroll
+        for (int j = 0; j < NI; ++j) voff[j] = kfirst + j * kstride < left ? voff[j] : kBufferNowhere;
+    }
+    // instruction j of the step at `base`
+    __device__ __forceinline__ void issue(int j, char* buf, int w) const {
         const __amdgpu_buffer_rsrc_t rs =
             __builtin_amdgcn_make_buffer_rsrc((void*)base, 0, (int)kBufferBytes, (int)kRawBufferWord3);
-#pragma unroll
-        for (int j = 0; j < NI; ++j) {
-            uint32_t v = voff[j];
-            if (left < kBK) v = kfirst + j * kstride < left ? v : kBufferNowhere;
-            lds_dma16_buf(rs, v, 0, buf + (j * W + w) * 1024);
-        }
-        base += step;
+        lds_dma16_buf(rs, voff[j], 0, buf + (j * W + w) * 1024);
     }
 };
 
@@ -253,17 +440,18 @@ struct Fragments {
     }
 };
 
-template <typename T, int BM, int BN, int WM, int WN, bool AT, bool BT>
-__global__ void __launch_bounds__(WM * WN * 64)
+template <typename T, int BM, int BN, bool AT, bool BT>
+__global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(BM == 256 ? 1 : 2, BM == 256 ? 1 : 2)))
 linear_tile_kernel(const TileArgs a) {
-    constexpr int W = WM * WN, NT = W * 64;
+    constexpr int WM = 2, WN = 2, W = WM * WN, NT = W * 64;
     constexpr int WTM = BM / WM, WTN = BN / WN, TM = WTM / 16, TN = WTN / 16;
     typedef Operand<BM, W, AT> OpA;
     typedef Operand<BN, W, BT> OpB;
-    constexpr int STAGE = OpA::BYTES + OpB::BYTES;
+    constexpr int RING = 5 * OpA::BYTES;
+    constexpr int PER = OpA::NI + OpB::NI;             // loads per wave and step
     constexpr int CROWS = WM * 32, CLD = BN + 4;       // epilogue chunk: 32 rows per wave row, fp32
-    constexpr int LDS = 2 * STAGE > CROWS * CLD * 4 ? 2 * STAGE : CROWS * CLD * 4;
-    __shared__ __attribute__((aligned(1024))) char lds[LDS];
+    static_assert(RING >= CROWS * CLD * 4, "the epilogue's chunk fits into the ring");
+    __shared__ __attribute__((aligned(1024))) char lds[RING];
 
     const int lane = threadIdx.x & 63;
     const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -300,36 +488,131 @@ linear_tile_kernel(const TileArgs a) {
 #pragma unroll
         for (int j = 0; j < TN; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
 
-    auto issue = [&](int t) {
-        char* buf = lds + (t & 1) * STAGE;
-        const int left = kend - kbeg - t * kBK;
-        opa.issue(buf, w, left);
-        opb.issue(buf + OpA::BYTES, w, left);
+    // A ring of five operand tiles in LDS -- A(t), B(t), A(t+1), B(t+1), A(t+2) in turn -- and two sets of fragments in
+    // registers.  The matrix instructions of half a step (32 reduction indices) run while the fragments of the next
+    // half are read; in the middle of step t a barrier says that every wave has read its last fragments of A(t) and
+    // B(t), whose places B(t+2) and A(t+3) take over the next two halves, one load (1 KiB) after every eighth matrix
+    // instruction: with one wave per SIMD a load that finds the memory pipe busy holds up the matrix unit, and evenly
+    // spaced loads do that least (8192^3: all of a step's loads in one eighth of it 872 us, in a quarter 836, in a
+    // half 813).  The instruction stream is held in the order written by scheduling fences.
+    constexpr int GROUPS = TM * TN / 4, READS = TM + TN;
+    constexpr int TILE = OpA::BYTES;
+    static_assert(OpA::BYTES == OpB::BYTES && GROUPS % OpA::NI == 0, "slots of one size, loads evenly spaced");
+    constexpr int SPACE = GROUPS / OpA::NI;
+    int left_a = kend - kbeg, left_b = left_a;
+    auto limit_a = [&]() {
+        if (left_a < kBK) opa.limit(left_a);
     };
-    if (nt > 0) issue(0);
+    auto limit_b = [&]() {
+        if (left_b < kBK) opb.limit(left_b);
+    };
+    auto next_a = [&]() {
+        opa.base += opa.step;
+        left_a -= kBK;
+        limit_a();
+    };
+    auto next_b = [&]() {
+        opb.base += opb.step;
+        left_b -= kBK;
+        limit_b();
+    };
+    // slot two on (one step), as byte offsets
+    auto two_on = [](int slot) { return slot >= 3 * TILE ? slot - 3 * TILE : slot + 2 * TILE; };
+    auto fetch = [&](v8<T> (&fr)[READS], int q, const char* ta, const char* tb, int s) {     // B's fragments, then A's
+        fr[q] = q < TN ? fb.get(tb, q, s) : fa.get(ta, q - TN, s);
+    };
+    auto products = [&](const v8<T> (&fr)[READS], int g) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const int i = (g * 4 + e) / TN, j = (g * 4 + e) % TN;
+            if constexpr (BM == 256) mfma_in_place(fr[j], fr[TN + i], acc[i][j]);
+            else acc[i][j] = mfma(fr[j], fr[TN + i], acc[i][j]);
+        }
+    };
+#define YA_FENCE() __builtin_amdgcn_sched_barrier(0)
+    v8<T> f0[READS], f1[READS];
+    limit_a();
+    limit_b();
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+#pragma unroll
+        for (int q = 0; q < OpA::NI; ++q) opa.issue(q, lds + t * 2 * TILE, w);
+#pragma unroll
+        for (int q = 0; q < OpB::NI; ++q) opb.issue(q, lds + t * 2 * TILE + TILE, w);
+        next_a();
+        next_b();
+    }
+    wait_vmcnt<PER>();
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+#pragma unroll
+    for (int q = 0; q < READS; ++q) fetch(f0, q, lds, lds + TILE, 0);
+    int sa = 0, sb = TILE, fill = 4 * TILE;            // slots of A(t), B(t), A(t+2)
     for (int t = 0; t < nt; ++t) {
-        // this wave's loads have landed and its reads of the other buffer have returned; then everybody's
-        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        // first half: the second half's fragments in the first three quarters of it
+        constexpr int RPG = (READS * 4 + GROUPS * 3 - 1) / (GROUPS * 3);
+#pragma unroll
+        for (int g = 0; g < GROUPS; ++g) {
+            if (g % SPACE == 0) opa.issue(g / SPACE, lds + fill, w);
+#pragma unroll
+            for (int q = g * RPG; q < (g + 1) * RPG; ++q)
+                if (q < READS) fetch(f1, q, lds + sa, lds + sb, 1);
+            products(f0, g);
+            YA_FENCE();
+        }
+        next_a();
+        // this wave's reads of A(t) and B(t) have returned and its loads of A(t+1) and B(t+1) landed (those of A(t+2)
+        // may be on their way); then everybody's
+        wait_vmcnt<OpA::NI>();
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
-        if (t + 1 < nt) issue(t + 1);
-        const char* buf = lds + (t & 1) * STAGE;
+        YA_FENCE();
+        // second half: the next step's first fragments
+        constexpr int RPG2 = (READS + GROUPS - 1) / GROUPS;
+        const int na = two_on(sa), nb = two_on(sb);
 #pragma unroll
-        for (int s = 0; s < 2; ++s) {
-            v8<T> av[TM], bv[TN];
+        for (int g = 0; g < GROUPS; ++g) {
+            if (g % SPACE == 0) opb.issue(g / SPACE, lds + sa, w);
 #pragma unroll
-            for (int j = 0; j < TN; ++j) bv[j] = fb.get(buf + OpA::BYTES, j, s);
-#pragma unroll
-            for (int i = 0; i < TM; ++i) av[i] = fa.get(buf, i, s);
-#pragma unroll
-            for (int i = 0; i < TM; ++i)
-#pragma unroll
-                for (int j = 0; j < TN; ++j) acc[i][j] = mfma(bv[j], av[i], acc[i][j]);
+            for (int q = g * RPG2; q < (g + 1) * RPG2; ++q)
+                if (q < READS) fetch(f0, q, lds + na, lds + nb, 0);
+            products(f1, g);
+            YA_FENCE();
         }
+        next_b();
+        fill = sb;
+        sa = na;
+        sb = nb;
     }
+#undef YA_FENCE
+    if constexpr (BM == 256) mfma_drain();
+    wait_vmcnt<0>();                                   // no load may land in the epilogue's LDS
 
-    // The accumulators (lane: row l & 15, four columns (l >> 4) * 4 ..) go through LDS in fp32, 32 rows of every
-    // wave row at a time, so that every access to memory behind it is 16 bytes per lane and coalesced.
+    if (a.e.vec) {
+        const int mw = m0 + wm * WTM, nw = n0 + wn * WTN;
+        Epilogue e = a.e;
+        if (e.part) {                                  // a K slice: raw sums
+            e.y = e.part + blockIdx.y * e.slice_stride;
+            e.ldy = e.ld_part;
+            e.y_f32 = 1;
+        }
+        if constexpr (AT || BT) {
+            finish_direct<T, YOLO_AMD_ACT_NONE, BM == 256>(e, acc, mw, nw, a.M, a.N, lane);
+        } else {
+            switch (e.act) {
+                case YOLO_AMD_ACT_LEAKY: finish_direct<T, YOLO_AMD_ACT_LEAKY, BM == 256>(e, acc, mw, nw, a.M, a.N, lane); break;
+                case YOLO_AMD_ACT_RELU: finish_direct<T, YOLO_AMD_ACT_RELU, BM == 256>(e, acc, mw, nw, a.M, a.N, lane); break;
+                case YOLO_AMD_ACT_GELU: finish_direct<T, YOLO_AMD_ACT_GELU, BM == 256>(e, acc, mw, nw, a.M, a.N, lane); break;
+                case YOLO_AMD_ACT_GELU_TANH: finish_direct<T, YOLO_AMD_ACT_GELU_TANH, BM == 256>(e, acc, mw, nw, a.M, a.N, lane); break;
+                case YOLO_AMD_ACT_SILU: finish_direct<T, YOLO_AMD_ACT_SILU, BM == 256>(e, acc, mw, nw, a.M, a.N, lane); break;
+                default: finish_direct<T, YOLO_AMD_ACT_NONE, BM == 256>(e, acc, mw, nw, a.M, a.N, lane); break;
+            }
+        }
+        return;
+    }
+    // Rows of y that do not start on 16-byte boundaries, or N no multiple of 8: the accumulators go through LDS in
+    // fp32, 32 rows of every wave row at a time, and are finished by element.
     float* out = reinterpret_cast<float*>(lds);
 #pragma unroll
     for (int c = 0; c < WTM / 32; ++c) {
@@ -338,8 +621,12 @@ linear_tile_kernel(const TileArgs a) {
         for (int i = 0; i < 2; ++i)
 #pragma unroll
             for (int j = 0; j < TN; ++j)
+            {
+                float v[4];
+                acc_read<BM == 256>(acc[c * 2 + i][j], v);
                 *reinterpret_cast<f32x4*>(out + (wm * 32 + i * 16 + (lane & 15)) * CLD + wn * WTN + j * 16 + (lane >> 4) * 4) =
-                    acc[c * 2 + i][j];
+                    f32x4{v[0], v[1], v[2], v[3]};
+            }
         __syncthreads();
         for (int it = threadIdx.x; it < CROWS * (BN / 8); it += NT) {
             const int lr = it / (BN / 8), n = n0 + (it % (BN / 8)) * 8;
@@ -347,8 +634,7 @@ linear_tile_kernel(const TileArgs a) {
             if (m < a.M && n < a.N) {
                 float v[8];
                 load8<T>(out, lr * CLD + (n - n0), 1, v);
-                if (a.e.part) store8<T>(a.e.part, blockIdx.y * a.e.slice_stride + m * a.e.ld_part + n, 1, v);
-                else finish8<T>(a.e, m, n, a.N, v);
+                finish8<T>(a.e, m, n, a.N, v);
             }
         }
     }
@@ -621,13 +907,15 @@ static int launch_product(const TilePlan& p, TileArgs a, void* partial, hipStrea
     a.ksteps = p.ksteps;
     const Epilogue e = a.e;
     if (p.slices > 1) {
+        a.e = Epilogue{};
+        a.e.vec = 1;                                   // rows of whole 8 columns, the last ones past N
         a.e.part = (float*)partial;
         a.e.ld_part = (long long)align_up(a.N, 8);
         a.e.slice_stride = a.e.ld_part * a.M;
     }
     const dim3 grid((unsigned)((long long)a.tiles_m * a.tiles_n), (unsigned)p.slices);
-    if (p.bm == 256) hipLaunchKernelGGL((linear_tile_kernel<T, 256, 256, 2, 4, AT, BT>), grid, dim3(512), 0, s, a);
-    else hipLaunchKernelGGL((linear_tile_kernel<T, 128, 128, 2, 2, AT, BT>), grid, dim3(256), 0, s, a);
+    if (p.bm == 256) hipLaunchKernelGGL((linear_tile_kernel<T, 256, 256, AT, BT>), grid, dim3(256), 0, s, a);
+    else hipLaunchKernelGGL((linear_tile_kernel<T, 128, 128, AT, BT>), grid, dim3(256), 0, s, a);
     if (p.slices > 1) {
         Epilogue f = e;
         f.ld_part = a.e.ld_part;
