@@ -369,6 +369,7 @@ typedef struct {
     int bm, bn;      /* rows x columns of y per workgroup                */
     int k_slices;    /* > 1: split reduction + finishing launch          */
     int copies_x, copies_weight; /* 1: the operand is copied into the workspace first */
+    int steps_ahead; /* TILE: steps of 64 reduction indices on their way  */
 } yolo_amd_linear_choice;
 int yolo_amd_linear_query(const yolo_amd_linear_desc* desc, yolo_amd_linear_choice* out);
 

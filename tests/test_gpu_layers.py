@@ -161,35 +161,36 @@ def test_linear_offsets_past_32_bits():
     assert torch.equal(y[5000], y[m - 400])
 
 
-def test_linear_kernels_of_the_dispatch():
-    """Every kernel of the dispatch is one that a test above runs."""
-    g = _gen(13)
-    seen = set()
-    for m, n, k in SHAPES + [(4096, 4096, 512)]:
-        x, w = torch.empty(m, k, dtype=BF16, device="cuda"), torch.empty(n, k, dtype=BF16, device="cuda")
-        name, c = _choice(x, w)
-        seen.add((name, c.bm, c.k_slices > 1))
-    assert {("rows", 16, False), ("tile", 128, True)} <= {(a, b, c) for a, b, c in seen}
-    assert any(a == "tile" and b == 256 for a, b, _ in seen)
+def _band_check(x, w, b, r, y, act, dtype):
+    """A band of rows and a band of columns of y, both with the ragged edge: the 64-bit product of all is slow here."""
+    m, n = y.shape
+    rows = torch.cat([torch.arange(0, 40), torch.arange(max(0, m - 300), m)]).cuda()
+    want, bound, _, _ = ref.linear_ref(x[rows], w, b, r[rows], act, dtype)
+    assert_within(y[rows], want, bound, "rows")
+    cols = torch.cat([torch.arange(0, 40), torch.arange(max(0, n - 300), n)]).cuda()
+    want, bound, _, _ = ref.linear_ref(x, w[cols], b[cols], r[:, cols], act, dtype)
+    assert_within(y[:, cols], want, bound, "columns")
+
+
+# (m, n, k), and the tile and split the library takes for it: every kernel of its choice, whole and ragged
+TILES = [((4096, 4096, 2048), 256, 1, 2), ((1266, 6976, 4624), 256, 1, 2), ((4090, 4093, 2051), 256, 1, 2),
+         ((2048, 4096, 256), 128, 1, 2), ((1990, 4072, 264), 128, 1, 2), ((1990, 4070, 265), 128, 1, 2),
+         ((2048, 2048, 1024), 128, 1, 4), ((1999, 2024, 1096), 128, 1, 4), ((2048, 1024, 8192), 128, 2, 4),
+         ((1024, 1024, 256), 64, 1, 4), ((333, 760, 200), 64, 1, 4), ((333, 759, 200), 64, 1, 4),
+         ((333, 760, 4104), 64, 3, 4), ((333, 761, 4104), 64, 3, 4), ((1100, 1000, 1000), 64, 1, 4)]
 
 
 @pytest.mark.parametrize("dtype", [BF16, F16])
-def test_linear_large_tile(dtype):
-    """The 256 x 256 tile, whole and ragged."""
+@pytest.mark.parametrize("shape,bm,slices,ahead", TILES)
+def test_linear_tiles(shape, bm, slices, ahead, dtype):
     from yolo_amd.layers import linear
-    g = _gen(14)
-    for m, n, k in ((4096, 4096, 512), (4000, 4104, 456)):
-        x, w, b = _rand(g, m, k, dtype=dtype), _rand(g, n, k, scale=k ** -0.5, dtype=dtype), _rand(g, n, dtype=dtype)
-        r = _rand(g, m, n, dtype=dtype)
-        assert _choice(x, w)[1].bm == 256
-        y = linear(x, w, b, activation="gelu_tanh", residual=r)
-        # a band of rows and a band of columns, both with the ragged edge: the 64-bit product of all is slow here
-        rows = torch.cat([torch.arange(0, 40), torch.arange(m - 300, m)]).cuda()
-        want, bound, _, _ = ref.linear_ref(x[rows], w, b, r[rows], "gelu_tanh", dtype)
-        assert_within(y[rows], want, bound, "rows")
-        cols = torch.cat([torch.arange(0, 40), torch.arange(n - 300, n)]).cuda()
-        want, bound, _, _ = ref.linear_ref(x, w[cols], b[cols], r[:, cols], "gelu_tanh", dtype)
-        assert_within(y[:, cols], want, bound, "columns")
+    m, n, k = shape
+    g = _gen(m + n + k)
+    x, w, b = _rand(g, m, k, dtype=dtype), _rand(g, n, k, scale=k ** -0.5, dtype=dtype), _rand(g, n, dtype=dtype)
+    r = _rand(g, m, n, dtype=dtype)
+    c = _choice(x, w)[1]
+    assert (c.bm, c.k_slices > 1, c.steps_ahead) == (bm, slices > 1, ahead)
+    _band_check(x, w, b, r, linear(x, w, b, activation="gelu_tanh", residual=r), "gelu_tanh", dtype)
 
 
 # ------------------------------------------------------------------ linear, backward
@@ -218,6 +219,23 @@ def test_linear_backward(m, n, k, dtype):
             assert_within(got["b"], *db, f"db {act}")
         if r is not None:
             assert torch.equal(got["r"], dy.to(res_dtype))
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("m,n,k", [(4096, 2048, 4096), (4100, 2056, 4104), (2048, 2048, 2048), (4100, 1032, 2056)])
+def test_linear_backward_large(m, n, k, dtype):
+    """The products of the backward pass on the larger tiles: bands of dx and dweight."""
+    from yolo_amd.layers import linear
+    g = _gen(m + n * 5 + k)
+    x = _rand(g, m, k, dtype=dtype).requires_grad_()
+    w = _rand(g, n, k, scale=k ** -0.5, dtype=dtype).requires_grad_()
+    dy = _rand(g, m, n, dtype=dtype)
+    dx, dw = torch.autograd.grad(linear(x, w), (x, w), dy)
+    rows, cols = torch.tensor([0, 1, 130, m - 257, m - 2, m - 1]).cuda(), torch.tensor([0, 1, 130, n - 257, n - 2, n - 1]).cuda()
+    d64, w64, x64 = dy.double(), w.detach().double(), x.detach().double()
+    for got, a, c, terms in ((dx[rows], d64[rows], w64, n), (dw[cols], d64[:, cols].t(), x64, m)):
+        want, mag = a @ c, a.abs() @ c.abs()
+        assert_within(got, want.cpu(), rounded(want, (terms + 4) * 2.0 ** -23 * mag, dtype).cpu(), "band")
 
 
 def test_linear_backward_one_gradient_at_a_time():

@@ -117,7 +117,7 @@ class LinearDesc(ctypes.Structure):
 class LinearChoice(ctypes.Structure):
     """yolo_amd_linear_choice of include/yolo_amd.h."""
     _fields_ = [("kernel", ctypes.c_int), ("bm", ctypes.c_int), ("bn", ctypes.c_int), ("k_slices", ctypes.c_int),
-                ("copies_x", ctypes.c_int), ("copies_weight", ctypes.c_int)]
+                ("copies_x", ctypes.c_int), ("copies_weight", ctypes.c_int), ("steps_ahead", ctypes.c_int)]
 
 
 class LinearBackwardDesc(ctypes.Structure):

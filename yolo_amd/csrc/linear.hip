@@ -59,21 +59,73 @@ __device__ __forceinline__ float erfc_scaled(float p, float& e) {
     return q * t * e;
 }
 
+// max(p, 0) in one instruction (fmaxf would canonicalise p first); 0 for NaN
+__device__ __forceinline__ float max0(float p) {
+    float r;
+    asm("v_max_f32 %0, %1, 0" : "=v"(r) : "v"(p));
+    return r;
+}
+
 template <int ACT>
 __device__ __forceinline__ float act_value(float p) {
     if constexpr (ACT == YOLO_AMD_ACT_LEAKY) return p > 0.f ? p : 0.1f * p;
     if constexpr (ACT == YOLO_AMD_ACT_RELU) return p < 0.f ? 0.f : p;
     if constexpr (ACT == YOLO_AMD_ACT_GELU) {
-        // max(p, 0) - |p| erfc(|p| / sqrt 2) / 2; the clamp keeps inf * 0 out (erfc is 0 from 15 on)
+        // max(p, 0) - |p| erfc(|p| / sqrt 2) / 2; the clamp keeps inf * 0 out (erfc is 0 from 15 on), NaN comes through q
         float e;
         const float q = erfc_scaled(p, e);
-        return fmaf(fminf(fabsf(p), 100.f) * -0.5f, q, p < 0.f ? 0.f : p);
+        return fmaf(fabsf(__builtin_amdgcn_fmed3f(p, -100.f, 100.f)) * q, -0.5f, max0(p));
     }
     // (1 + tanh z) / 2 = 1 / (1 + exp(-2 z))
     if constexpr (ACT == YOLO_AMD_ACT_GELU_TANH)
         return p * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(p * fmaf(p * p, -2.f * kLog2e * kGeluC * kGeluA, -2.f * kLog2e * kGeluC)));
     if constexpr (ACT == YOLO_AMD_ACT_SILU) return p * sigmoid_fast(p);
     return p;
+}
+// Eight of them, stage by stage: one after the other, as the compiler likes to order them, every element waits for its
+// own exponential and reciprocal, and an epilogue with one wave per SIMD has nothing else to run meanwhile.
+template <int ACT>
+__device__ __forceinline__ void act_values(float (&v)[2][4]) {
+#define YA_EACH _Pragma("unroll") for (int i = 0; i < 8; ++i)
+#define YA_STAGE() __builtin_amdgcn_sched_barrier(0)
+    float* p = &v[0][0];
+    if constexpr (ACT == YOLO_AMD_ACT_GELU) {
+        float t[8], e[8], q[8];
+        YA_EACH t[i] = fmaf(fabsf(p[i]), 0.3275911f * 0.70710678118654752f, 1.f);
+        YA_STAGE();
+        YA_EACH t[i] = __builtin_amdgcn_rcpf(t[i]);
+        YA_EACH e[i] = p[i] * p[i] * (-0.5f * kLog2e);
+        YA_STAGE();
+        YA_EACH e[i] = __builtin_amdgcn_exp2f(e[i]);
+        YA_EACH q[i] = fmaf(t[i], 1.061405429f, -1.453152027f);
+        YA_STAGE();
+        YA_EACH q[i] = fmaf(q[i], t[i], 1.421413741f);
+        YA_STAGE();
+        YA_EACH q[i] = fmaf(q[i], t[i], -0.284496736f);
+        YA_STAGE();
+        YA_EACH q[i] = fmaf(q[i], t[i], 0.254829592f);
+        YA_STAGE();
+        YA_EACH q[i] = q[i] * t[i] * e[i];
+        YA_STAGE();
+        YA_EACH p[i] = fmaf(fabsf(__builtin_amdgcn_fmed3f(p[i], -100.f, 100.f)) * q[i], -0.5f, max0(p[i]));
+    } else if constexpr (ACT == YOLO_AMD_ACT_GELU_TANH || ACT == YOLO_AMD_ACT_SILU) {
+        float z[8];
+        if constexpr (ACT == YOLO_AMD_ACT_SILU) {
+            YA_EACH z[i] = p[i] * -kLog2e;
+        } else {
+            YA_EACH z[i] = p[i] * fmaf(p[i] * p[i], -2.f * kLog2e * kGeluC * kGeluA, -2.f * kLog2e * kGeluC);
+        }
+        YA_STAGE();
+        YA_EACH z[i] = 1.f + __builtin_amdgcn_exp2f(z[i]);
+        YA_STAGE();
+        YA_EACH z[i] = __builtin_amdgcn_rcpf(z[i]);
+        YA_STAGE();
+        YA_EACH p[i] *= z[i];
+    } else {
+        YA_EACH p[i] = act_value<ACT>(p[i]);
+    }
+#undef YA_EACH
+#undef YA_STAGE
 }
 __device__ __forceinline__ float act_value(float p, int act) {
     switch (act) {
@@ -158,6 +210,16 @@ __device__ __forceinline__ void store1(void* p, long long at, int f32, float v) 
     else ((T*)p)[at] = (T)v;
 }
 
+// One sum of row m, column n: bias, activation, residual, one rounding, store.
+template <typename T>
+__device__ __forceinline__ void finish1(const Epilogue& e, long long m, int n, float s) {
+    if (e.bias) s += load1<T>(e.bias, n, e.bias_f32);
+    if (e.pre) store1<T>(e.pre, m * e.ldp + n, 0, s);
+    s = act_value(s, e.act);
+    if (e.res) s += load1<T>(e.res, m * e.ldr + n, e.res_f32);
+    store1<T>(e.y, m * e.ldy + n, e.y_f32, s);
+}
+
 // Eight sums of row m, columns n .. n + 7 (n a multiple of 8, n < N): bias, activation, residual, one
 // rounding, store.
 template <typename T>
@@ -184,16 +246,8 @@ __device__ __forceinline__ void finish8(const Epilogue& e, long long m, int n, i
         return;
     }
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        if (n + i < N) {
-            float s = v[i];
-            if (e.bias) s += load1<T>(e.bias, n + i, e.bias_f32);
-            if (e.pre) store1<T>(e.pre, m * e.ldp + n + i, 0, s);
-            s = act_value(s, e.act);
-            if (e.res) s += load1<T>(e.res, m * e.ldr + n + i, e.res_f32);
-            store1<T>(e.y, m * e.ldy + n + i, e.y_f32, s);
-        }
-    }
+    for (int i = 0; i < 8; ++i)
+        if (n + i < N) finish1<T>(e, m, n + i, v[i]);
 }
 
 // ---- from the accumulators of a wave, without LDS
@@ -307,10 +361,7 @@ __device__ __forceinline__ void finish_direct(const Epilogue& e, f32x4 (&acc)[TM
                 const u32x4 o = pair_out<T>(v);
                 if (in8) *reinterpret_cast<u32x4*>((T*)e.pre + m * e.ldp + n + c8) = o;
             }
-#pragma unroll
-            for (int h = 0; h < 2; ++h)
-#pragma unroll
-                for (int k = 0; k < 4; ++k) v[h][k] = act_value<ACT>(v[h][k]);
+            act_values<ACT>(v);
             if (res_t) {
                 float r[2][4];
                 pair_in<T>(now[p], r);
@@ -357,10 +408,17 @@ constexpr uint32_t kBufferBytes = 0x80000000u;   // descriptor size: offsets bui
 //   TR = false: contiguous along k in memory.  Image: R rows of 128 bytes, 16-byte chunk c of row r at
 //     position c ^ (r & 7): the 16 lanes of a fragment read then hit 8 different bank groups.
 //   TR = true: contiguous along R.  Image: 64 rows (k) of 2R bytes, 16-byte chunk c of row k at position
-//     c ^ 2 f(k), f(k) = (k & 3) | (k >> 3 & 1) << 2: the 32 lanes that one transposing read serves at a time
-//     (4 k-rows x 2 groups of 8 k apart, 32 bytes each) then cover all 64 banks once.
+//     c ^ 2 f(k), f(k) = (k & 3) | (k >> 3 & 1) << 2 for R >= 128, (k >> 1 & 1) | (k >> 3 & 1) << 1 for R = 64: the
+//     32 lanes that one transposing read serves at a time (4 k-rows x 2 groups of 8 k apart, 32 bytes each) then
+//     cover all 64 banks once.
 // Rows past the operand's end and reduction indices past K are read as zero through the buffer
 // descriptor's range check, so no tile reads outside its matrix.
+template <int R>
+__device__ __forceinline__ int k_swizzle(int k) {
+    static_assert(R == 64 || R % 128 == 0, "rows of half or whole bank widths");
+    return R == 64 ? (k >> 1 & 1) | (k >> 3 & 1) << 1 : (k & 3) | (k >> 3 & 1) << 2;
+}
+
 template <int R, int W, bool TR>
 struct Operand {
     static constexpr int NI = R / 8 / W;          // LDS-DMA instructions (1 KiB each) per wave and step
@@ -384,15 +442,13 @@ struct Operand {
             step = kBK * 2;
         } else {
             constexpr int CPR = R / 8, RPI = 64 / CPR;     // chunks per row, rows per instruction
-            // f(k) of instruction j: k advances by W * RPI, a multiple of 8; where it is an odd one, bit 3 changes
-            static_assert((W * RPI) % 8 == 0, "only bit 2 of f(k) differs between a lane's instructions");
             const int k = w * RPI + lane / CPR;
             kfirst = k;
             kstride = W * RPI;
 #pragma unroll
             for (int j = 0; j < NI; ++j) {
                 const int kj = k + j * W * RPI;
-                const int c = (lane % CPR) ^ (((kj & 3) | ((kj >> 3 & 1) << 2)) << 1);
+                const int c = (lane % CPR) ^ (k_swizzle<R>(kj) << 1);
                 voff[j] = row0 + c * 8 < extent ? (uint32_t)(kj * (uint32_t)ld * 2u) + c * 16u : kBufferNowhere;
             }
             base = (const char*)p + ((long long)kbeg * ld + row0) * 2;
@@ -411,6 +467,11 @@ struct Operand {
             __builtin_amdgcn_make_buffer_rsrc((void*)base, 0, (int)kBufferBytes, (int)kRawBufferWord3);
         lds_dma16_buf(rs, voff[j], 0, buf + (j * W + w) * 1024);
     }
+    // the same in two parts with other instructions between them
+    __device__ __forceinline__ void target(int j, char* buf, int w) const { lds_dma_to(buf + (j * W + w) * 1024); }
+    __device__ __forceinline__ void issue_here(int j) const {
+        lds_dma16_buf_here(__builtin_amdgcn_make_buffer_rsrc((void*)base, 0, (int)kBufferBytes, (int)kRawBufferWord3), voff[j], 0);
+    }
 };
 
 // fragment reads: 16 rows x 32 reduction indices; lane l holds row (l & 15), indices (l >> 4) * 8 ..
@@ -422,7 +483,7 @@ struct Fragments {
             at0 = (row0 + (lane & 15)) * 128 + (((lane >> 4) ^ (lane & 7)) << 4);
         } else {
             const int g = lane >> 4, j = lane & 15;
-            const int f = (j >> 2) | ((g & 1) << 2);
+            const int f = k_swizzle<R>(g * 8 + (j >> 2));
             at0 = (uint32_t)((g * 8 + (j >> 2)) * (R * 2) + (((row0 >> 4) ^ f) << 5) + ((j & 3) << 3));
         }
     }
@@ -440,14 +501,18 @@ struct Fragments {
     }
 };
 
-template <typename T, int BM, int BN, bool AT, bool BT>
-__global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(BM == 256 ? 1 : 2, BM == 256 ? 1 : 2)))
+// Workgroups (of one wave per SIMD) that a CU's 160 KB of LDS hold.
+constexpr int tile_occupancy(int b, int ahead) { return 163840 / ((2 * ahead + 1) * b * kBK * 2); }
+
+template <typename T, int BM, int BN, int AHEAD, bool AT, bool BT>
+__global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(tile_occupancy(BM, AHEAD), tile_occupancy(BM, AHEAD))))
 linear_tile_kernel(const TileArgs a) {
     constexpr int WM = 2, WN = 2, W = WM * WN, NT = W * 64;
     constexpr int WTM = BM / WM, WTN = BN / WN, TM = WTM / 16, TN = WTN / 16;
     typedef Operand<BM, W, AT> OpA;
     typedef Operand<BN, W, BT> OpB;
-    constexpr int RING = 5 * OpA::BYTES;
+    constexpr int SLOTS = 2 * AHEAD + 1, RING = SLOTS * OpA::BYTES;
+    constexpr bool IN_PLACE = tile_occupancy(BM, AHEAD) == 1;
     constexpr int PER = OpA::NI + OpB::NI;             // loads per wave and step
     constexpr int CROWS = WM * 32, CLD = BN + 4;       // epilogue chunk: 32 rows per wave row, fp32
     static_assert(RING >= CROWS * CLD * 4, "the epilogue's chunk fits into the ring");
@@ -488,17 +553,20 @@ linear_tile_kernel(const TileArgs a) {
 #pragma unroll
         for (int j = 0; j < TN; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
 
-    // A ring of five operand tiles in LDS -- A(t), B(t), A(t+1), B(t+1), A(t+2) in turn -- and two sets of fragments in
-    // registers.  The matrix instructions of half a step (32 reduction indices) run while the fragments of the next
+    // A ring of 2 AHEAD + 1 operand tiles in LDS -- A(t), B(t), A(t+1), B(t+1), .. in turn -- and two sets of fragments
+    // in registers.  The matrix instructions of half a step (32 reduction indices) run while the fragments of the next
     // half are read; in the middle of step t a barrier says that every wave has read its last fragments of A(t) and
-    // B(t), whose places B(t+2) and A(t+3) take over the next two halves, one load (1 KiB) after every eighth matrix
-    // instruction: with one wave per SIMD a load that finds the memory pipe busy holds up the matrix unit, and evenly
+    // B(t), whose places B(t + AHEAD) and A(t + 1 + AHEAD) take over the next two halves, one load (1 KiB) after every
+    // eighth matrix instruction of the 256-wide tile: with one wave per SIMD a load that finds the memory pipe busy holds up the matrix unit, and evenly
     // spaced loads do that least (8192^3: all of a step's loads in one eighth of it 872 us, in a quarter 836, in a
     // half 813).  The instruction stream is held in the order written by scheduling fences.
-    constexpr int GROUPS = TM * TN / 4, READS = TM + TN;
+    // the reads and loads spread one by one between the matrix instructions: a wave issues an instruction every four
+    // cycles and a matrix instruction occupies its unit for sixteen, so three others fit behind each and no more.
+    constexpr int PRODUCTS = TM * TN, READS = TM + TN;
     constexpr int TILE = OpA::BYTES;
-    static_assert(OpA::BYTES == OpB::BYTES && GROUPS % OpA::NI == 0, "slots of one size, loads evenly spaced");
-    constexpr int SPACE = GROUPS / OpA::NI;
+    static_assert(OpA::BYTES == OpB::BYTES && PRODUCTS % OpA::NI == 0, "slots of one size, loads evenly spaced");
+    constexpr int SPACE = PRODUCTS / OpA::NI, TARGET_AT = SPACE > 2 ? SPACE - 3 : 0;
+    static_assert(TARGET_AT + 1 < SPACE, "a load's two parts lie in one interval");
     int left_a = kend - kbeg, left_b = left_a;
     auto limit_a = [&]() {
         if (left_a < kBK) opa.limit(left_a);
@@ -516,25 +584,22 @@ linear_tile_kernel(const TileArgs a) {
         left_b -= kBK;
         limit_b();
     };
-    // slot two on (one step), as byte offsets
-    auto two_on = [](int slot) { return slot >= 3 * TILE ? slot - 3 * TILE : slot + 2 * TILE; };
+    // the slot two on (one step), as byte offsets
+    auto two_on = [](int slot) { return slot >= (SLOTS - 2) * TILE ? slot - (SLOTS - 2) * TILE : slot + 2 * TILE; };
     auto fetch = [&](v8<T> (&fr)[READS], int q, const char* ta, const char* tb, int s) {     // B's fragments, then A's
         fr[q] = q < TN ? fb.get(tb, q, s) : fa.get(ta, q - TN, s);
     };
-    auto products = [&](const v8<T> (&fr)[READS], int g) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const int i = (g * 4 + e) / TN, j = (g * 4 + e) % TN;
-            if constexpr (BM == 256) mfma_in_place(fr[j], fr[TN + i], acc[i][j]);
-            else acc[i][j] = mfma(fr[j], fr[TN + i], acc[i][j]);
-        }
+    auto product = [&](const v8<T> (&fr)[READS], int e) {
+        const int i = e / TN, j = e % TN;
+        if constexpr (IN_PLACE) mfma_in_place(fr[j], fr[TN + i], acc[i][j]);
+        else acc[i][j] = mfma(fr[j], fr[TN + i], acc[i][j]);
     };
 #define YA_FENCE() __builtin_amdgcn_sched_barrier(0)
     v8<T> f0[READS], f1[READS];
     limit_a();
     limit_b();
 #pragma unroll
-    for (int t = 0; t < 2; ++t) {
+    for (int t = 0; t < AHEAD; ++t) {
 #pragma unroll
         for (int q = 0; q < OpA::NI; ++q) opa.issue(q, lds + t * 2 * TILE, w);
 #pragma unroll
@@ -542,42 +607,42 @@ linear_tile_kernel(const TileArgs a) {
         next_a();
         next_b();
     }
-    wait_vmcnt<PER>();
+    wait_vmcnt<(AHEAD - 1) * PER>();
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
 #pragma unroll
     for (int q = 0; q < READS; ++q) fetch(f0, q, lds, lds + TILE, 0);
-    int sa = 0, sb = TILE, fill = 4 * TILE;            // slots of A(t), B(t), A(t+2)
+    int sa = 0, sb = TILE, fill = (SLOTS - 1) * TILE;  // slots of A(t), B(t), A(t + AHEAD)
     for (int t = 0; t < nt; ++t) {
         // first half: the second half's fragments in the first three quarters of it
-        constexpr int RPG = (READS * 4 + GROUPS * 3 - 1) / (GROUPS * 3);
 #pragma unroll
-        for (int g = 0; g < GROUPS; ++g) {
-            if (g % SPACE == 0) opa.issue(g / SPACE, lds + fill, w);
+        for (int e = 0; e < PRODUCTS; ++e) {
+            product(f0, e);
 #pragma unroll
-            for (int q = g * RPG; q < (g + 1) * RPG; ++q)
-                if (q < READS) fetch(f1, q, lds + sa, lds + sb, 1);
-            products(f0, g);
+            for (int q = 0; q < READS; ++q)
+                if (q * PRODUCTS / (READS * 2) == e) fetch(f1, q, lds + sa, lds + sb, 1);
+            if (e % SPACE == TARGET_AT) opa.target(e / SPACE, lds + fill, w);
+            if (e % SPACE == TARGET_AT + 1) opa.issue_here(e / SPACE);
             YA_FENCE();
         }
         next_a();
-        // this wave's reads of A(t) and B(t) have returned and its loads of A(t+1) and B(t+1) landed (those of A(t+2)
-        // may be on their way); then everybody's
-        wait_vmcnt<OpA::NI>();
+        // this wave's reads of A(t) and B(t) have returned and its loads of A(t+1) and B(t+1) landed (those of
+        // A(t+2 .. t + AHEAD) and B(t+2 .. t + AHEAD - 1) may be on their way); then everybody's
+        wait_vmcnt<(AHEAD - 1) * OpA::NI + (AHEAD - 2) * OpB::NI>();
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
         YA_FENCE();
         // second half: the next step's first fragments
-        constexpr int RPG2 = (READS + GROUPS - 1) / GROUPS;
         const int na = two_on(sa), nb = two_on(sb);
 #pragma unroll
-        for (int g = 0; g < GROUPS; ++g) {
-            if (g % SPACE == 0) opb.issue(g / SPACE, lds + sa, w);
+        for (int e = 0; e < PRODUCTS; ++e) {
+            product(f1, e);
 #pragma unroll
-            for (int q = g * RPG2; q < (g + 1) * RPG2; ++q)
-                if (q < READS) fetch(f0, q, lds + na, lds + nb, 0);
-            products(f1, g);
+            for (int q = 0; q < READS; ++q)
+                if (q * PRODUCTS / READS == e) fetch(f0, q, lds + na, lds + nb, 0);
+            if (e % SPACE == TARGET_AT) opb.target(e / SPACE, lds + sa, w);
+            if (e % SPACE == TARGET_AT + 1) opb.issue_here(e / SPACE);
             YA_FENCE();
         }
         next_b();
@@ -586,7 +651,7 @@ linear_tile_kernel(const TileArgs a) {
         sb = nb;
     }
 #undef YA_FENCE
-    if constexpr (BM == 256) mfma_drain();
+    if constexpr (IN_PLACE) mfma_drain();
     wait_vmcnt<0>();                                   // no load may land in the epilogue's LDS
 
     if (a.e.vec) {
@@ -598,21 +663,21 @@ linear_tile_kernel(const TileArgs a) {
             e.y_f32 = 1;
         }
         if constexpr (AT || BT) {
-            finish_direct<T, YOLO_AMD_ACT_NONE, BM == 256>(e, acc, mw, nw, a.M, a.N, lane);
+            finish_direct<T, YOLO_AMD_ACT_NONE, IN_PLACE>(e, acc, mw, nw, a.M, a.N, lane);
         } else {
             switch (e.act) {
-                case YOLO_AMD_ACT_LEAKY: finish_direct<T, YOLO_AMD_ACT_LEAKY, BM == 256>(e, acc, mw, nw, a.M, a.N, lane); break;
-                case YOLO_AMD_ACT_RELU: finish_direct<T, YOLO_AMD_ACT_RELU, BM == 256>(e, acc, mw, nw, a.M, a.N, lane); break;
-                case YOLO_AMD_ACT_GELU: finish_direct<T, YOLO_AMD_ACT_GELU, BM == 256>(e, acc, mw, nw, a.M, a.N, lane); break;
-                case YOLO_AMD_ACT_GELU_TANH: finish_direct<T, YOLO_AMD_ACT_GELU_TANH, BM == 256>(e, acc, mw, nw, a.M, a.N, lane); break;
-                case YOLO_AMD_ACT_SILU: finish_direct<T, YOLO_AMD_ACT_SILU, BM == 256>(e, acc, mw, nw, a.M, a.N, lane); break;
-                default: finish_direct<T, YOLO_AMD_ACT_NONE, BM == 256>(e, acc, mw, nw, a.M, a.N, lane); break;
+                case YOLO_AMD_ACT_LEAKY: finish_direct<T, YOLO_AMD_ACT_LEAKY, IN_PLACE>(e, acc, mw, nw, a.M, a.N, lane); break;
+                case YOLO_AMD_ACT_RELU: finish_direct<T, YOLO_AMD_ACT_RELU, IN_PLACE>(e, acc, mw, nw, a.M, a.N, lane); break;
+                case YOLO_AMD_ACT_GELU: finish_direct<T, YOLO_AMD_ACT_GELU, IN_PLACE>(e, acc, mw, nw, a.M, a.N, lane); break;
+                case YOLO_AMD_ACT_GELU_TANH: finish_direct<T, YOLO_AMD_ACT_GELU_TANH, IN_PLACE>(e, acc, mw, nw, a.M, a.N, lane); break;
+                case YOLO_AMD_ACT_SILU: finish_direct<T, YOLO_AMD_ACT_SILU, IN_PLACE>(e, acc, mw, nw, a.M, a.N, lane); break;
+                default: finish_direct<T, YOLO_AMD_ACT_NONE, IN_PLACE>(e, acc, mw, nw, a.M, a.N, lane); break;
             }
         }
         return;
     }
     // Rows of y that do not start on 16-byte boundaries, or N no multiple of 8: the accumulators go through LDS in
-    // fp32, 32 rows of every wave row at a time, and are finished by element.
+    // fp32, 32 rows of every wave row at a time, and are finished by element, a wave along a row.
     float* out = reinterpret_cast<float*>(lds);
 #pragma unroll
     for (int c = 0; c < WTM / 32; ++c) {
@@ -620,43 +685,49 @@ linear_tile_kernel(const TileArgs a) {
 #pragma unroll
         for (int i = 0; i < 2; ++i)
 #pragma unroll
-            for (int j = 0; j < TN; ++j)
-            {
+            for (int j = 0; j < TN; ++j) {
                 float v[4];
-                acc_read<BM == 256>(acc[c * 2 + i][j], v);
+                acc_read<IN_PLACE>(acc[c * 2 + i][j], v);
                 *reinterpret_cast<f32x4*>(out + (wm * 32 + i * 16 + (lane & 15)) * CLD + wn * WTN + j * 16 + (lane >> 4) * 4) =
                     f32x4{v[0], v[1], v[2], v[3]};
             }
         __syncthreads();
-        for (int it = threadIdx.x; it < CROWS * (BN / 8); it += NT) {
-            const int lr = it / (BN / 8), n = n0 + (it % (BN / 8)) * 8;
+#pragma unroll 4
+        for (int it = threadIdx.x; it < CROWS * BN; it += NT) {
+            const int lr = it / BN, n = it % BN;
             const long long m = m0 + (lr >> 5) * WTM + c * 32 + (lr & 31);
-            if (m < a.M && n < a.N) {
-                float v[8];
-                load8<T>(out, lr * CLD + (n - n0), 1, v);
-                finish8<T>(a.e, m, n, a.N, v);
-            }
+            if (m < a.M && n0 + n < a.N) finish1<T>(a.e, m, n0 + n, out[lr * CLD + n]);
         }
     }
 }
 
-// Adds the K slices in ascending order and finishes: one thread per eight columns.
-template <typename T>
+// Adds the K slices in ascending order and finishes: a thread has eight columns, or, where rows of y are not whole and
+// aligned eights, one, so that a wave still runs along a row.
+template <typename T, int V>
 __global__ void __launch_bounds__(256)
-linear_finish_kernel(const Epilogue e, const float* part, int slices, int M, int N, int n8) {
-    const long long total = (long long)M * n8;
-    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < total; i += (long long)gridDim.x * 256) {
-        const long long m = i / n8;
-        const int n = (int)(i - m * n8) * 8;
-        float v[8];
-        load8<T>(part, m * e.ld_part + n, 1, v);
-        for (int s = 1; s < slices; ++s) {
-            float u[8];
-            load8<T>(part, s * e.slice_stride + m * e.ld_part + n, 1, u);
+linear_finish_kernel(const Epilogue e, const float* part, int slices, int M, int N) {
+    const int n = (blockIdx.x * 64 + (threadIdx.x & 63)) * V;
+    const int step = gridDim.y * 4;
+    if (n >= N) return;
+    for (int m = blockIdx.y * 4 + (threadIdx.x >> 6); m < M; m += step) {
+        const float* p = part + (long long)m * e.ld_part + n;
+        if constexpr (V == 8) {
+            float v[8];
+            load8<T>(p, 0, 1, v);
+#pragma unroll 4
+            for (int s = 1; s < slices; ++s) {
+                float u[8];
+                load8<T>(p, s * e.slice_stride, 1, u);
 #pragma unroll
-            for (int k = 0; k < 8; ++k) v[k] += u[k];
+                for (int k = 0; k < 8; ++k) v[k] += u[k];
+            }
+            finish8<T>(e, m, n, N, v);
+        } else {
+            float v = *p;
+#pragma unroll 4
+            for (int s = 1; s < slices; ++s) v += p[s * e.slice_stride];
+            finish1<T>(e, m, n, v);
         }
-        finish8<T>(e, m, n, N, v);
     }
 }
 
@@ -741,17 +812,24 @@ linear_rows_kernel(const TileArgs a) {
 // ---------------------------------------------------------------- operand copies
 // Rows of C elements at any stride and alignment -> rows of C rounded up to 8, zero filled: what the kernels
 // above need (16-byte chunks that never straddle a row's end).  One thread per chunk.
+struct PackArgs {
+    const void* src[2];
+    void* dst[2];
+    long long ld[2], chunks[2];
+    int cols[2], c8[2];
+};
 template <typename T>
 __global__ void __launch_bounds__(256)
-linear_pack_kernel(const T* src, long long ld, long long rows, int C, T* dst, int c8) {
-    const long long total = rows * c8;
-    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < total; i += (long long)gridDim.x * 256) {
-        const long long r = i / c8;
-        const int c = (int)(i - r * c8) * 8;
+linear_pack_kernel(const PackArgs a) {
+    const int w = blockIdx.y;
+    const T* src = (const T*)a.src[w];
+    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < a.chunks[w]; i += (long long)gridDim.x * 256) {
+        const long long r = i / a.c8[w];
+        const int c = (int)(i - r * a.c8[w]) * 8;
         v8<T> v;
 #pragma unroll
-        for (int k = 0; k < 8; ++k) v[k] = c + k < C ? src[r * ld + c + k] : (T)0.f;
-        *reinterpret_cast<v8<T>*>(dst + i * 8) = v;
+        for (int k = 0; k < 8; ++k) v[k] = c + k < a.cols[w] ? src[r * a.ld[w] + c + k] : (T)0.f;
+        *reinterpret_cast<v8<T>*>((T*)a.dst[w] + i * 8) = v;
     }
 }
 
@@ -778,6 +856,7 @@ linear_dpre_kernel(const DpreArgs a) {
     const long long r1 = min((long long)a.M, r0 + a.rows);
     float sum[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
     if (n < a.N) {
+#pragma unroll 2
         for (long long m = r0 + lane_r; m < r1; m += 8) {
             float d[8], p[8];
             if (a.vec) {
@@ -812,14 +891,25 @@ linear_dpre_kernel(const DpreArgs a) {
     }
 }
 
+// 64 columns per workgroup; wave w adds runs w, w + 16, .. in ascending order, the waves are added in order.
 template <typename T>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(1024)
 linear_dbias_kernel(const float* part, int blocks, int N, void* db, int db_f32) {
-    const int n = blockIdx.x * 256 + threadIdx.x;
-    if (n >= N) return;
+    __shared__ float red[16][64];
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+    const int n = blockIdx.x * 64 + lane;
     float s = 0.f;
-    for (int b = 0; b < blocks; ++b) s += part[(long long)b * N + n];
-    store1<T>(db, n, db_f32, s);
+    if (n < N) {
+#pragma unroll 8
+        for (int b = w; b < blocks; b += 16) s += part[(long long)b * N + n];
+    }
+    red[w][lane] = s;
+    __syncthreads();
+    if (w == 0 && n < N) {
+#pragma unroll
+        for (int i = 1; i < 16; ++i) s += red[i][lane];
+        store1<T>(db, n, db_f32, s);
+    }
 }
 
 // ---------------------------------------------------------------- host side
@@ -839,7 +929,25 @@ static size_t packed_bytes(const Matrix& m) {
 
 // Which kernel a product D[M][N] over K runs on.
 struct TilePlan {
-    int kernel, bm, bn, slices, ksteps;
+    int kernel, bm, bn, slices, ksteps, ahead;
+};
+
+// The tile kernels, with what a full round of workgroups takes (microseconds: start, prologue and epilogue; then each
+// step of 64 reduction indices), and a round that leaves at most one workgroup to a CU.  Fitted to bf16 products in
+// captured graphs, every kernel and split on 70 sizes from 33 x 64 x 64 to 8192^3: the choice they make is 1.0 % slower
+// than the fastest of each size (geometric mean; 22 % at the worst).  The 256-wide tile moves the fewest bytes per
+// product but wants a tile for every CU; 128 four steps ahead hides memory's latency where a CU has one workgroup
+// (4096 x 1024 x 4096: 38.8 against 46.1 us), two ahead lets two workgroups do that for each other (2048 x 4096 x 4096:
+// 69.5 against 76.6); 64 is for what has fewer than 256 tiles of 128 (1024^3: 7.4 against 12.8).
+struct TileConfig {
+    int b, ahead;
+    double start, step, start_1, step_1;
+};
+static const TileConfig kTileConfigs[] = {
+    {256, 2, 10.9, 1.44, 10.5, 1.04},
+    {128, 2, 4.0, 1.02, 4.4, 0.59},
+    {128, 4, 4.1, 0.54, 4.9, 0.52},
+    {64, 4, 3.2, 0.436, 3.1, 0.274},
 };
 
 static TilePlan plan_product(long long M, int N, long long K, bool kc_operands) {
@@ -854,20 +962,21 @@ static TilePlan plan_product(long long M, int N, long long K, bool kc_operands) 
         return p;
     }
     double best = 0;
-    for (int cfg = 0; cfg < 2; ++cfg) {
-        const int bt = cfg ? 128 : 256;
-        const long long tiles = ((M + bt - 1) / bt) * ((N + bt - 1) / bt);
-        const double slots = cfg ? 512 : 256, cyc = cfg ? 1700 : 2700;
+    for (const TileConfig& c : kTileConfigs) {
+        const long long tiles = ((M + c.b - 1) / c.b) * ((N + c.b - 1) / c.b);
+        const int slots = 256 * tile_occupancy(c.b, c.ahead);
         for (int s = 1; s <= 64 && s <= steps; ++s) {
-            const long long per = (steps + s - 1) / s;
+            const long long per = (steps + s - 1) / s, wgs = tiles * s, rest = wgs % slots;
             if ((steps + per - 1) / per != s) continue;
-            const double rounds = (double)((tiles * s + (long long)slots - 1) / (long long)slots);
-            double t = rounds * (per * cyc + 6000);
-            if (s > 1) t += 8000 + (double)s * M * N * 8 / 2000;    // partial sums out and back at about 4.5 TB/s
+            if (s > 1 && wgs > slots) break;           // a split only fills a round that is not full
+            double t = (double)(wgs / slots) * (c.start + per * c.step);
+            if (rest > 0) t += rest <= 256 ? c.start_1 + per * c.step_1 : c.start + per * c.step;
+            if (s > 1) t += 3.4 + 0.08 * s + (double)s * M * N * 2e-6;     // one more launch; partial sums out and in at 4 TB/s
             if (p.kernel == 0 || t < best) {
                 best = t;
                 p.kernel = YOLO_AMD_LINEAR_TILE;
-                p.bm = p.bn = bt;
+                p.bm = p.bn = c.b;
+                p.ahead = c.ahead;
                 p.slices = s;
                 p.ksteps = (int)per;
             }
@@ -880,12 +989,36 @@ static size_t partial_bytes(const TilePlan& p, long long M, int N) {
     return p.slices > 1 ? align_up((size_t)p.slices * M * align_up(N, 8) * 4, 256) : 0;
 }
 
+// Scratch of a call, handed out front to back.
+struct Scratch {
+    char* p;
+    void* take(size_t bytes) {
+        void* r = p;
+        p += bytes;
+        return r;
+    }
+};
+
+// Copies of the operands that want one (bytes > 0), in one launch.
 template <typename T>
-static void launch_pack(const Matrix& m, void* dst, hipStream_t s) {
-    const int c8 = (int)(align_up(m.cols, 8) / 8);
-    const long long total = m.rows * c8;
-    const unsigned blocks = (unsigned)std::min<long long>((total + 255) / 256, 1 << 16);
-    hipLaunchKernelGGL((linear_pack_kernel<T>), dim3(blocks), dim3(256), 0, s, (const T*)m.p, m.ld, m.rows, m.cols, (T*)dst, c8);
+static void launch_pack(Matrix (&m)[2], const size_t (&bytes)[2], Scratch& sc, hipStream_t s) {
+    PackArgs a{};
+    int n = 0;
+    for (int i = 0; i < 2; ++i) {
+        if (bytes[i] == 0) continue;
+        const int c8 = (int)(align_up(m[i].cols, 8) / 8);
+        a.src[n] = m[i].p;
+        a.dst[n] = sc.take(bytes[i]);
+        a.ld[n] = m[i].ld;
+        a.cols[n] = m[i].cols;
+        a.c8[n] = c8;
+        a.chunks[n] = m[i].rows * c8;
+        m[i] = Matrix{a.dst[n], c8 * 8, m[i].rows, c8 * 8};
+        ++n;
+    }
+    if (n == 0) return;
+    const long long most = std::max(a.chunks[0], a.chunks[1]);
+    hipLaunchKernelGGL((linear_pack_kernel<T>), dim3((unsigned)std::min<long long>((most + 255) / 256, 1 << 14), n), dim3(256), 0, s, a);
 }
 
 template <typename T, bool AT, bool BT>
@@ -914,15 +1047,18 @@ static int launch_product(const TilePlan& p, TileArgs a, void* partial, hipStrea
         a.e.slice_stride = a.e.ld_part * a.M;
     }
     const dim3 grid((unsigned)((long long)a.tiles_m * a.tiles_n), (unsigned)p.slices);
-    if (p.bm == 256) hipLaunchKernelGGL((linear_tile_kernel<T, 256, 256, AT, BT>), grid, dim3(256), 0, s, a);
-    else hipLaunchKernelGGL((linear_tile_kernel<T, 128, 128, AT, BT>), grid, dim3(256), 0, s, a);
+    if (p.bm == 256) hipLaunchKernelGGL((linear_tile_kernel<T, 256, 256, 2, AT, BT>), grid, dim3(256), 0, s, a);
+    else if (p.bm == 128 && p.ahead == 2) hipLaunchKernelGGL((linear_tile_kernel<T, 128, 128, 2, AT, BT>), grid, dim3(256), 0, s, a);
+    else if (p.bm == 128) hipLaunchKernelGGL((linear_tile_kernel<T, 128, 128, 4, AT, BT>), grid, dim3(256), 0, s, a);
+    else hipLaunchKernelGGL((linear_tile_kernel<T, 64, 64, 4, AT, BT>), grid, dim3(256), 0, s, a);
     if (p.slices > 1) {
         Epilogue f = e;
         f.ld_part = a.e.ld_part;
         f.slice_stride = a.e.slice_stride;
-        const long long total = (long long)a.M * (a.e.ld_part / 8);
-        hipLaunchKernelGGL((linear_finish_kernel<T>), dim3((unsigned)std::min<long long>((total + 255) / 256, 8192)), dim3(256), 0, s,
-                           f, (const float*)partial, p.slices, a.M, a.N, (int)(a.e.ld_part / 8));
+        const int cols = f.vec ? 512 : 64;
+        const dim3 fgrid((a.N + cols - 1) / cols, (unsigned)std::min<long long>((a.M + 3) / 4, 4096));
+        if (f.vec) hipLaunchKernelGGL((linear_finish_kernel<T, 8>), fgrid, dim3(256), 0, s, f, (const float*)partial, p.slices, a.M, a.N);
+        else hipLaunchKernelGGL((linear_finish_kernel<T, 1>), fgrid, dim3(256), 0, s, f, (const float*)partial, p.slices, a.M, a.N);
     }
     YA_CHECK_HIP(hipGetLastError());
     return YA_OK;
@@ -982,16 +1118,6 @@ static ForwardPlan plan_forward(const yolo_amd_linear_desc* d) {
     return f;
 }
 
-// Scratch of a call, handed out front to back.
-struct Scratch {
-    char* p;
-    void* take(size_t bytes) {
-        void* r = p;
-        p += bytes;
-        return r;
-    }
-};
-
 static int check_workspace(const char* what, const void* ws, size_t have, size_t need) {
     if (need == 0) return YA_OK;
     YA_REQUIRE(ws && ((uintptr_t)ws & 255) == 0, "%s: the workspace is null or not 256-byte aligned", what);
@@ -1003,22 +1129,15 @@ static int check_workspace(const char* what, const void* ws, size_t have, size_t
 }
 
 template <typename T>
-static Matrix packed(const Matrix& m, size_t bytes, Scratch& sc, hipStream_t s) {
-    if (bytes == 0) return m;
-    void* dst = sc.take(bytes);
-    launch_pack<T>(m, dst, s);
-    const int c8 = (int)align_up(m.cols, 8);
-    return Matrix{dst, c8, m.rows, c8};
-}
-
-template <typename T>
 static int forward(const yolo_amd_linear_desc* d, const ForwardPlan& f, hipStream_t s) {
     Scratch sc{(char*)d->workspace};
-    const Matrix x = packed<T>(f.x, f.x_bytes, sc, s), w = packed<T>(f.w, f.w_bytes, sc, s);
+    Matrix in[2] = {f.x, f.w};
+    launch_pack<T>(in, {f.x_bytes, f.w_bytes}, sc, s);
+    const Matrix &x = in[0], &w = in[1];
     TileArgs a{};
     a.A = x.p; a.lda = x.ld;
     a.B = w.p; a.ldb = w.ld;
-    a.M = (int)d->m; a.N = (int)d->n; a.K = std::min(x.cols, w.cols) ;
+    a.M = (int)d->m; a.N = (int)d->n; a.K = std::min(x.cols, w.cols);
     Epilogue& e = a.e;
     e.bias = d->bias; e.res = d->residual; e.y = d->y; e.pre = d->pre;
     e.ldr = d->ldr; e.ldy = d->ldy; e.ldp = d->n;
@@ -1121,7 +1240,7 @@ static int backward(const yolo_amd_linear_backward_desc* d, const BackwardPlan& 
         g.M = M; g.N = N; g.rows = b.rows;
         hipLaunchKernelGGL((linear_dpre_kernel<T>), dim3((N + 255) / 256, b.blocks), dim3(256), 0, s, g);
         if (d->dbias)
-            hipLaunchKernelGGL((linear_dbias_kernel<T>), dim3((N + 255) / 256), dim3(256), 0, s, db, b.blocks, N, d->dbias, d->dbias_f32);
+            hipLaunchKernelGGL((linear_dbias_kernel<T>), dim3((N + 63) / 64), dim3(1024), 0, s, db, b.blocks, N, d->dbias, d->dbias_f32);
     }
     const void* P = b.own_dp ? dp : d->dy;
     const long long ldP = b.own_dp ? (long long)align_up(N, 8) : d->lddy;
@@ -1130,8 +1249,9 @@ static int backward(const yolo_amd_linear_backward_desc* d, const BackwardPlan& 
         a.e.act = YOLO_AMD_ACT_NONE;
         a.e.vec = K % 8 == 0;
         a.e.ldy = K;
-        const Matrix w = d->dx ? packed<T>(b.w, b.w_bytes, sc, s) : Matrix{};
-        const Matrix x = d->dweight ? packed<T>(b.x, b.x_bytes, sc, s) : Matrix{};
+        Matrix in[2] = {b.x, b.w};
+        launch_pack<T>(in, {b.x_bytes, b.w_bytes}, sc, s);
+        const Matrix &x = in[0], &w = in[1];
         void* part = sc.take(b.part_bytes);
         if (d->dx) {
             a.A = P; a.lda = ldP;
@@ -1166,7 +1286,7 @@ extern "C" int yolo_amd_linear_query(const yolo_amd_linear_desc* d, yolo_amd_lin
     YA_REQUIRE(out, "linear_query: null output");
     YA_TRY(check_forward(d));
     const ForwardPlan f = plan_forward(d);
-    *out = yolo_amd_linear_choice{f.tile.kernel, f.tile.bm, f.tile.bn, f.tile.slices, f.x_bytes != 0, f.w_bytes != 0};
+    *out = yolo_amd_linear_choice{f.tile.kernel, f.tile.bm, f.tile.bn, f.tile.slices, f.x_bytes != 0, f.w_bytes != 0, f.tile.ahead};
     return YA_OK;
 }
 
