@@ -167,20 +167,23 @@ struct Epilogue {
     void* pre;             // [M][ldp] or null: P, rounded to T, for the backward pass
     long long ldr, ldy, ldp;
     int bias_f32, res_f32, y_f32, act;
-    int vec;               // every row of every tensor above starts on a 16-byte boundary and N % 8 == 0
     float* part;           // not null: the raw sums of one K slice go to [slice][M][ld_part] instead
     long long ld_part, slice_stride;
 };
 
+// Rows of a user's tensor may start anywhere: 16-byte accesses at the elements' own alignment (the machine takes them;
+// a wave that runs along a row touches one more line for it).
+typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));
+typedef uint32_t u32x4u __attribute__((ext_vector_type(4), aligned(2)));
 template <typename T>
 __device__ __forceinline__ void load8(const void* p, long long at, int f32, float (&v)[8]) {
     if (f32) {
-        const f32x4 a = *reinterpret_cast<const f32x4*>((const float*)p + at);
-        const f32x4 b = *reinterpret_cast<const f32x4*>((const float*)p + at + 4);
+        const f32x4u a = *reinterpret_cast<const f32x4u*>((const float*)p + at);
+        const f32x4u b = *reinterpret_cast<const f32x4u*>((const float*)p + at + 4);
 #pragma unroll
         for (int i = 0; i < 4; ++i) { v[i] = a[i]; v[4 + i] = b[i]; }
     } else {
-        const v8<T> a = *reinterpret_cast<const v8<T>*>((const T*)p + at);
+        const v8<T> a = __builtin_bit_cast(v8<T>, *reinterpret_cast<const u32x4u*>((const T*)p + at));
 #pragma unroll
         for (int i = 0; i < 8; ++i) v[i] = (float)a[i];
     }
@@ -188,16 +191,16 @@ __device__ __forceinline__ void load8(const void* p, long long at, int f32, floa
 template <typename T>
 __device__ __forceinline__ void store8(void* p, long long at, int f32, const float (&v)[8]) {
     if (f32) {
-        f32x4 a, b;
+        f32x4u a, b;
 #pragma unroll
         for (int i = 0; i < 4; ++i) { a[i] = v[i]; b[i] = v[4 + i]; }
-        *reinterpret_cast<f32x4*>((float*)p + at) = a;
-        *reinterpret_cast<f32x4*>((float*)p + at + 4) = b;
+        *reinterpret_cast<f32x4u*>((float*)p + at) = a;
+        *reinterpret_cast<f32x4u*>((float*)p + at + 4) = b;
     } else {
         v8<T> a;
 #pragma unroll
         for (int i = 0; i < 8; ++i) a[i] = (T)v[i];
-        *reinterpret_cast<v8<T>*>((T*)p + at) = a;
+        *reinterpret_cast<u32x4u*>((T*)p + at) = __builtin_bit_cast(u32x4u, a);
     }
 }
 template <typename T>
@@ -224,7 +227,7 @@ __device__ __forceinline__ void finish1(const Epilogue& e, long long m, int n, f
 // rounding, store.
 template <typename T>
 __device__ __forceinline__ void finish8(const Epilogue& e, long long m, int n, int N, float (&v)[8]) {
-    if (e.vec) {
+    if (n + 8 <= N) {
         if (e.bias) {
             float b[8];
             load8<T>(e.bias, n, e.bias_f32, b);
@@ -313,9 +316,12 @@ __device__ __forceinline__ void acc_read(f32x4& c, float (&v)[4]) {
     }
 }
 
-// The wave's rows m0 .. and columns n0 .. (e.vec holds).
+// The wave's rows m0 .. and columns n0 ...  Whole eights of columns (below NV = N rounded down) are stored from here; the
+// last one to seven columns of a row go, with bias and activation, through `tail` (LDS of this wave, [2][16 TM][8]:
+// outputs, pre-activations) and are finished by element behind the loop, in code that is short because it is cold.
 template <typename T, int ACT, bool IN_PLACE, int TM, int TN>
-__device__ __forceinline__ void finish_direct(const Epilogue& e, f32x4 (&acc)[TM][TN], int m0, int n0, int M, int N, int lane) {
+__device__ __forceinline__ void finish_direct(const Epilogue& e, f32x4 (&acc)[TM][TN], int m0, int n0, int M, int N, int NV,
+                                              int lane, float* tail) {
     const int row = lane & 15, c4 = (lane >> 4) * 4, c8 = (lane >> 4) * 8;
     float bias[TN][4];
 #pragma unroll
@@ -323,9 +329,9 @@ __device__ __forceinline__ void finish_direct(const Epilogue& e, f32x4 (&acc)[TM
         const int n = n0 + j * 16 + c4;
 #pragma unroll
         for (int k = 0; k < 4; ++k) bias[j][k] = 0.f;
-        if (e.bias && n < N) {
+        if (e.bias) {
 #pragma unroll
-            for (int k = 0; k < 4; ++k) bias[j][k] = load1<T>(e.bias, n + k, e.bias_f32);
+            for (int k = 0; k < 4; ++k) bias[j][k] = load1<T>(e.bias, min(n + k, N - 1), e.bias_f32);
         }
     }
     u32x4 ahead[TN / 2];                               // the next rows' residual, if it has T's size
@@ -334,7 +340,7 @@ __device__ __forceinline__ void finish_direct(const Epilogue& e, f32x4 (&acc)[TM
 #pragma unroll
         for (int p = 0; p < TN / 2; ++p) {
             const int n = n0 + p * 32 + c8;
-            if (m < M && n < N) ahead[p] = *reinterpret_cast<const u32x4*>((const T*)e.res + m * e.ldr + n);
+            if (m < M && n < NV) ahead[p] = *reinterpret_cast<const u32x4u*>((const T*)e.res + m * e.ldr + n);
         }
     };
     const bool res_t = e.res && !e.res_f32;
@@ -349,7 +355,8 @@ __device__ __forceinline__ void finish_direct(const Epilogue& e, f32x4 (&acc)[TM
 #pragma unroll
         for (int p = 0; p < TN / 2; ++p) {
             const int n = n0 + p * 32;
-            const bool in8 = m < M && n + c8 < N;
+            const bool in8 = m < M && n + c8 < NV;
+            const bool ends = tail && n <= NV && NV < n + 32;          // the last columns are among these (wave-uniform)
             float v[2][4];
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
@@ -357,11 +364,20 @@ __device__ __forceinline__ void finish_direct(const Epilogue& e, f32x4 (&acc)[TM
 #pragma unroll
                 for (int k = 0; k < 4; ++k) v[h][k] += bias[p * 2 + h][k];
             }
+            auto to_tail = [&](float* t) {
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const int c = n + h * 16 + c4 - NV;
+                    if (c >= 0 && c < 8) *reinterpret_cast<f32x4*>(t + (i * 16 + row) * 8 + c) = f32x4{v[h][0], v[h][1], v[h][2], v[h][3]};
+                }
+            };
             if (e.pre) {
+                if (ends) to_tail(tail + TM * 16 * 8);
                 const u32x4 o = pair_out<T>(v);
-                if (in8) *reinterpret_cast<u32x4*>((T*)e.pre + m * e.ldp + n + c8) = o;
+                if (in8) *reinterpret_cast<u32x4u*>((T*)e.pre + m * e.ldp + n + c8) = o;
             }
             act_values<ACT>(v);
+            if (ends) to_tail(tail);
             if (res_t) {
                 float r[2][4];
                 pair_in<T>(now[p], r);
@@ -372,8 +388,8 @@ __device__ __forceinline__ void finish_direct(const Epilogue& e, f32x4 (&acc)[TM
             } else if (e.res) {
 #pragma unroll
                 for (int h = 0; h < 2; ++h)
-                    if (m < M && n + h * 16 + c4 < N) {
-                        const f32x4 r = *reinterpret_cast<const f32x4*>((const float*)e.res + m * e.ldr + n + h * 16 + c4);
+                    if (m < M && n + h * 16 + c4 < NV) {
+                        const f32x4 r = *reinterpret_cast<const f32x4u*>((const float*)e.res + m * e.ldr + n + h * 16 + c4);
 #pragma unroll
                         for (int k = 0; k < 4; ++k) v[h][k] += r[k];
                     }
@@ -381,12 +397,26 @@ __device__ __forceinline__ void finish_direct(const Epilogue& e, f32x4 (&acc)[TM
             if (e.y_f32) {
 #pragma unroll
                 for (int h = 0; h < 2; ++h)
-                    if (m < M && n + h * 16 + c4 < N)
-                        *reinterpret_cast<f32x4*>((float*)e.y + m * e.ldy + n + h * 16 + c4) = f32x4{v[h][0], v[h][1], v[h][2], v[h][3]};
+                    if (m < M && n + h * 16 + c4 < NV)
+                        *reinterpret_cast<f32x4u*>((float*)e.y + m * e.ldy + n + h * 16 + c4) = f32x4{v[h][0], v[h][1], v[h][2], v[h][3]};
             } else {
                 const u32x4 o = pair_out<T>(v);
-                if (in8) *reinterpret_cast<u32x4*>((T*)e.y + m * e.ldy + n + c8) = o;
+                if (in8) *reinterpret_cast<u32x4u*>((T*)e.y + m * e.ldy + n + c8) = o;
             }
+        }
+    }
+    if (!tail || n0 > NV || NV >= n0 + TN * 16) return;
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");                 // this wave's own writes
+    const int c = lane & 7;
+    if (c >= N - NV) return;
+#pragma unroll 4
+    for (int r = lane >> 3; r < TM * 16; r += 8) {
+        const long long m = (long long)m0 + r;
+        if (m < M) {
+            float s = tail[r * 8 + c];
+            if (e.res) s += load1<T>(e.res, m * e.ldr + NV + c, e.res_f32);
+            if (e.pre) store1<T>(e.pre, m * e.ldp + NV + c, 0, tail[TM * 16 * 8 + r * 8 + c]);
+            store1<T>(e.y, m * e.ldy + NV + c, e.y_f32, s);
         }
     }
 }
@@ -507,15 +537,14 @@ constexpr int tile_occupancy(int b, int ahead) { return 163840 / ((2 * ahead + 1
 template <typename T, int BM, int BN, int AHEAD, bool AT, bool BT>
 __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(tile_occupancy(BM, AHEAD), tile_occupancy(BM, AHEAD))))
 linear_tile_kernel(const TileArgs a) {
-    constexpr int WM = 2, WN = 2, W = WM * WN, NT = W * 64;
+    constexpr int WM = 2, WN = 2, W = WM * WN;
     constexpr int WTM = BM / WM, WTN = BN / WN, TM = WTM / 16, TN = WTN / 16;
     typedef Operand<BM, W, AT> OpA;
     typedef Operand<BN, W, BT> OpB;
     constexpr int SLOTS = 2 * AHEAD + 1, RING = SLOTS * OpA::BYTES;
     constexpr bool IN_PLACE = tile_occupancy(BM, AHEAD) == 1;
     constexpr int PER = OpA::NI + OpB::NI;             // loads per wave and step
-    constexpr int CROWS = WM * 32, CLD = BN + 4;       // epilogue chunk: 32 rows per wave row, fp32
-    static_assert(RING >= CROWS * CLD * 4, "the epilogue's chunk fits into the ring");
+    static_assert(RING >= W * 2 * WTM * 8 * 4, "the epilogue's last columns fit into the ring");
     __shared__ __attribute__((aligned(1024))) char lds[RING];
 
     const int lane = threadIdx.x & 63;
@@ -654,80 +683,55 @@ linear_tile_kernel(const TileArgs a) {
     if constexpr (IN_PLACE) mfma_drain();
     wait_vmcnt<0>();                                   // no load may land in the epilogue's LDS
 
-    if (a.e.vec) {
-        const int mw = m0 + wm * WTM, nw = n0 + wn * WTN;
-        Epilogue e = a.e;
-        if (e.part) {                                  // a K slice: raw sums
-            e.y = e.part + blockIdx.y * e.slice_stride;
-            e.ldy = e.ld_part;
-            e.y_f32 = 1;
-        }
-        if constexpr (AT || BT) {
-            finish_direct<T, YOLO_AMD_ACT_NONE, IN_PLACE>(e, acc, mw, nw, a.M, a.N, lane);
-        } else {
-            switch (e.act) {
-                case YOLO_AMD_ACT_LEAKY: finish_direct<T, YOLO_AMD_ACT_LEAKY, IN_PLACE>(e, acc, mw, nw, a.M, a.N, lane); break;
-                case YOLO_AMD_ACT_RELU: finish_direct<T, YOLO_AMD_ACT_RELU, IN_PLACE>(e, acc, mw, nw, a.M, a.N, lane); break;
-                case YOLO_AMD_ACT_GELU: finish_direct<T, YOLO_AMD_ACT_GELU, IN_PLACE>(e, acc, mw, nw, a.M, a.N, lane); break;
-                case YOLO_AMD_ACT_GELU_TANH: finish_direct<T, YOLO_AMD_ACT_GELU_TANH, IN_PLACE>(e, acc, mw, nw, a.M, a.N, lane); break;
-                case YOLO_AMD_ACT_SILU: finish_direct<T, YOLO_AMD_ACT_SILU, IN_PLACE>(e, acc, mw, nw, a.M, a.N, lane); break;
-                default: finish_direct<T, YOLO_AMD_ACT_NONE, IN_PLACE>(e, acc, mw, nw, a.M, a.N, lane); break;
-            }
-        }
-        return;
+    const int mw = m0 + wm * WTM, nw = n0 + wn * WTN;
+    Epilogue e = a.e;
+    int nv = a.N & ~7;
+    if (e.part) {                                      // a K slice: raw sums, rows of whole eights
+        e.y = e.part + blockIdx.y * e.slice_stride;
+        e.ldy = e.ld_part;
+        e.y_f32 = 1;
+        nv = (a.N + 7) & ~7;
     }
-    // Rows of y that do not start on 16-byte boundaries, or N no multiple of 8: the accumulators go through LDS in
-    // fp32, 32 rows of every wave row at a time, and are finished by element, a wave along a row.
-    float* out = reinterpret_cast<float*>(lds);
-#pragma unroll
-    for (int c = 0; c < WTM / 32; ++c) {
-        __syncthreads();
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-#pragma unroll
-            for (int j = 0; j < TN; ++j) {
-                float v[4];
-                acc_read<IN_PLACE>(acc[c * 2 + i][j], v);
-                *reinterpret_cast<f32x4*>(out + (wm * 32 + i * 16 + (lane & 15)) * CLD + wn * WTN + j * 16 + (lane >> 4) * 4) =
-                    f32x4{v[0], v[1], v[2], v[3]};
-            }
-        __syncthreads();
-#pragma unroll 4
-        for (int it = threadIdx.x; it < CROWS * BN; it += NT) {
-            const int lr = it / BN, n = it % BN;
-            const long long m = m0 + (lr >> 5) * WTM + c * 32 + (lr & 31);
-            if (m < a.M && n0 + n < a.N) finish1<T>(a.e, m, n0 + n, out[lr * CLD + n]);
+    float* tail = nullptr;
+    if (nv < a.N && n0 + BN > nv) {
+        __syncthreads();                               // every wave is done with the ring
+        tail = reinterpret_cast<float*>(lds) + w * (2 * WTM * 8);
+    }
+#define YA_FINISH(ACT) finish_direct<T, ACT, IN_PLACE>(e, acc, mw, nw, a.M, a.N, nv, lane, tail)
+    if constexpr (AT || BT) {
+        YA_FINISH(YOLO_AMD_ACT_NONE);
+    } else {
+        switch (e.act) {
+            case YOLO_AMD_ACT_LEAKY: YA_FINISH(YOLO_AMD_ACT_LEAKY); break;
+            case YOLO_AMD_ACT_RELU: YA_FINISH(YOLO_AMD_ACT_RELU); break;
+            case YOLO_AMD_ACT_GELU: YA_FINISH(YOLO_AMD_ACT_GELU); break;
+            case YOLO_AMD_ACT_GELU_TANH: YA_FINISH(YOLO_AMD_ACT_GELU_TANH); break;
+            case YOLO_AMD_ACT_SILU: YA_FINISH(YOLO_AMD_ACT_SILU); break;
+            default: YA_FINISH(YOLO_AMD_ACT_NONE); break;
         }
     }
+#undef YA_FINISH
 }
 
-// Adds the K slices in ascending order and finishes: a thread has eight columns, or, where rows of y are not whole and
-// aligned eights, one, so that a wave still runs along a row.
-template <typename T, int V>
+// Adds the K slices in ascending order and finishes, eight columns per thread.
+template <typename T>
 __global__ void __launch_bounds__(256)
 linear_finish_kernel(const Epilogue e, const float* part, int slices, int M, int N) {
-    const int n = (blockIdx.x * 64 + (threadIdx.x & 63)) * V;
+    const int n = (blockIdx.x * 64 + (threadIdx.x & 63)) * 8;
     const int step = gridDim.y * 4;
     if (n >= N) return;
     for (int m = blockIdx.y * 4 + (threadIdx.x >> 6); m < M; m += step) {
         const float* p = part + (long long)m * e.ld_part + n;
-        if constexpr (V == 8) {
-            float v[8];
-            load8<T>(p, 0, 1, v);
+        float v[8];
+        load8<T>(p, 0, 1, v);
 #pragma unroll 4
-            for (int s = 1; s < slices; ++s) {
-                float u[8];
-                load8<T>(p, s * e.slice_stride, 1, u);
+        for (int s = 1; s < slices; ++s) {
+            float u[8];
+            load8<T>(p, s * e.slice_stride, 1, u);
 #pragma unroll
-                for (int k = 0; k < 8; ++k) v[k] += u[k];
-            }
-            finish8<T>(e, m, n, N, v);
-        } else {
-            float v = *p;
-#pragma unroll 4
-            for (int s = 1; s < slices; ++s) v += p[s * e.slice_stride];
-            finish1<T>(e, m, n, v);
+            for (int k = 0; k < 8; ++k) v[k] += u[k];
         }
+        finish8<T>(e, m, n, N, v);
     }
 }
 
@@ -735,7 +739,8 @@ linear_finish_kernel(const Epilogue e, const float* part, int slices, int M, int
 // M <= 16 * MT rows of x: the product is a read of W.  A workgroup owns 16 * NT rows of W (columns of Y) and
 // its eight waves take 64 reduction indices each in turn, straight from memory into matrix-instruction fragments;
 // the eight partial sums meet in LDS in a fixed order.  No second launch, no atomics.
-template <typename T, int MT, int NT>
+// U steps' loads are issued before the first product: what bounds this kernel is how much of W is on its way.
+template <typename T, int MT, int NT, int U>
 __global__ void __launch_bounds__(512)
 linear_rows_kernel(const TileArgs a) {
     __shared__ __attribute__((aligned(16))) f32x4 red[8][MT][NT][64];
@@ -746,44 +751,46 @@ linear_rows_kernel(const TileArgs a) {
     const T* xp[MT];
     const T* wp[NT];
 #pragma unroll
-    for (int i = 0; i < MT; ++i) xp[i] = (const T*)a.A + (long long)min(i * 16 + (lane & 15), a.M - 1) * a.lda + kl;
+    for (int i = 0; i < MT; ++i) xp[i] = (const T*)a.A + (long long)min(i * 16 + (lane & 15), a.M - 1) * a.lda;
 #pragma unroll
-    for (int j = 0; j < NT; ++j) wp[j] = (const T*)a.B + (long long)min(n0 + j * 16 + (lane & 15), a.N - 1) * a.ldb + kl;
+    for (int j = 0; j < NT; ++j) wp[j] = (const T*)a.B + (long long)min(n0 + j * 16 + (lane & 15), a.N - 1) * a.ldb;
     f32x4 acc[MT][NT];
 #pragma unroll
     for (int i = 0; i < MT; ++i)
 #pragma unroll
         for (int j = 0; j < NT; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-    int k = w * 64;
-#pragma unroll 4
-    for (; k + 64 <= a.K; k += 512) {
+    for (int k = w * 64; k < a.K; k += 512 * U) {
+        v8<T> xv[U][2][MT], wv[U][2][NT];
+        bool in[U][2];
 #pragma unroll
-        for (int s = 0; s < 2; ++s) {
-            v8<T> xv[MT], wv[NT];
+        for (int u = 0; u < U; ++u)
 #pragma unroll
-            for (int j = 0; j < NT; ++j) wv[j] = *reinterpret_cast<const v8<T>*>(wp[j] + k + s * 32);
+            for (int s = 0; s < 2; ++s) {
+                // past K (whole chunks: K is a multiple of 8): the row's start, taken as zeros below
+                const int at = k + u * 512 + s * 32 + kl;
+                in[u][s] = at < a.K;
+                const int from = in[u][s] ? at : 0;
 #pragma unroll
-            for (int i = 0; i < MT; ++i) xv[i] = *reinterpret_cast<const v8<T>*>(xp[i] + k + s * 32);
+                for (int j = 0; j < NT; ++j) wv[u][s][j] = *reinterpret_cast<const v8<T>*>(wp[j] + from);
 #pragma unroll
-            for (int i = 0; i < MT; ++i)
+                for (int i = 0; i < MT; ++i) xv[u][s][i] = *reinterpret_cast<const v8<T>*>(xp[i] + from);
+            }
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                for (int j = 0; j < NT; ++j) acc[i][j] = mfma(wv[j], xv[i], acc[i][j]);
-        }
-    }
-    if (k < a.K) {                                  // one wave has the last, partial step
+        for (int u = 0; u < U; ++u)
 #pragma unroll
-        for (int s = 0; s < 2; ++s) {
-            const bool in = k + s * 32 + kl < a.K;  // whole chunks: K is a multiple of 8
-            v8<T> xv[MT], wv[NT];
+            for (int s = 0; s < 2; ++s) {
+                if (!in[u][s]) {
 #pragma unroll
-            for (int j = 0; j < NT; ++j) wv[j] = in ? *reinterpret_cast<const v8<T>*>(wp[j] + k + s * 32) : v8<T>{};
+                    for (int j = 0; j < NT; ++j) wv[u][s][j] = v8<T>{};
 #pragma unroll
-            for (int i = 0; i < MT; ++i) xv[i] = in ? *reinterpret_cast<const v8<T>*>(xp[i] + k + s * 32) : v8<T>{};
+                    for (int i = 0; i < MT; ++i) xv[u][s][i] = v8<T>{};
+                }
 #pragma unroll
-            for (int i = 0; i < MT; ++i)
+                for (int i = 0; i < MT; ++i)
 #pragma unroll
-                for (int j = 0; j < NT; ++j) acc[i][j] = mfma(wv[j], xv[i], acc[i][j]);
-        }
+                    for (int j = 0; j < NT; ++j) acc[i][j] = mfma(wv[u][s][j], xv[u][s][i], acc[i][j]);
+            }
     }
 #pragma unroll
     for (int i = 0; i < MT; ++i)
@@ -837,56 +844,68 @@ linear_pack_kernel(const PackArgs a) {
 struct DpreArgs {
     const void *dy, *pre;
     long long lddy, ldpre;
-    int dy_f32, act, vec;
+    int dy_f32, act;
     void* dp;               // [M][ldp], zero filled past N; null: only the column sums are wanted
     long long ldp;
     float* part;            // [row block][N] column sums, or null
     int M, N, rows;         // rows per block
 };
 
-// Thread = eight columns of a run of rows; column sums in fp32 over that run, added over the runs by
-// linear_dbias_kernel in ascending order.
-template <typename T>
+// Thread = V columns of a run of rows: eight where rows are whole eights, else one, so that a wave
+// runs along a row.  Column sums in fp32 over that run, added over the runs by linear_dbias_kernel.
+template <typename T, int V>
 __global__ void __launch_bounds__(256)
 linear_dpre_kernel(const DpreArgs a) {
-    const int lane_c = threadIdx.x & 31, lane_r = threadIdx.x >> 5;      // 32 chunks x 8 rows
-    const int n = (blockIdx.x * 32 + lane_c) * 8;
-    __shared__ float red[8][32 * 8 + 1];
+    constexpr int CL = V == 8 ? 32 : 64, RL = 256 / CL, U = 4;           // column lanes x rows, rows in flight
+    const int lane_c = threadIdx.x % CL, lane_r = threadIdx.x / CL;
+    const int n = (blockIdx.x * CL + lane_c) * V;
+    __shared__ float red[RL][CL * V + 1];
     const long long r0 = (long long)blockIdx.y * a.rows;
     const long long r1 = min((long long)a.M, r0 + a.rows);
-    float sum[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    if (n < a.N) {
-#pragma unroll 2
-        for (long long m = r0 + lane_r; m < r1; m += 8) {
-            float d[8], p[8];
-            if (a.vec) {
-                load8<T>(a.dy, m * a.lddy + n, a.dy_f32, d);
-                if (a.pre) load8<T>(a.pre, m * a.ldpre + n, 0, p);
-            } else {
+    float sum[V];
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    d[i] = n + i < a.N ? load1<T>(a.dy, m * a.lddy + n + i, a.dy_f32) : 0.f;
-                    p[i] = a.pre && n + i < a.N ? load1<T>(a.pre, m * a.ldpre + n + i, 0) : 0.f;
-                }
-            }
-            if (a.pre) {
+    for (int i = 0; i < V; ++i) sum[i] = 0.f;
+    auto value = [&](const float (&d)[V], const float (&p)[V], long long m) {
+        float o[V];
 #pragma unroll
-                for (int i = 0; i < 8; ++i) d[i] *= act_slope(p[i], a.act);
-            }
-            if (a.dp) store8<T>(a.dp, m * a.ldp + n, 0, d);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) sum[i] += d[i];
+        for (int i = 0; i < V; ++i) {
+            o[i] = a.pre ? d[i] * act_slope(p[i], a.act) : d[i];
+            sum[i] += o[i];
         }
+        if (a.dp) {
+            if constexpr (V == 8) store8<T>(a.dp, m * a.ldp + n, 0, o);
+            else store1<T>(a.dp, m * a.ldp + n, 0, o[0]);
+        }
+    };
+    auto fetch = [&](const void* p, long long at, int f32, float (&v)[V]) {
+        if constexpr (V == 8) load8<T>(p, at, f32, v);
+        else v[0] = load1<T>(p, at, f32);
+    };
+    if (n < a.N) {
+        for (long long m = r0 + lane_r; m < r1; m += RL * U) {
+            float d[U][V], p[U][V];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {              // rows past the run: its last one again, not used
+                const long long mu = min(m + u * RL, r1 - 1);
+                fetch(a.dy, mu * a.lddy + n, a.dy_f32, d[u]);
+                if (a.pre) fetch(a.pre, mu * a.ldpre + n, 0, p[u]);
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+                if (m + u * RL < r1) value(d[u], p[u], m + u * RL);
+        }
+    } else if (V == 1 && a.dp && n < a.ldp) {          // zeros up to the padded row's end
+        for (long long m = r0 + lane_r; m < r1; m += RL) store1<T>(a.dp, m * a.ldp + n, 0, 0.f);
     }
     if (!a.part) return;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) red[lane_r][lane_c * 8 + i] = sum[i];
+    for (int i = 0; i < V; ++i) red[lane_r][lane_c * V + i] = sum[i];
     __syncthreads();
-    const int c = blockIdx.x * 256 + threadIdx.x;
-    if (c < a.N) {
+    const int c = blockIdx.x * (CL * V) + threadIdx.x;
+    if (threadIdx.x < CL * V && c < a.N) {
         float s = 0.f;
 #pragma unroll
-        for (int r = 0; r < 8; ++r) s += red[r][threadIdx.x];
+        for (int r = 0; r < RL; ++r) s += red[r][threadIdx.x];
         a.part[(long long)blockIdx.y * a.N + c] = s;
     }
 }
@@ -1025,12 +1044,18 @@ template <typename T, bool AT, bool BT>
 static int launch_product(const TilePlan& p, TileArgs a, void* partial, hipStream_t s) {
     if (p.kernel == YOLO_AMD_LINEAR_ROWS) {
         if constexpr (!AT && !BT) {
-            const int nt = p.bn / 16;
             const dim3 grid((a.N + p.bn - 1) / p.bn);
-            if (p.bm == 16 && nt == 1) hipLaunchKernelGGL((linear_rows_kernel<T, 1, 1>), grid, dim3(512), 0, s, a);
-            else if (p.bm == 16) hipLaunchKernelGGL((linear_rows_kernel<T, 1, 2>), grid, dim3(512), 0, s, a);
-            else if (nt == 1) hipLaunchKernelGGL((linear_rows_kernel<T, 2, 1>), grid, dim3(512), 0, s, a);
-            else hipLaunchKernelGGL((linear_rows_kernel<T, 2, 2>), grid, dim3(512), 0, s, a);
+            const bool deep = a.K > 1024;              // four steps of 512 in flight
+#define YA_ROWS(MT, NT)                                                                                              \
+    do {                                                                                                             \
+        if (deep) hipLaunchKernelGGL((linear_rows_kernel<T, MT, NT, 4>), grid, dim3(512), 0, s, a);                  \
+        else hipLaunchKernelGGL((linear_rows_kernel<T, MT, NT, 2>), grid, dim3(512), 0, s, a);                       \
+    } while (0)
+            if (p.bm == 16 && p.bn == 16) YA_ROWS(1, 1);
+            else if (p.bm == 16) YA_ROWS(1, 2);
+            else if (p.bn == 16) YA_ROWS(2, 1);
+            else YA_ROWS(2, 2);
+#undef YA_ROWS
         }
         YA_CHECK_HIP(hipGetLastError());
         return YA_OK;
@@ -1041,7 +1066,6 @@ static int launch_product(const TilePlan& p, TileArgs a, void* partial, hipStrea
     const Epilogue e = a.e;
     if (p.slices > 1) {
         a.e = Epilogue{};
-        a.e.vec = 1;                                   // rows of whole 8 columns, the last ones past N
         a.e.part = (float*)partial;
         a.e.ld_part = (long long)align_up(a.N, 8);
         a.e.slice_stride = a.e.ld_part * a.M;
@@ -1055,17 +1079,11 @@ static int launch_product(const TilePlan& p, TileArgs a, void* partial, hipStrea
         Epilogue f = e;
         f.ld_part = a.e.ld_part;
         f.slice_stride = a.e.slice_stride;
-        const int cols = f.vec ? 512 : 64;
-        const dim3 fgrid((a.N + cols - 1) / cols, (unsigned)std::min<long long>((a.M + 3) / 4, 4096));
-        if (f.vec) hipLaunchKernelGGL((linear_finish_kernel<T, 8>), fgrid, dim3(256), 0, s, f, (const float*)partial, p.slices, a.M, a.N);
-        else hipLaunchKernelGGL((linear_finish_kernel<T, 1>), fgrid, dim3(256), 0, s, f, (const float*)partial, p.slices, a.M, a.N);
+        const dim3 fgrid((a.N + 511) / 512, (unsigned)std::min<long long>((a.M + 3) / 4, 4096));
+        hipLaunchKernelGGL((linear_finish_kernel<T>), fgrid, dim3(256), 0, s, f, (const float*)partial, p.slices, a.M, a.N);
     }
     YA_CHECK_HIP(hipGetLastError());
     return YA_OK;
-}
-
-static bool rows16(const void* p, long long ld, int esize) {
-    return p == nullptr || (((uintptr_t)p & 15) == 0 && (ld * esize) % 16 == 0);
 }
 
 constexpr long long kMaxLd = (1ll << 22) - 1, kMaxRows = (1ll << 31) - 1024;
@@ -1142,8 +1160,6 @@ static int forward(const yolo_amd_linear_desc* d, const ForwardPlan& f, hipStrea
     e.bias = d->bias; e.res = d->residual; e.y = d->y; e.pre = d->pre;
     e.ldr = d->ldr; e.ldy = d->ldy; e.ldp = d->n;
     e.bias_f32 = d->bias_f32; e.res_f32 = d->residual_f32; e.y_f32 = d->y_f32; e.act = d->activation;
-    e.vec = d->n % 8 == 0 && rows16(e.bias, 0, 2) && rows16(e.res, e.ldr, e.res_f32 ? 4 : 2) &&
-            rows16(e.y, e.ldy, e.y_f32 ? 4 : 2) && rows16(e.pre, e.ldp, 2);
     return launch_product<T, false, false>(f.tile, a, sc.take(f.part_bytes), s);
 }
 
@@ -1180,15 +1196,10 @@ static BackwardPlan plan_backward(const yolo_amd_linear_backward_desc* d) {
     const bool products = (d->dx || d->dweight) && d->k > 0 && !empty;
     b.own_dp = products && (d->activation != YOLO_AMD_ACT_NONE || d->dy_f32 || !packed_ok(dy));
     if (b.own_dp) b.dp_bytes = align_up((size_t)d->m * align_up(d->n, 8) * 2, 256);
-    if (d->dbias && !empty) {
-        // enough blocks of rows to fill the chip, at least 32 rows each
-        const long long cols = (d->n + 255) / 256;
-        long long want = std::max<long long>(1, 2048 / cols);
-        b.rows = (int)std::max<long long>(32, (d->m + want - 1) / want);
-        b.db_bytes = align_up((size_t)((d->m + b.rows - 1) / b.rows) * d->n * 4, 256);
-    } else {
-        b.rows = 64;
-    }
+    // enough blocks of rows to fill the chip, at least 32 rows each
+    const long long cols = std::max<long long>(1, d->n / (d->n % 8 ? 64 : 256)), want = std::max<long long>(1, 2048 / cols);
+    b.rows = (int)std::max<long long>(32, (d->m + want - 1) / want);
+    if (d->dbias && !empty) b.db_bytes = align_up((size_t)((d->m + b.rows - 1) / b.rows) * d->n * 4, 256);
     b.blocks = (int)((d->m + b.rows - 1) / b.rows);
     if (!products) return b;
     if (d->dx) {
@@ -1233,12 +1244,12 @@ static int backward(const yolo_amd_linear_backward_desc* d, const BackwardPlan& 
         g.act = d->activation;
         g.pre = g.act == YOLO_AMD_ACT_NONE ? nullptr : d->pre;
         g.ldpre = N;
-        g.vec = N % 8 == 0 && rows16(g.dy, M > 1 ? g.lddy : 0, g.dy_f32 ? 4 : 2) && rows16(g.pre, N, 2);
         g.dp = b.own_dp ? dp : nullptr;
         g.ldp = (long long)align_up(N, 8);
         g.part = d->dbias ? db : nullptr;
         g.M = M; g.N = N; g.rows = b.rows;
-        hipLaunchKernelGGL((linear_dpre_kernel<T>), dim3((N + 255) / 256, b.blocks), dim3(256), 0, s, g);
+        if (N % 8 == 0) hipLaunchKernelGGL((linear_dpre_kernel<T, 8>), dim3((N + 255) / 256, b.blocks), dim3(256), 0, s, g);
+        else hipLaunchKernelGGL((linear_dpre_kernel<T, 1>), dim3((N + 63) / 64, b.blocks), dim3(256), 0, s, g);
         if (d->dbias)
             hipLaunchKernelGGL((linear_dbias_kernel<T>), dim3((N + 63) / 64), dim3(1024), 0, s, db, b.blocks, N, d->dbias, d->dbias_f32);
     }
@@ -1247,7 +1258,6 @@ static int backward(const yolo_amd_linear_backward_desc* d, const BackwardPlan& 
     if (K > 0) {
         TileArgs a{};
         a.e.act = YOLO_AMD_ACT_NONE;
-        a.e.vec = K % 8 == 0;
         a.e.ldy = K;
         Matrix in[2] = {b.x, b.w};
         launch_pack<T>(in, {b.x_bytes, b.w_bytes}, sc, s);
@@ -1258,7 +1268,6 @@ static int backward(const yolo_amd_linear_backward_desc* d, const BackwardPlan& 
             a.B = w.p; a.ldb = w.ld;
             a.M = M; a.N = K; a.K = N;
             a.e.y = d->dx;
-            a.e.vec = K % 8 == 0 && ((uintptr_t)d->dx & 15) == 0;
             YA_TRY((launch_product<T, false, true>(b.dx, a, part, s)));
         }
         if (d->dweight) {
@@ -1266,7 +1275,6 @@ static int backward(const yolo_amd_linear_backward_desc* d, const BackwardPlan& 
             a.B = x.p; a.ldb = x.ld;
             a.M = N; a.N = K; a.K = M;
             a.e.y = d->dweight;
-            a.e.vec = K % 8 == 0 && ((uintptr_t)d->dweight & 15) == 0;
             YA_TRY((launch_product<T, true, true>(b.dw, a, part, s)));
         }
     }
