@@ -138,25 +138,41 @@ __device__ __forceinline__ float act_value(float p, int act) {
     }
 }
 
-__device__ __forceinline__ float act_slope(float p, int act) {
-    switch (act) {
-        case YOLO_AMD_ACT_LEAKY: return p > 0.f ? 1.f : 0.1f;
-        case YOLO_AMD_ACT_RELU: return p > 0.f ? 1.f : 0.f;
-        case YOLO_AMD_ACT_GELU: {
-            float e;
-            const float q = 0.5f * erfc_scaled(p, e);
-            return fmaf(p * 0.3989422804014327f, e, p < 0.f ? q : 1.f - q);
-        }
-        case YOLO_AMD_ACT_GELU_TANH: {
-            const float z = sigmoid_fast(2.f * kGeluC * (p + kGeluA * p * p * p));
-            return z + p * z * (1.f - z) * 2.f * kGeluC * (1.f + 3.f * kGeluA * p * p);
-        }
-        case YOLO_AMD_ACT_SILU: {
-            const float z = sigmoid_fast(p);
-            return z * (1.f + p * (1.f - z));
-        }
-        default: return 1.f;
+template <int ACT>
+__device__ __forceinline__ float act_slope(float p) {
+    if constexpr (ACT == YOLO_AMD_ACT_LEAKY) return p > 0.f ? 1.f : 0.1f;
+    if constexpr (ACT == YOLO_AMD_ACT_RELU) return p > 0.f ? 1.f : 0.f;
+    if constexpr (ACT == YOLO_AMD_ACT_GELU) {
+        float e;
+        const float q = 0.5f * erfc_scaled(p, e);
+        return fmaf(p * 0.3989422804014327f, e, p < 0.f ? q : 1.f - q);
     }
+    if constexpr (ACT == YOLO_AMD_ACT_GELU_TANH) {
+        const float z = sigmoid_fast(2.f * kGeluC * (p + kGeluA * p * p * p));
+        return z + p * z * (1.f - z) * 2.f * kGeluC * (1.f + 3.f * kGeluA * p * p);
+    }
+    if constexpr (ACT == YOLO_AMD_ACT_SILU) {
+        const float z = sigmoid_fast(p);
+        return z * (1.f + p * (1.f - z));
+    }
+    return 1.f;
+}
+// d *= act'(p)
+template <int V>
+__device__ __forceinline__ void times_slopes(float (&d)[V], const float (&p)[V], int act) {
+#define YA_SLOPES(ACT)                                                   \
+    case ACT:                                                            \
+        _Pragma("unroll") for (int i = 0; i < V; ++i) d[i] *= act_slope<ACT>(p[i]); \
+        break;
+    switch (act) {
+        YA_SLOPES(YOLO_AMD_ACT_LEAKY)
+        YA_SLOPES(YOLO_AMD_ACT_RELU)
+        YA_SLOPES(YOLO_AMD_ACT_GELU)
+        YA_SLOPES(YOLO_AMD_ACT_GELU_TANH)
+        YA_SLOPES(YOLO_AMD_ACT_SILU)
+        default: break;
+    }
+#undef YA_SLOPES
 }
 
 // ---------------------------------------------------------------- epilogue
@@ -851,58 +867,47 @@ struct DpreArgs {
     int M, N, rows;         // rows per block
 };
 
-// Thread = V columns of a run of rows: eight where rows are whole eights, else one, so that a wave
-// runs along a row.  Column sums in fp32 over that run, added over the runs by linear_dbias_kernel.
-template <typename T, int V>
+// Thread = eight columns of a run of rows (the last ones by element); column sums in fp32 over that run, added over the
+// runs by linear_dbias_kernel.  One row at a time: more rows in flight cost registers that hide more of memory's
+// latency as further waves (4096 x 4096 with GELU: 1 row 20.8 us, 2 rows 23.9, 4 rows 28.2; 100 MB).
+template <typename T>
 __global__ void __launch_bounds__(256)
 linear_dpre_kernel(const DpreArgs a) {
-    constexpr int CL = V == 8 ? 32 : 64, RL = 256 / CL, U = 4;           // column lanes x rows, rows in flight
+    constexpr int CL = 32, RL = 8;                     // column lanes x rows
     const int lane_c = threadIdx.x % CL, lane_r = threadIdx.x / CL;
-    const int n = (blockIdx.x * CL + lane_c) * V;
-    __shared__ float red[RL][CL * V + 1];
+    const int n = (blockIdx.x * CL + lane_c) * 8;
+    __shared__ float red[RL][CL * 8 + 1];
     const long long r0 = (long long)blockIdx.y * a.rows;
     const long long r1 = min((long long)a.M, r0 + a.rows);
-    float sum[V];
+    const bool whole = n + 8 <= a.N;
+    float sum[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    auto fetch = [&](const void* p, long long at, int f32, float (&v)[8]) {
+        if (whole) {
+            load8<T>(p, at, f32, v);
+        } else {
 #pragma unroll
-    for (int i = 0; i < V; ++i) sum[i] = 0.f;
-    auto value = [&](const float (&d)[V], const float (&p)[V], long long m) {
-        float o[V];
-#pragma unroll
-        for (int i = 0; i < V; ++i) {
-            o[i] = a.pre ? d[i] * act_slope(p[i], a.act) : d[i];
-            sum[i] += o[i];
+            for (int i = 0; i < 8; ++i) v[i] = n + i < a.N ? load1<T>(p, at + i, f32) : 0.f;
         }
-        if (a.dp) {
-            if constexpr (V == 8) store8<T>(a.dp, m * a.ldp + n, 0, o);
-            else store1<T>(a.dp, m * a.ldp + n, 0, o[0]);
-        }
-    };
-    auto fetch = [&](const void* p, long long at, int f32, float (&v)[V]) {
-        if constexpr (V == 8) load8<T>(p, at, f32, v);
-        else v[0] = load1<T>(p, at, f32);
     };
     if (n < a.N) {
-        for (long long m = r0 + lane_r; m < r1; m += RL * U) {
-            float d[U][V], p[U][V];
-#pragma unroll
-            for (int u = 0; u < U; ++u) {              // rows past the run: its last one again, not used
-                const long long mu = min(m + u * RL, r1 - 1);
-                fetch(a.dy, mu * a.lddy + n, a.dy_f32, d[u]);
-                if (a.pre) fetch(a.pre, mu * a.ldpre + n, 0, p[u]);
+        for (long long m = r0 + lane_r; m < r1; m += RL) {
+            float d[8], p[8];
+            fetch(a.dy, m * a.lddy + n, a.dy_f32, d);
+            if (a.pre) {
+                fetch(a.pre, m * a.ldpre + n, 0, p);
+                times_slopes<8>(d, p, a.act);
             }
 #pragma unroll
-            for (int u = 0; u < U; ++u)
-                if (m + u * RL < r1) value(d[u], p[u], m + u * RL);
+            for (int i = 0; i < 8; ++i) sum[i] += d[i];
+            if (a.dp) store8<T>(a.dp, m * a.ldp + n, 0, d);          // padded rows: zeros behind the last column
         }
-    } else if (V == 1 && a.dp && n < a.ldp) {          // zeros up to the padded row's end
-        for (long long m = r0 + lane_r; m < r1; m += RL) store1<T>(a.dp, m * a.ldp + n, 0, 0.f);
     }
     if (!a.part) return;
 #pragma unroll
-    for (int i = 0; i < V; ++i) red[lane_r][lane_c * V + i] = sum[i];
+    for (int i = 0; i < 8; ++i) red[lane_r][lane_c * 8 + i] = sum[i];
     __syncthreads();
-    const int c = blockIdx.x * (CL * V) + threadIdx.x;
-    if (threadIdx.x < CL * V && c < a.N) {
+    const int c = blockIdx.x * (CL * 8) + threadIdx.x;
+    if (c < a.N) {
         float s = 0.f;
 #pragma unroll
         for (int r = 0; r < RL; ++r) s += red[r][threadIdx.x];
@@ -969,7 +974,7 @@ static const TileConfig kTileConfigs[] = {
     {64, 4, 3.2, 0.436, 3.1, 0.274},
 };
 
-static TilePlan plan_product(long long M, int N, long long K, bool kc_operands) {
+static TilePlan plan_product(long long M, int N, long long K, bool kc_operands, int act) {
     TilePlan p{};
     const long long steps = std::max<long long>(1, (K + kBK - 1) / kBK);
     if (kc_operands && M <= 32) {
@@ -980,6 +985,9 @@ static TilePlan plan_product(long long M, int N, long long K, bool kc_operands) 
         p.ksteps = (int)steps;
         return p;
     }
+    // An activation's instructions lengthen an epilogue that nothing overlaps (256: 12 us a round for erf, 4.5 for the two
+    // with an exponential and a reciprocal) more than one that another workgroup's products run beside (128: 2.3 and 1).
+    const double slow = act == YOLO_AMD_ACT_GELU ? 1.0 : act == YOLO_AMD_ACT_GELU_TANH || act == YOLO_AMD_ACT_SILU ? 0.4 : 0.0;
     double best = 0;
     for (const TileConfig& c : kTileConfigs) {
         const long long tiles = ((M + c.b - 1) / c.b) * ((N + c.b - 1) / c.b);
@@ -989,6 +997,7 @@ static TilePlan plan_product(long long M, int N, long long K, bool kc_operands) 
             if ((steps + per - 1) / per != s) continue;
             if (s > 1 && wgs > slots) break;           // a split only fills a round that is not full
             double t = (double)(wgs / slots) * (c.start + per * c.step);
+            if (s == 1) t += (double)((wgs + slots - 1) / slots) * slow * (c.b == 256 ? 12.0 : c.b == 128 ? 2.5 : 0.7);
             if (rest > 0) t += rest <= 256 ? c.start_1 + per * c.step_1 : c.start + per * c.step;
             if (s > 1) t += 3.4 + 0.08 * s + (double)s * M * N * 2e-6;     // one more launch; partial sums out and in at 4 TB/s
             if (p.kernel == 0 || t < best) {
@@ -1129,7 +1138,7 @@ static ForwardPlan plan_forward(const yolo_amd_linear_desc* d) {
     f.x = Matrix{d->x, d->ldx, d->m, (int)d->k};
     f.w = Matrix{d->weight, d->ldw, d->n, (int)d->k};
     if (d->m == 0 || d->n == 0) return f;
-    f.tile = plan_product(d->m, (int)d->n, d->k, true);
+    f.tile = plan_product(d->m, (int)d->n, d->k, true, d->activation);
     f.x_bytes = packed_bytes(f.x);
     f.w_bytes = packed_bytes(f.w);
     f.part_bytes = partial_bytes(f.tile, d->m, (int)d->n);
@@ -1196,19 +1205,19 @@ static BackwardPlan plan_backward(const yolo_amd_linear_backward_desc* d) {
     const bool products = (d->dx || d->dweight) && d->k > 0 && !empty;
     b.own_dp = products && (d->activation != YOLO_AMD_ACT_NONE || d->dy_f32 || !packed_ok(dy));
     if (b.own_dp) b.dp_bytes = align_up((size_t)d->m * align_up(d->n, 8) * 2, 256);
-    // enough blocks of rows to fill the chip, at least 32 rows each
-    const long long cols = std::max<long long>(1, d->n / (d->n % 8 ? 64 : 256)), want = std::max<long long>(1, 2048 / cols);
-    b.rows = (int)std::max<long long>(32, (d->m + want - 1) / want);
+    // enough blocks of rows to fill the chip, at least 16 rows each
+    const long long cols = std::max<long long>(1, (d->n + 255) / 256), want = std::max<long long>(1, 2048 / cols);
+    b.rows = (int)std::max<long long>(16, (d->m + want - 1) / want);
     if (d->dbias && !empty) b.db_bytes = align_up((size_t)((d->m + b.rows - 1) / b.rows) * d->n * 4, 256);
     b.blocks = (int)((d->m + b.rows - 1) / b.rows);
     if (!products) return b;
     if (d->dx) {
-        b.dx = plan_product(d->m, (int)d->k, d->n, false);
+        b.dx = plan_product(d->m, (int)d->k, d->n, false, YOLO_AMD_ACT_NONE);
         b.w_bytes = packed_bytes(b.w);
         b.part_bytes = partial_bytes(b.dx, d->m, (int)d->k);
     }
     if (d->dweight) {
-        b.dw = plan_product(d->n, (int)d->k, d->m, false);
+        b.dw = plan_product(d->n, (int)d->k, d->m, false, YOLO_AMD_ACT_NONE);
         b.x_bytes = packed_bytes(b.x);
         b.part_bytes = std::max(b.part_bytes, partial_bytes(b.dw, d->n, (int)d->k));
     }
@@ -1248,8 +1257,7 @@ static int backward(const yolo_amd_linear_backward_desc* d, const BackwardPlan& 
         g.ldp = (long long)align_up(N, 8);
         g.part = d->dbias ? db : nullptr;
         g.M = M; g.N = N; g.rows = b.rows;
-        if (N % 8 == 0) hipLaunchKernelGGL((linear_dpre_kernel<T, 8>), dim3((N + 255) / 256, b.blocks), dim3(256), 0, s, g);
-        else hipLaunchKernelGGL((linear_dpre_kernel<T, 1>), dim3((N + 63) / 64, b.blocks), dim3(256), 0, s, g);
+        hipLaunchKernelGGL((linear_dpre_kernel<T>), dim3((N + 255) / 256, b.blocks), dim3(256), 0, s, g);
         if (d->dbias)
             hipLaunchKernelGGL((linear_dbias_kernel<T>), dim3((N + 63) / 64), dim3(1024), 0, s, db, b.blocks, N, d->dbias, d->dbias_f32);
     }
