@@ -22,7 +22,7 @@
 
 namespace yolo_amd {
 
-typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 struct NormArgs {
     const void *x, *res, *gate, *aw, *ab, *bw, *bb;
@@ -32,6 +32,7 @@ struct NormArgs {
     int D;
     int gate_f32, after_f32, before_f32;
     long long rows_per_gate;       // rows that share a row of the gate
+    int gate_shared;               // all of them do
     int after, before, layer;
     float eps, scale, inv_d;
     // backward
@@ -46,84 +47,126 @@ struct NormArgs {
     float* gate_part;              // [sequence][chunk][D]: gate sums where a run of rows shares a gate row
 };
 
-// 8 consecutive values, 16-byte aligned
-__device__ __forceinline__ void get8(const float* p, float* v) {
-    const f32x4 a = *reinterpret_cast<const f32x4*>(p), b = *reinterpret_cast<const f32x4*>(p + 4);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) { v[i] = a[i]; v[4 + i] = b[i]; }
-}
-template <typename T>
-__device__ __forceinline__ void get8(const T* p, float* v) {
-    typedef T t8 __attribute__((ext_vector_type(8)));
-    const t8 a = *reinterpret_cast<const t8*>(p);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = (float)a[i];
-}
-__device__ __forceinline__ void put8(float* p, const float* v) {
-    f32x4 a, b;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) { a[i] = v[i]; b[i] = v[4 + i]; }
-    *reinterpret_cast<f32x4*>(p) = a;
-    *reinterpret_cast<f32x4*>(p + 4) = b;
-}
-template <typename T>
-__device__ __forceinline__ void put8(T* p, const float* v) {
-    typedef T t8 __attribute__((ext_vector_type(8)));
-    t8 a;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) a[i] = (T)v[i];
-    *reinterpret_cast<t8*>(p) = a;
-}
+// Eight consecutive values at the elements' own alignment (the machine takes 16-byte accesses anywhere).
+template <typename S>
+struct Eight {
+    typedef S vec __attribute__((ext_vector_type(8)));
+    typedef S vecu __attribute__((ext_vector_type(8), aligned(sizeof(S))));
+};
 
-// The columns thread t of a group owns: with VEC runs of 8 (D % 8 == 0, rows 16-byte aligned), else single
-// columns TPR apart, which keeps element-wise accesses coalesced.
-template <int TPR, int CH, bool VEC>
+// The columns thread t of a group owns: CH runs of eight, TPR * 8 apart.  D may be any number: the thread whose run
+// holds a row's last one to seven values (D % 8) reads the row's last eight and moves them down, and stores by element.
+// FULL: D is exactly TPR * CH * 8 and no column needs a check.
+template <int TPR, int CH, bool FULL>
 struct Cols {
     static constexpr int E = CH * 8;
-    __device__ static __forceinline__ int col(int t, int e) { return VEC ? ((e >> 3) * TPR + t) * 8 + (e & 7) : e * TPR + t; }
-    // columns past D read as 0 (from an address inside the row)
+    __device__ static __forceinline__ int col(int t, int e) { return ((e >> 3) * TPR + t) * 8 + (e & 7); }
+    __device__ static __forceinline__ bool in(int t, int e, int D) { return FULL || col(t, e) < D; }
+
+    // a row's values as they are in memory, so that a row can be on its way while another is worked on
     template <typename S>
-    __device__ static __forceinline__ void load(const S* row, int D, int t, float (&v)[E]) {
-        if constexpr (VEC) {
+    struct Raw {
+        typename Eight<S>::vec v[CH];
+        __device__ __forceinline__ void load(const S* row, int D, int t) {
+            if constexpr (FULL) {
 #pragma unroll
-            for (int c = 0; c < CH; ++c) {
-                const int at = (c * TPR + t) * 8;
-                get8(row + min(at, D - 8), v + c * 8);
-                if (at >= D) {
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) v[c * 8 + i] = 0.f;
+                for (int c = 0; c < CH; ++c) {
+                    const typename Eight<S>::vecu x = *reinterpret_cast<const typename Eight<S>::vecu*>(row + (c * TPR + t) * 8);
+                    v[c] = x;
                 }
-            }
-        } else {
+            } else if (D >= 8) {
 #pragma unroll
-            for (int e = 0; e < E; ++e) {
-                const int at = e * TPR + t;
-                const float x = (float)row[min(at, D - 1)];
-                v[e] = at < D ? x : 0.f;
+                for (int c = 0; c < CH; ++c) {
+                    const typename Eight<S>::vecu x = *reinterpret_cast<const typename Eight<S>::vecu*>(row + min((c * TPR + t) * 8, D - 8));
+                    v[c] = x;
+                }
+            } else {                                   // a row shorter than eight: by element, thread 0
+#pragma unroll
+                for (int i = 0; i < 8; ++i) v[0][i] = row[min(i, D - 1)];
             }
+        }
+        // columns past D as 0
+        __device__ __forceinline__ void get(int D, int t, float (&f)[E]) const {
+#pragma unroll
+            for (int e = 0; e < E; ++e) f[e] = (float)v[e >> 3][e & 7];
+            if constexpr (!FULL) finish(D, t, f);
+        }
+    };
+    __device__ static __forceinline__ void finish(int D, int t, float (&f)[E]) {
+#pragma unroll
+        for (int c = 0; c < CH; ++c) {
+            const int at = (c * TPR + t) * 8;
+            if ((D & 7) && D >= 8) {
+                const bool last = at < D && at + 8 > D;
+                const int s = 8 - (D & 7);             // places to move down (the same for all rows)
+#pragma unroll
+                for (int bit = 1; bit < 8; bit *= 2)
+                    if (s & bit) {
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) f[c * 8 + i] = last ? (i + bit < 8 ? f[c * 8 + i + bit] : 0.f) : f[c * 8 + i];
+                    }
+            }
+#pragma unroll
+            for (int i = 0; i < 8; ++i) f[c * 8 + i] = at + i < D ? f[c * 8 + i] : 0.f;
         }
     }
     template <typename S>
     __device__ static __forceinline__ void store(S* row, int D, int t, const float (&v)[E]) {
-        if constexpr (VEC) {
 #pragma unroll
-            for (int c = 0; c < CH; ++c) {
-                const int at = (c * TPR + t) * 8;
-                if (at < D) put8(row + at, v + c * 8);
-            }
-        } else {
+        for (int c = 0; c < CH; ++c) {
+            const int at = (c * TPR + t) * 8;
+            if (FULL || at + 8 <= D) {
+                typename Eight<S>::vecu x;
 #pragma unroll
-            for (int e = 0; e < E; ++e) {
-                const int at = e * TPR + t;
-                if (at < D) row[at] = (S)v[e];
+                for (int i = 0; i < 8; ++i) x[i] = (S)v[c * 8 + i];
+                *reinterpret_cast<typename Eight<S>::vecu*>(row + at) = x;
+            } else if (at < D) {
+#pragma unroll
+                for (int i = 0; i < 7; ++i)
+                    if (at + i < D) row[at + i] = (S)v[c * 8 + i];
             }
         }
     }
-    // a parameter vector, fp32 or T
+    // a parameter row, fp32 or T, in two steps: the same registers for either
+    template <typename T>
+    struct Param {
+        u32x4 w[CH][2];
+        __device__ __forceinline__ void load(const void* p, int f32, long long at, int D, int t) {
+            if (f32) {
+                Raw<float> r;
+                r.load((const float*)p + at, D, t);
+#pragma unroll
+                for (int c = 0; c < CH; ++c) {
+                    w[c][0] = __builtin_bit_cast(u32x4, __builtin_shufflevector(r.v[c], r.v[c], 0, 1, 2, 3));
+                    w[c][1] = __builtin_bit_cast(u32x4, __builtin_shufflevector(r.v[c], r.v[c], 4, 5, 6, 7));
+                }
+            } else if constexpr (sizeof(T) == 2) {
+                Raw<T> r;
+                r.load((const T*)p + at, D, t);
+#pragma unroll
+                for (int c = 0; c < CH; ++c) w[c][0] = __builtin_bit_cast(u32x4, r.v[c]);
+            }
+        }
+        __device__ __forceinline__ void get(int f32, int D, int t, float (&f)[E]) const {
+            if (f32) {
+#pragma unroll
+                for (int e = 0; e < E; ++e) f[e] = __uint_as_float(w[e >> 3][(e >> 2) & 1][e & 3]);
+            } else if constexpr (sizeof(T) == 2) {
+#pragma unroll
+                for (int c = 0; c < CH; ++c) {
+                    const typename Eight<T>::vec v = __builtin_bit_cast(typename Eight<T>::vec, w[c][0]);
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) f[c * 8 + i] = (float)v[i];
+                }
+            }
+            if constexpr (!FULL) finish(D, t, f);
+        }
+    };
     template <typename T>
     __device__ static __forceinline__ void param(const void* p, int f32, long long at, int D, int t, float (&v)[E]) {
-        if (f32) load((const float*)p + at, D, t, v);
-        else load((const T*)p + at, D, t, v);
+        Param<T> r;
+        r.load(p, f32, at, D, t);
+        r.get(f32, D, t, v);
     }
 };
 
@@ -184,6 +227,10 @@ struct GroupSum {
     }
 };
 
+__device__ __forceinline__ long long gate_row(const NormArgs& a, long long row) {
+    return a.gate_shared ? 0 : (long long)((uint32_t)row / (uint32_t)a.rows_per_gate);
+}
+
 // mean (0 for rms) and factor of a row; columns past D hold 0
 template <typename C, typename G>
 __device__ __forceinline__ void row_stats(const float (&v)[C::E], const NormArgs& a, int t, G& sum, float& mean, float& f) {
@@ -197,17 +244,17 @@ __device__ __forceinline__ void row_stats(const float (&v)[C::E], const NormArgs
     float q = 0.f;
 #pragma unroll
     for (int e = 0; e < C::E; ++e) {
-        const float d = C::col(t, e) < a.D ? v[e] - mean : 0.f;
+        const float d = C::in(t, e, a.D) ? v[e] - mean : 0.f;
         q = fmaf(d, d, q);
     }
     f = rsqrtf(sum.one(q) * a.inv_d + a.eps);
 }
 
-template <typename T, typename R, int TPR, int CH, bool VEC>
+template <typename T, typename R, int TPR, int CH, bool FULL>
 __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR)
 block_norm_forward_kernel(const NormArgs a) {
     constexpr int NT = TPR < 256 ? 256 : TPR, GROUPS = NT / TPR, E = CH * 8;
-    typedef Cols<TPR, CH, VEC> C;
+    typedef Cols<TPR, CH, FULL> C;
     __shared__ float slots[2][2][NT / 64];
     GroupSum<TPR, NT> sum{slots, 0};
     const int t = threadIdx.x % TPR, group = threadIdx.x / TPR;
@@ -215,15 +262,21 @@ block_norm_forward_kernel(const NormArgs a) {
         const bool valid = base + group < a.rows;
         const long long row = valid ? base + group : a.rows - 1;
         float u[E], h[E], w[E];
-        C::load((const T*)a.x + row * a.ldx, a.D, t, u);
-        if (a.res) C::load((const R*)a.res + row * a.ldr, a.D, t, h);
+        typename C::template Raw<T> ru;
+        typename C::template Raw<R> rh;
+        typename C::template Param<T> rg, rw;
+        ru.load((const T*)a.x + row * a.ldx, a.D, t);
+        if (a.res) rh.load((const R*)a.res + row * a.ldr, a.D, t);
+        if (a.gate) rg.load(a.gate, a.gate_f32, gate_row(a, row) * a.D, a.D, t);
+        if (a.aw) rw.load(a.aw, a.after_f32, 0, a.D, t);
+        ru.get(a.D, t, u);
         if (a.after) {
             float mean, f;
             row_stats<C>(u, a, t, sum, mean, f);
 #pragma unroll
-            for (int e = 0; e < E; ++e) u[e] = C::col(t, e) < a.D ? (u[e] - mean) * f : 0.f;
+            for (int e = 0; e < E; ++e) u[e] = C::in(t, e, a.D) ? (u[e] - mean) * f : 0.f;
             if (a.aw) {
-                C::template param<T>(a.aw, a.after_f32, 0, a.D, t, w);
+                rw.get(a.after_f32, a.D, t, w);
 #pragma unroll
                 for (int e = 0; e < E; ++e) u[e] *= w[e];
             }
@@ -233,12 +286,14 @@ block_norm_forward_kernel(const NormArgs a) {
                 for (int e = 0; e < E; ++e) u[e] += w[e];
             }
         }
+        if (a.bw) rw.load(a.bw, a.before_f32, 0, a.D, t);
         if (a.gate) {
-            C::template param<T>(a.gate, a.gate_f32, row / a.rows_per_gate * a.D, a.D, t, w);
+            rg.get(a.gate_f32, a.D, t, w);
 #pragma unroll
             for (int e = 0; e < E; ++e) u[e] *= w[e];
         }
         if (a.res) {
+            rh.get(a.D, t, h);
 #pragma unroll
             for (int e = 0; e < E; ++e) h[e] = fmaf(a.scale, u[e], h[e]);
         } else {
@@ -252,7 +307,7 @@ block_norm_forward_kernel(const NormArgs a) {
 #pragma unroll
             for (int e = 0; e < E; ++e) h[e] = (h[e] - mean) * f;
             if (a.bw) {
-                C::template param<T>(a.bw, a.before_f32, 0, a.D, t, w);
+                rw.get(a.before_f32, a.D, t, w);
 #pragma unroll
                 for (int e = 0; e < E; ++e) h[e] *= w[e];
             }
@@ -272,7 +327,7 @@ __device__ __forceinline__ void write_sums(float* lds, const float (&v)[C::E], i
     if constexpr (GROUPS == 1) {
 #pragma unroll
         for (int e = 0; e < C::E; ++e)
-            if (C::col(t, e) < D) out[C::col(t, e)] = v[e];
+            if (C::in(t, e, D)) out[C::col(t, e)] = v[e];
     } else {
         // [group][e][t]: conflict free both ways
         __syncthreads();
@@ -289,11 +344,13 @@ __device__ __forceinline__ void write_sums(float* lds, const float (&v)[C::E], i
     }
 }
 
-template <typename T, typename R, int TPR, int CH, bool VEC, bool LAYER>
+// The next row of each group is on its way (as it is in memory) while one is worked on; parameters that all rows share
+// stay in registers.
+template <typename T, typename R, int TPR, int CH, bool FULL, bool LAYER>
 __global__ void __launch_bounds__(TPR < 512 ? 512 : TPR)
 block_norm_backward_kernel(const NormArgs a) {
     constexpr int NT = TPR < 512 ? 512 : TPR, GROUPS = NT / TPR, E = CH * 8;
-    typedef Cols<TPR, CH, VEC> C;
+    typedef Cols<TPR, CH, FULL> C;
     __shared__ float slots[2][2][NT / 64];
     __shared__ float lds[GROUPS > 1 ? GROUPS * E * TPR : 1];
     GroupSum<TPR, NT> sum{slots, 0};
@@ -302,77 +359,73 @@ block_norm_backward_kernel(const NormArgs a) {
     const long long s0 = (long long)(blockIdx.x / a.chunks) * a.seq_per_block;
     const long long s1 = min(a.sequences, s0 + a.seq_per_block);
     float wb[E], wa[E], wg[E], bb[E], ba[E];
+    float pa[E], pb[E], pg[E];
 #pragma unroll
-    for (int e = 0; e < E; ++e) wb[e] = wa[e] = wg[e] = bb[e] = ba[e] = 0.f;
+    for (int e = 0; e < E; ++e) {
+        wb[e] = wa[e] = wg[e] = bb[e] = ba[e] = 0.f;
+        pa[e] = pb[e] = pg[e] = 1.f;
+    }
+    if (a.aw) C::template param<T>(a.aw, a.after_f32, 0, a.D, t, pa);
+    if (a.bw) C::template param<T>(a.bw, a.before_f32, 0, a.D, t, pb);
+    if (a.gate && a.gate_shared) C::template param<T>(a.gate, a.gate_f32, 0, a.D, t, pg);
+    const bool row_gate = a.gate && !a.gate_shared;
+    typename C::template Raw<T> ru, ry;
+    typename C::template Raw<R> rh, rd;
+    typename C::template Param<T> rg;
+    auto fetch = [&](long long row) {
+        ru.load((const T*)a.x + row * a.ldx, a.D, t);
+        if (a.res) rh.load((const R*)a.res + row * a.ldr, a.D, t);
+        if (a.dy) ry.load((const T*)a.dy + row * a.D, a.D, t);
+        if (a.dh) rd.load((const R*)a.dh + row * a.D, a.D, t);
+        if (row_gate) rg.load(a.gate, a.gate_f32, gate_row(a, row) * a.D, a.D, t);
+    };
     for (long long seq = s0; seq < s1; ++seq) {
         const long long r0 = seq * a.length + chunk * a.chunk_rows;
         const long long r1 = min(seq * a.length + a.length, r0 + a.chunk_rows);
+        fetch(min(r0 + group, r1 - 1));
         for (long long base = r0; base < r1; base += GROUPS) {
             const bool valid = base + group < r1;
             const long long row = valid ? base + group : r1 - 1;
-            float u[E], h[E], d[E], dy[E], w[E];
-            C::load((const T*)a.x + row * a.ldx, a.D, t, u);
-            if (a.res) C::load((const R*)a.res + row * a.ldr, a.D, t, h);
-            if (a.dy) C::load((const T*)a.dy + row * a.D, a.D, t, dy);
-            if (a.dh) C::load((const R*)a.dh + row * a.D, a.D, t, d);
-            if (!a.res) {
+            float u[E], h[E], d[E], dy[E], p[E];
+            ru.get(a.D, t, u);
 #pragma unroll
-                for (int e = 0; e < E; ++e) h[e] = 0.f;
-            }
-            if (!a.dh) {
-#pragma unroll
-                for (int e = 0; e < E; ++e) d[e] = 0.f;
-            }
+            for (int e = 0; e < E; ++e) h[e] = d[e] = 0.f;
+            if (a.res) rh.get(a.D, t, h);
+            if (a.dy) ry.get(a.D, t, dy);
+            if (a.dh) rd.get(a.D, t, d);
+            if (row_gate) rg.get(a.gate_f32, a.D, t, pg);
+            if (base + GROUPS < r1) fetch(min(base + GROUPS + group, r1 - 1));
             // forward again: u becomes u^ (its norm without weights), h the stream
             float fu = 1.f;
             if (a.after) {
                 float mean;
                 row_stats<C>(u, a, t, sum, mean, fu);
 #pragma unroll
-                for (int e = 0; e < E; ++e) u[e] = C::col(t, e) < a.D ? (u[e] - mean) * fu : 0.f;
+                for (int e = 0; e < E; ++e) u[e] = C::in(t, e, a.D) ? (u[e] - mean) * fu : 0.f;
             }
-            float p[E];
 #pragma unroll
-            for (int e = 0; e < E; ++e) p[e] = u[e];
-            if (a.aw) {
-                C::template param<T>(a.aw, a.after_f32, 0, a.D, t, w);
-#pragma unroll
-                for (int e = 0; e < E; ++e) p[e] *= w[e];
-            }
-            if (a.ab) {
+            for (int e = 0; e < E; ++e) p[e] = u[e] * pa[e];
+            if (LAYER && a.ab) {
+                float w[E];
                 C::template param<T>(a.ab, a.after_f32, 0, a.D, t, w);
 #pragma unroll
                 for (int e = 0; e < E; ++e) p[e] += w[e];
             }
-            float g[E];
-            if (a.gate) {
-                C::template param<T>(a.gate, a.gate_f32, row / a.rows_per_gate * a.D, a.D, t, g);
-            } else {
-#pragma unroll
-                for (int e = 0; e < E; ++e) g[e] = 1.f;
-            }
             if (a.dy) {
                 float mean, f;
 #pragma unroll
-                for (int e = 0; e < E; ++e) h[e] = fmaf(a.scale, g[e] * p[e], h[e]);
+                for (int e = 0; e < E; ++e) h[e] = fmaf(a.scale, pg[e] * p[e], h[e]);
                 row_stats<C>(h, a, t, sum, mean, f);
 #pragma unroll
-                for (int e = 0; e < E; ++e) h[e] = C::col(t, e) < a.D ? (h[e] - mean) * f : 0.f;
-                if (valid) {
-#pragma unroll
-                    for (int e = 0; e < E; ++e) {
-                        wb[e] = fmaf(dy[e], h[e], wb[e]);
-                        if (LAYER) bb[e] += dy[e];
-                    }
-                }
-                if (a.bw) {
-                    C::template param<T>(a.bw, a.before_f32, 0, a.D, t, w);
-#pragma unroll
-                    for (int e = 0; e < E; ++e) dy[e] *= w[e];
-                }
+                for (int e = 0; e < E; ++e) h[e] = C::in(t, e, a.D) ? (h[e] - mean) * f : 0.f;
                 float c0 = 0.f, c1 = 0.f;
 #pragma unroll
                 for (int e = 0; e < E; ++e) {
+                    if (valid) {
+                        wb[e] = fmaf(dy[e], h[e], wb[e]);
+                        if (LAYER) bb[e] += dy[e];
+                    }
+                    dy[e] *= pb[e];
                     c0 += dy[e];
                     c1 = fmaf(dy[e], h[e], c1);
                 }
@@ -381,14 +434,14 @@ block_norm_backward_kernel(const NormArgs a) {
                 c0 *= a.inv_d;
                 c1 *= a.inv_d;
 #pragma unroll
-                for (int e = 0; e < E; ++e) d[e] += f * (dy[e] - c0 - h[e] * c1);
+                for (int e = 0; e < E; ++e) d[e] = C::in(t, e, a.D) ? d[e] + f * (dy[e] - c0 - h[e] * c1) : 0.f;
             }
             if (a.dres && valid) C::store((R*)a.dres + row * a.D, a.D, t, d);
             // gate
 #pragma unroll
             for (int e = 0; e < E; ++e) {
                 p[e] *= a.scale * d[e];
-                d[e] *= a.scale * g[e];
+                d[e] *= a.scale * pg[e];
             }
             if (a.dgate && valid) {
                 if (a.gate_f32) C::store((float*)a.dgate + row * a.D, a.D, t, p);
@@ -397,21 +450,17 @@ block_norm_backward_kernel(const NormArgs a) {
             if (valid) {
 #pragma unroll
                 for (int e = 0; e < E; ++e) {
-                    if (C::col(t, e) < a.D) wg[e] += p[e];
+                    wg[e] += p[e];
                     wa[e] = fmaf(d[e], u[e], wa[e]);
                     if (LAYER) ba[e] += d[e];
                 }
             }
             if (a.after && a.dx) {
-                if (a.aw) {
-                    C::template param<T>(a.aw, a.after_f32, 0, a.D, t, w);
-#pragma unroll
-                    for (int e = 0; e < E; ++e) d[e] *= w[e];
-                }
                 float c0 = 0.f, c1 = 0.f;
 #pragma unroll
                 for (int e = 0; e < E; ++e) {
-                    c0 += C::col(t, e) < a.D ? d[e] : 0.f;
+                    d[e] *= pa[e];
+                    c0 += d[e];
                     c1 = fmaf(d[e], u[e], c1);
                 }
                 if (LAYER) sum.two(c0, c1);
@@ -438,40 +487,51 @@ block_norm_backward_kernel(const NormArgs a) {
 }
 
 // ---------------------------------------------------------------- launch, one translation unit per element type
-// Groups by row length: up to 16 values per thread, so that the backward kernel's row (four tensors) and its
-// column sums (up to five) stay in registers.
-template <typename T, typename R, bool VEC, int TPR, int CH>
-static void norm_launch_shape(const NormArgs& a, int blocks, bool backward, hipStream_t s) {
+// Threads per row by its length: eight values each, sixteen beyond what 1024 (forward) and 512 (backward, whose row,
+// parameters and column sums share the registers) threads hold.
+template <typename T, typename R, int TPR, int CH>
+static void norm_launch_forward(const NormArgs& a, int blocks, hipStream_t s) {
+    constexpr int NT = TPR < 256 ? 256 : TPR;
+    if (a.D == TPR * CH * 8) hipLaunchKernelGGL((block_norm_forward_kernel<T, R, TPR, CH, true>), dim3(blocks), dim3(NT), 0, s, a);
+    else hipLaunchKernelGGL((block_norm_forward_kernel<T, R, TPR, CH, false>), dim3(blocks), dim3(NT), 0, s, a);
+}
+template <typename T, typename R, int TPR, int CH, bool FULL>
+static void norm_launch_backward(const NormArgs& a, int blocks, hipStream_t s) {
+    constexpr int NT = TPR < 512 ? 512 : TPR;
+    if (a.layer) hipLaunchKernelGGL((block_norm_backward_kernel<T, R, TPR, CH, FULL, true>), dim3(blocks), dim3(NT), 0, s, a);
+    else hipLaunchKernelGGL((block_norm_backward_kernel<T, R, TPR, CH, FULL, false>), dim3(blocks), dim3(NT), 0, s, a);
+}
+template <typename T, typename R, int TPR, int CH>
+static void norm_launch_backward(const NormArgs& a, int blocks, hipStream_t s) {
+    if (a.D == TPR * CH * 8) norm_launch_backward<T, R, TPR, CH, true>(a, blocks, s);
+    else norm_launch_backward<T, R, TPR, CH, false>(a, blocks, s);
+}
+
+// rows a workgroup has in hand at a time
+static inline int norm_forward_groups(int D) { return D <= 512 ? 4 : D <= 1024 ? 2 : 1; }
+static inline int norm_backward_groups(int D) { return D <= 512 ? 8 : D <= 1024 ? 4 : D <= 2048 ? 2 : 1; }
+
+template <typename T, typename R>
+static void norm_launch(const NormArgs& a, int blocks, bool backward, hipStream_t s) {
     if (!backward) {
-        constexpr int NT = TPR < 256 ? 256 : TPR;
-        hipLaunchKernelGGL((block_norm_forward_kernel<T, R, TPR, CH, VEC>), dim3(blocks), dim3(NT), 0, s, a);
+        if (a.D <= 512) norm_launch_forward<T, R, 64, 1>(a, blocks, s);
+        else if (a.D <= 1024) norm_launch_forward<T, R, 128, 1>(a, blocks, s);
+        else if (a.D <= 2048) norm_launch_forward<T, R, 256, 1>(a, blocks, s);
+        else if (a.D <= 4096) norm_launch_forward<T, R, 512, 1>(a, blocks, s);
+        else if (a.D <= 8192) norm_launch_forward<T, R, 1024, 1>(a, blocks, s);
+        else norm_launch_forward<T, R, 1024, 2>(a, blocks, s);
     } else {
-        constexpr int NT = TPR < 512 ? 512 : TPR;
-        if (a.layer) hipLaunchKernelGGL((block_norm_backward_kernel<T, R, TPR, CH, VEC, true>), dim3(blocks), dim3(NT), 0, s, a);
-        else hipLaunchKernelGGL((block_norm_backward_kernel<T, R, TPR, CH, VEC, false>), dim3(blocks), dim3(NT), 0, s, a);
+        if (a.D <= 512) norm_launch_backward<T, R, 64, 1>(a, blocks, s);
+        else if (a.D <= 1024) norm_launch_backward<T, R, 128, 1>(a, blocks, s);
+        else if (a.D <= 2048) norm_launch_backward<T, R, 256, 1>(a, blocks, s);
+        else if (a.D <= 4096) norm_launch_backward<T, R, 512, 1>(a, blocks, s);
+        else if (a.D <= 8192) norm_launch_backward<T, R, 512, 2>(a, blocks, s);
+        else norm_launch_backward<T, R, 1024, 2>(a, blocks, s);
     }
 }
 
-static inline int norm_tpr(int D) { return D <= 1024 ? 64 : D <= 2048 ? 128 : D <= 4096 ? 256 : D <= 8192 ? 512 : 1024; }
-
-template <typename T, typename R, bool VEC>
-static void norm_launch_width(const NormArgs& a, int blocks, bool backward, hipStream_t s) {
-    if (a.D <= 512) norm_launch_shape<T, R, VEC, 64, 1>(a, blocks, backward, s);
-    else if (a.D <= 1024) norm_launch_shape<T, R, VEC, 64, 2>(a, blocks, backward, s);
-    else if (a.D <= 2048) norm_launch_shape<T, R, VEC, 128, 2>(a, blocks, backward, s);
-    else if (a.D <= 4096) norm_launch_shape<T, R, VEC, 256, 2>(a, blocks, backward, s);
-    else if (a.D <= 8192) norm_launch_shape<T, R, VEC, 512, 2>(a, blocks, backward, s);
-    else norm_launch_shape<T, R, VEC, 1024, 2>(a, blocks, backward, s);
-}
-
-template <typename T, typename R>
-static void norm_launch(const NormArgs& a, bool vec, int blocks, bool backward, hipStream_t s) {
-    if (vec) norm_launch_width<T, R, true>(a, blocks, backward, s);
-    else norm_launch_width<T, R, false>(a, blocks, backward, s);
-}
-
-void block_norm_launch_bf16(const NormArgs& a, bool stream_f32, bool vec, int blocks, bool backward, hipStream_t s);
-void block_norm_launch_f16(const NormArgs& a, bool stream_f32, bool vec, int blocks, bool backward, hipStream_t s);
-void block_norm_launch_f32(const NormArgs& a, bool vec, int blocks, bool backward, hipStream_t s);
+void block_norm_launch_bf16(const NormArgs& a, bool stream_f32, int blocks, bool backward, hipStream_t s);
+void block_norm_launch_f16(const NormArgs& a, bool stream_f32, int blocks, bool backward, hipStream_t s);
+void block_norm_launch_f32(const NormArgs& a, int blocks, bool backward, hipStream_t s);
 
 }  // namespace yolo_amd

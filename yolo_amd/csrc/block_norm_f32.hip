@@ -3,8 +3,8 @@
 
 namespace yolo_amd {
 
-void block_norm_launch_f32(const NormArgs& a, bool vec, int blocks, bool backward, hipStream_t s) {
-    norm_launch<float, float>(a, vec, blocks, backward, s);
+void block_norm_launch_f32(const NormArgs& a, int blocks, bool backward, hipStream_t s) {
+    norm_launch<float, float>(a, blocks, backward, s);
 }
 
 // Sums of partial column sums: out[o][c] = sum over b of part[(o * blocks + b) * stride + c], b ascending within
@@ -45,7 +45,7 @@ static int check(const char* me, const yolo_amd_block_norm_desc* d) {
     YA_REQUIRE(d, "%s: null descriptor", me);
     YA_REQUIRE(d->type >= YOLO_AMD_TYPE_F32 && d->type <= YOLO_AMD_TYPE_F16, "%s: type %d", me, d->type);
     YA_REQUIRE(d->norm == YOLO_AMD_NORM_RMS || d->norm == YOLO_AMD_NORM_LAYER, "%s: norm %d", me, d->norm);
-    YA_REQUIRE(d->rows >= 0 && d->rows < (1ll << 40) && d->d >= 1 && d->d <= kMaxWidth,
+    YA_REQUIRE(d->rows >= 0 && d->rows < (1ll << 31) && d->d >= 1 && d->d <= kMaxWidth,
                "%s: %lld rows of %lld values (rows of 1 to %d values)", me, (long long)d->rows, (long long)d->d, kMaxWidth);
     YA_REQUIRE(d->eps >= 0.f, "%s: eps=%g", me, (double)d->eps);
     YA_REQUIRE(!d->gate || d->rows_per_gate >= 1, "%s: rows_per_gate=%lld", me, (long long)d->rows_per_gate);
@@ -75,23 +75,16 @@ static NormArgs arguments(const yolo_amd_block_norm_desc* d) {
     a.rows = d->rows; a.D = (int)d->d;
     a.gate_f32 = d->gate_f32 || f32; a.after_f32 = d->after_f32 || f32; a.before_f32 = d->before_f32 || f32;
     a.rows_per_gate = d->gate ? d->rows_per_gate : 1;
+    a.gate_shared = d->gate && d->rows_per_gate >= d->rows;
     a.after = d->after != 0; a.before = d->before != 0; a.layer = d->norm == YOLO_AMD_NORM_LAYER;
     a.eps = d->eps; a.scale = d->scale; a.inv_d = 1.f / (float)d->d;
     return a;
 }
 
-static bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
-static bool vec_inputs(const yolo_amd_block_norm_desc* d) {
-    const int e = d->type == YOLO_AMD_TYPE_F32 ? 4 : 2, r = d->stream_f32 ? 4 : e;
-    return d->d % 8 == 0 && aligned16(d->x) && aligned16(d->residual) && aligned16(d->gate) && aligned16(d->after_weight) &&
-           aligned16(d->after_bias) && aligned16(d->before_weight) && aligned16(d->before_bias) &&
-           (d->rows == 1 || ((d->ldx * e) % 16 == 0 && (!d->residual || (d->ldr * r) % 16 == 0)));
-}
-
-static int launch(const yolo_amd_block_norm_desc* d, const NormArgs& a, bool vec, int blocks, bool backward, hipStream_t s) {
-    if (d->type == YOLO_AMD_TYPE_BF16) block_norm_launch_bf16(a, d->stream_f32 != 0, vec, blocks, backward, s);
-    else if (d->type == YOLO_AMD_TYPE_F16) block_norm_launch_f16(a, d->stream_f32 != 0, vec, blocks, backward, s);
-    else block_norm_launch_f32(a, vec, blocks, backward, s);
+static int launch(const yolo_amd_block_norm_desc* d, const NormArgs& a, int blocks, bool backward, hipStream_t s) {
+    if (d->type == YOLO_AMD_TYPE_BF16) block_norm_launch_bf16(a, d->stream_f32 != 0, blocks, backward, s);
+    else if (d->type == YOLO_AMD_TYPE_F16) block_norm_launch_f16(a, d->stream_f32 != 0, blocks, backward, s);
+    else block_norm_launch_f32(a, blocks, backward, s);
     YA_CHECK_HIP(hipGetLastError());
     return YA_OK;
 }
@@ -116,7 +109,7 @@ static BackwardPlan plan(const yolo_amd_block_norm_backward_desc* b) {
     p.sequence_gate = want_gate && !p.token_gate && !p.channel_gate;
     p.length = p.sequence_gate ? d->rows_per_gate : d->rows;
     p.sequences = (d->rows + p.length - 1) / p.length;
-    const int tpr = norm_tpr((int)d->d), groups = tpr < 512 ? 512 / tpr : 1;
+    const int groups = norm_backward_groups((int)d->d);
     const long long target = 512;
     if (p.sequences >= target) {
         p.chunks = 1;
@@ -178,10 +171,9 @@ extern "C" int yolo_amd_block_norm_forward(const yolo_amd_block_norm_desc* d, vo
     NormArgs a = arguments(d);
     a.h = d->stream;
     a.y = d->normed;
-    const bool vec = vec_inputs(d) && aligned16(d->stream) && aligned16(d->normed);
-    const int tpr = norm_tpr(a.D), groups = tpr < 256 ? 256 / tpr : 1;
+    const int groups = norm_forward_groups(a.D);
     const long long blocks = std::min<long long>((d->rows + groups - 1) / groups, 1 << 20);
-    return launch(d, a, vec, (int)blocks, false, (hipStream_t)stream);
+    return launch(d, a, (int)blocks, false, (hipStream_t)stream);
 }
 
 extern "C" size_t yolo_amd_block_norm_backward_workspace_bytes(const yolo_amd_block_norm_backward_desc* b) {
@@ -196,7 +188,6 @@ extern "C" int yolo_amd_block_norm_backward(const yolo_amd_block_norm_backward_d
     const yolo_amd_block_norm_desc* d = &b->forward;
     hipStream_t s = (hipStream_t)stream;
     NormArgs a = arguments(d);
-    const int e = d->type == YOLO_AMD_TYPE_F32 ? 4 : 2;
     if (d->rows == 0) {                          // sums over no rows are zero
         void* out[5] = {b->dafter_weight, b->dafter_bias, b->dbefore_weight, b->dbefore_bias, nullptr};
         const int f32[5] = {a.after_f32, a.after_f32, a.before_f32, a.before_f32, 0};
@@ -228,10 +219,7 @@ extern "C" int yolo_amd_block_norm_backward(const yolo_amd_block_norm_backward_d
     a.at_ba = b->dafter_bias ? at++ : -1;
     a.sequences = p.sequences; a.length = p.length; a.chunk_rows = p.chunk_rows;
     a.seq_per_block = p.seq_per_block; a.chunks = p.chunks;
-    const bool vec = vec_inputs(d) && aligned16(b->dnormed) && aligned16(b->dstream) && aligned16(b->dx) && aligned16(b->dresidual) &&
-                     aligned16(a.dgate);
-    (void)e;
-    YA_TRY(launch(d, a, vec, p.blocks, true, s));
+    YA_TRY(launch(d, a, p.blocks, true, s));
     SumArgs g{};
     g.D = a.D;
     g.type = d->type;
