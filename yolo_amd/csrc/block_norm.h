@@ -23,6 +23,7 @@
 namespace yolo_amd {
 
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
 
 struct NormArgs {
     const void *x, *res, *gate, *aw, *ab, *bw, *bb;
@@ -321,50 +322,93 @@ block_norm_forward_kernel(const NormArgs a) {
     }
 }
 
-// Adds the column sums v of a workgroup's groups in group order and writes them to out[0 .. D).
-template <typename C, int TPR, int GROUPS>
-__device__ __forceinline__ void write_sums(float* lds, const float (&v)[C::E], int t, int group, int D, float* out) {
-    if constexpr (GROUPS == 1) {
+// The column sums of a workgroup: N vectors, each thread's eight columns of each.  In LDS while a thread has eight columns
+// (a thread only ever touches its own words, in order): the registers they would take hide more of memory's latency as
+// further waves.  Sixteen columns would not fit there and stay in registers.
+template <typename C, int TPR, int GROUPS, int N>
+struct Sums {
+    static constexpr bool LDS = C::E == 8;
+    static constexpr int NT = TPR * GROUPS, WORDS = LDS ? N * 2 * NT : GROUPS > 1 ? GROUPS * C::E * TPR / 4 : 1;
+    f32x4* lds;                                        // WORDS of them
+    float v[LDS ? 1 : N][C::E];
+
+    __device__ __forceinline__ void clear(int k) {
+        if constexpr (LDS) {
+            lds[(k * 2) * NT + threadIdx.x] = lds[(k * 2 + 1) * NT + threadIdx.x] = f32x4{0.f, 0.f, 0.f, 0.f};
+        } else {
 #pragma unroll
-        for (int e = 0; e < C::E; ++e)
-            if (C::in(t, e, D)) out[C::col(t, e)] = v[e];
-    } else {
-        // [group][e][t]: conflict free both ways
-        __syncthreads();
-#pragma unroll
-        for (int e = 0; e < C::E; ++e) lds[(group * C::E + e) * TPR + t] = v[e];
-        __syncthreads();
-        for (int i = threadIdx.x; i < C::E * TPR; i += GROUPS * TPR) {
-            float s = lds[i];
-#pragma unroll
-            for (int g = 1; g < GROUPS; ++g) s += lds[g * C::E * TPR + i];
-            const int c = C::col(i % TPR, i / TPR);
-            if (c < D) out[c] = s;
+            for (int e = 0; e < C::E; ++e) v[k][e] = 0.f;
         }
     }
-}
+    // sums[k] += x * y
+    __device__ __forceinline__ void add(int k, const float (&x)[C::E], const float (&y)[C::E]) {
+        if constexpr (LDS) {
+#pragma unroll
+            for (int q = 0; q < 2; ++q) {
+                f32x4 s = lds[(k * 2 + q) * NT + threadIdx.x];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) s[i] = fmaf(x[q * 4 + i], y[q * 4 + i], s[i]);
+                lds[(k * 2 + q) * NT + threadIdx.x] = s;
+            }
+        } else {
+#pragma unroll
+            for (int e = 0; e < C::E; ++e) v[k][e] = fmaf(x[e], y[e], v[k][e]);
+        }
+    }
+    __device__ __forceinline__ void add(int k, const float (&x)[C::E]) {
+        float one[C::E];
+#pragma unroll
+        for (int e = 0; e < C::E; ++e) one[e] = 1.f;
+        add(k, x, one);
+    }
+    // the groups' sums in group order -> out[0 .. D); every thread calls it
+    __device__ __forceinline__ void write(int k, int t, int group, int D, float* out) {
+        if constexpr (LDS) {
+            __syncthreads();
+            if (group == 0) {
+#pragma unroll
+                for (int q = 0; q < 2; ++q) {
+                    f32x4 s = lds[(k * 2 + q) * NT + t];
+#pragma unroll
+                    for (int g = 1; g < GROUPS; ++g) s += lds[(k * 2 + q) * NT + g * TPR + t];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        if (C::in(t, q * 4 + i, D)) out[C::col(t, q * 4 + i)] = s[i];
+                }
+            }
+            __syncthreads();
+        } else {
+            static_assert(LDS || GROUPS == 1, "rows this long have a workgroup each");
+#pragma unroll
+            for (int e = 0; e < C::E; ++e)
+                if (C::in(t, e, D)) out[C::col(t, e)] = v[k][e];
+        }
+    }
+};
 
 // The next row of each group is on its way (as it is in memory) while one is worked on; parameters that all rows share
 // stay in registers.
 template <typename T, typename R, int TPR, int CH, bool FULL, bool LAYER>
-__global__ void __launch_bounds__(TPR < 512 ? 512 : TPR)
+__global__ void __launch_bounds__(TPR < 256 ? 256 : TPR)
 block_norm_backward_kernel(const NormArgs a) {
-    constexpr int NT = TPR < 512 ? 512 : TPR, GROUPS = NT / TPR, E = CH * 8;
+    constexpr int NT = TPR < 256 ? 256 : TPR, GROUPS = NT / TPR, E = CH * 8;
     typedef Cols<TPR, CH, FULL> C;
     __shared__ float slots[2][2][NT / 64];
-    __shared__ float lds[GROUPS > 1 ? GROUPS * E * TPR : 1];
+    enum { WB, WA, WG, BB, BA };
+    typedef Sums<C, TPR, GROUPS, LAYER ? 5 : 3> S;
+    __shared__ f32x4 words[S::WORDS];
+    S sums;
+    sums.lds = words;
     GroupSum<TPR, NT> sum{slots, 0};
     const int t = threadIdx.x % TPR, group = threadIdx.x / TPR;
     const int chunk = blockIdx.x % a.chunks;
     const long long s0 = (long long)(blockIdx.x / a.chunks) * a.seq_per_block;
     const long long s1 = min(a.sequences, s0 + a.seq_per_block);
-    float wb[E], wa[E], wg[E], bb[E], ba[E];
+#pragma unroll
+    for (int k = 0; k < (LAYER ? 5 : 3); ++k) sums.clear(k);
     float pa[E], pb[E], pg[E];
 #pragma unroll
-    for (int e = 0; e < E; ++e) {
-        wb[e] = wa[e] = wg[e] = bb[e] = ba[e] = 0.f;
-        pa[e] = pb[e] = pg[e] = 1.f;
-    }
+    for (int e = 0; e < E; ++e) pa[e] = pb[e] = pg[e] = 1.f;
     if (a.aw) C::template param<T>(a.aw, a.after_f32, 0, a.D, t, pa);
     if (a.bw) C::template param<T>(a.bw, a.before_f32, 0, a.D, t, pb);
     if (a.gate && a.gate_shared) C::template param<T>(a.gate, a.gate_f32, 0, a.D, t, pg);
@@ -418,13 +462,13 @@ block_norm_backward_kernel(const NormArgs a) {
                 row_stats<C>(h, a, t, sum, mean, f);
 #pragma unroll
                 for (int e = 0; e < E; ++e) h[e] = C::in(t, e, a.D) ? (h[e] - mean) * f : 0.f;
+                if (valid) {
+                    if (a.at_wb >= 0) sums.add(WB, dy, h);
+                    if (LAYER && a.at_bb >= 0) sums.add(BB, dy);
+                }
                 float c0 = 0.f, c1 = 0.f;
 #pragma unroll
                 for (int e = 0; e < E; ++e) {
-                    if (valid) {
-                        wb[e] = fmaf(dy[e], h[e], wb[e]);
-                        if (LAYER) bb[e] += dy[e];
-                    }
                     dy[e] *= pb[e];
                     c0 += dy[e];
                     c1 = fmaf(dy[e], h[e], c1);
@@ -448,12 +492,9 @@ block_norm_backward_kernel(const NormArgs a) {
                 else C::store((T*)a.dgate + row * a.D, a.D, t, p);
             }
             if (valid) {
-#pragma unroll
-                for (int e = 0; e < E; ++e) {
-                    wg[e] += p[e];
-                    wa[e] = fmaf(d[e], u[e], wa[e]);
-                    if (LAYER) ba[e] += d[e];
-                }
+                if (a.gate_part || a.at_g >= 0) sums.add(WG, p);
+                if (a.at_wa >= 0) sums.add(WA, d, u);
+                if (LAYER && a.at_ba >= 0) sums.add(BA, d);
             }
             if (a.after && a.dx) {
                 float c0 = 0.f, c1 = 0.f;
@@ -473,17 +514,16 @@ block_norm_backward_kernel(const NormArgs a) {
             if (a.dx && valid) C::store((T*)a.dx + row * a.D, a.D, t, d);
         }
         if (a.gate_part) {
-            write_sums<C, TPR, GROUPS>(lds, wg, t, group, a.D, a.gate_part + (seq * a.chunks + chunk) * a.D);
-#pragma unroll
-            for (int e = 0; e < E; ++e) wg[e] = 0.f;
+            sums.write(WG, t, group, a.D, a.gate_part + (seq * a.chunks + chunk) * a.D);
+            sums.clear(WG);
         }
     }
     float* out = a.part + (long long)blockIdx.x * a.vectors * a.D;
-    if (a.at_wb >= 0) write_sums<C, TPR, GROUPS>(lds, wb, t, group, a.D, out + (long long)a.at_wb * a.D);
-    if (a.at_wa >= 0) write_sums<C, TPR, GROUPS>(lds, wa, t, group, a.D, out + (long long)a.at_wa * a.D);
-    if (a.at_g >= 0) write_sums<C, TPR, GROUPS>(lds, wg, t, group, a.D, out + (long long)a.at_g * a.D);
-    if (LAYER && a.at_bb >= 0) write_sums<C, TPR, GROUPS>(lds, bb, t, group, a.D, out + (long long)a.at_bb * a.D);
-    if (LAYER && a.at_ba >= 0) write_sums<C, TPR, GROUPS>(lds, ba, t, group, a.D, out + (long long)a.at_ba * a.D);
+    if (a.at_wb >= 0) sums.write(WB, t, group, a.D, out + (long long)a.at_wb * a.D);
+    if (a.at_wa >= 0) sums.write(WA, t, group, a.D, out + (long long)a.at_wa * a.D);
+    if (a.at_g >= 0) sums.write(WG, t, group, a.D, out + (long long)a.at_g * a.D);
+    if (LAYER && a.at_bb >= 0) sums.write(BB, t, group, a.D, out + (long long)a.at_bb * a.D);
+    if (LAYER && a.at_ba >= 0) sums.write(BA, t, group, a.D, out + (long long)a.at_ba * a.D);
 }
 
 // ---------------------------------------------------------------- launch, one translation unit per element type
@@ -497,7 +537,7 @@ static void norm_launch_forward(const NormArgs& a, int blocks, hipStream_t s) {
 }
 template <typename T, typename R, int TPR, int CH, bool FULL>
 static void norm_launch_backward(const NormArgs& a, int blocks, hipStream_t s) {
-    constexpr int NT = TPR < 512 ? 512 : TPR;
+    constexpr int NT = TPR < 256 ? 256 : TPR;
     if (a.layer) hipLaunchKernelGGL((block_norm_backward_kernel<T, R, TPR, CH, FULL, true>), dim3(blocks), dim3(NT), 0, s, a);
     else hipLaunchKernelGGL((block_norm_backward_kernel<T, R, TPR, CH, FULL, false>), dim3(blocks), dim3(NT), 0, s, a);
 }
@@ -509,7 +549,7 @@ static void norm_launch_backward(const NormArgs& a, int blocks, hipStream_t s) {
 
 // rows a workgroup has in hand at a time
 static inline int norm_forward_groups(int D) { return D <= 512 ? 4 : D <= 1024 ? 2 : 1; }
-static inline int norm_backward_groups(int D) { return D <= 512 ? 8 : D <= 1024 ? 4 : D <= 2048 ? 2 : 1; }
+static inline int norm_backward_groups(int D) { return D <= 512 ? 4 : D <= 1024 ? 2 : 1; }
 
 template <typename T, typename R>
 static void norm_launch(const NormArgs& a, int blocks, bool backward, hipStream_t s) {
