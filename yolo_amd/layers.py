@@ -17,33 +17,42 @@ The reference has no counterpart of either.
 """
 from __future__ import annotations
 
-import ctypes
-
 import torch
 
 from . import _lib
 from ._lib import BlockNormBackwardDesc, BlockNormDesc, LinearBackwardDesc, LinearDesc, YoloAmdError, check, lib
 
+# A call's own work on the host is what bounds it at few rows: descriptors are filled in one constructor call, the
+# stream is asked for as a number, nothing is looked up twice.
 _TYPES = {torch.float32: _lib.TYPE_F32, torch.bfloat16: _lib.TYPE_BF16, torch.float16: _lib.TYPE_F16}
 _F32 = torch.float32
-_byref = ctypes.byref
+_empty = torch.empty
+_current_device = torch.cuda.current_device
 
 
-def _on_gpu(what, first, **others):
-    """Every tensor is a GPU tensor on the first one's device."""
-    if not torch.is_tensor(first):
-        raise TypeError(f"{what}: expected a torch tensor, got {type(first).__name__}")
-    dev = first.device
-    if dev.type != "cuda":
-        raise YoloAmdError(f"{what}: the tensors are on the CPU; this path runs on the GPU only")
-    for name, t in others.items():
+def _raw_stream(index):
+    return torch.cuda.current_stream(index).cuda_stream
+
+
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", _raw_stream)
+
+
+def _on_gpu(what, **tensors):
+    """Every argument is a tensor (or None) on one GPU, the first one's.  Returns its index."""
+    index = None
+    for name, t in tensors.items():
         if t is None:
             continue
         if not torch.is_tensor(t):
-            raise TypeError(f"{what}: {name} is not a torch tensor")
-        if t.device != dev:
-            raise YoloAmdError(f"{what}: {name} is on {t.device}, the first argument on {dev}")
-    return dev
+            raise TypeError(f"{what}: {name} is not a torch tensor but {type(t).__name__}")
+        i = t.get_device() if t.is_cuda else -1
+        if index is None:
+            index = i
+            if i < 0:
+                raise YoloAmdError(f"{what}: {name} is on the CPU; this path runs on the GPU only")
+        elif i != index:
+            raise YoloAmdError(f"{what}: {name} is on {t.device}, the first argument on cuda:{index}")
+    return index
 
 
 def _rows(t):
@@ -63,27 +72,23 @@ def _rows(t):
     return t, shape[-1]
 
 
-def _call(dev, fn, desc, what):
-    """Run ``fn(desc, current stream)`` on ``dev``."""
-    if dev.index == torch.cuda.current_device():
-        check(fn(_byref(desc), torch.cuda.current_stream(dev).cuda_stream), what)
+def _call(index, fn, desc, what):
+    """Run ``fn(desc, current stream)`` on GPU ``index``."""
+    if index == _current_device():
+        rc = fn(desc, _raw_stream(index))
     else:
-        with torch.cuda.device(dev):
-            check(fn(_byref(desc), torch.cuda.current_stream(dev).cuda_stream), what)
+        with torch.cuda.device(index):
+            rc = fn(desc, _raw_stream(index))
+    if rc:
+        check(rc, what)
 
 
-def _scratch(desc, nbytes, dev):
+def _scratch(desc, nbytes, like):
     """Scratch of one call.  Taken from torch's allocator each time: calls on different streams, or in different
     captured graphs, never share it."""
-    if nbytes == 0:
-        return None
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    ws = _empty(nbytes, dtype=torch.uint8, device=like.device)
     desc.workspace, desc.workspace_bytes = ws.data_ptr(), nbytes
     return ws
-
-
-def _ptr(t):
-    return None if t is None else t.data_ptr()
 
 
 # --------------------------------------------------------------------------
@@ -92,76 +97,81 @@ def _ptr(t):
 def _linear_forward(x, weight, bias, residual, act, out_dtype, keep_pre):
     """Returns (y, pre or None)."""
     n, k = weight.shape
-    xr, ldx = _rows(x)
-    wr, ldw = _rows(weight)
+    dt, dev = x.dtype, x.device
+    x, ldx = _rows(x)
+    weight, ldw = _rows(weight)
     shape = x.shape[:-1] + (n,)
     m = x.numel() // k if k else shape.numel() // n if n else 0
-    y = torch.empty(shape, dtype=out_dtype, device=x.device)
-    d = LinearDesc()
-    d.x, d.weight, d.y = xr.data_ptr(), wr.data_ptr(), y.data_ptr()
-    d.m, d.n, d.k, d.ldx, d.ldw, d.ldy = m, n, k, ldx, ldw, n
-    d.type, d.y_f32, d.activation = _TYPES[x.dtype], out_dtype == _F32, act
+    y = _empty(shape, dtype=out_dtype, device=dev)
+    b = r = p = ldr = 0
+    b32 = r32 = False
+    pre = None
     if bias is not None:
         bias = bias.contiguous()
-        d.bias, d.bias_f32 = bias.data_ptr(), bias.dtype == _F32
+        b, b32 = bias.data_ptr(), bias.dtype is _F32
     if residual is not None:
-        rr, d.ldr = _rows(residual)
-        d.residual, d.residual_f32 = rr.data_ptr(), residual.dtype == _F32
-    pre = None
+        residual, ldr = _rows(residual)
+        r, r32 = residual.data_ptr(), residual.dtype is _F32
     if keep_pre:
-        pre = torch.empty(shape, dtype=x.dtype, device=x.device)
-        d.pre = pre.data_ptr()
-    ws = _scratch(d, lib.yolo_amd_linear_workspace_bytes(_byref(d)), x.device)     # noqa: F841  (alive over the call)
-    _call(x.device, lib.yolo_amd_linear_forward, d, "linear")
+        pre = _empty(shape, dtype=dt, device=dev)
+        p = pre.data_ptr()
+    d = LinearDesc(x.data_ptr(), weight.data_ptr(), b, r, y.data_ptr(), p, m, n, k, ldx, ldw, ldr, n, _TYPES[dt], b32, r32,
+                   out_dtype is _F32, act)
+    nbytes = lib.yolo_amd_linear_workspace_bytes(d)
+    ws = _scratch(d, nbytes, y) if nbytes else None      # noqa: F841  (alive over the call)
+    _call(x.get_device(), lib.yolo_amd_linear_forward, d, "linear")
     return y, pre
+
+
+def _linear_backward(ctx, dy):
+    need_x, need_w, need_b, need_r = ctx.needs_input_grad[:4]
+    act, x_shape, w_shape, dt, b_dtype, r_dtype = ctx.conf
+    dres = (dy if dy.dtype is r_dtype else dy.to(r_dtype)) if need_r else None
+    if not (need_x or need_w or need_b):
+        return None, None, None, dres, None, None
+    x, weight, pre = ctx.saved_tensors
+    n, k = w_shape
+    dev = dy.device
+    dyr, lddy = _rows(dy)
+    m = dy.numel() // n if n else x_shape[:-1].numel()
+    xp = wp = dxp = dwp = dbp = ldx = ldw = 0
+    dx = dw = db = None
+    if need_x:
+        weight, ldw = _rows(weight)
+        dx = _empty(x_shape, dtype=dt, device=dev)
+        wp, dxp = weight.data_ptr(), dx.data_ptr()
+    if need_w:
+        x, ldx = _rows(x)
+        dw = _empty(w_shape, dtype=dt, device=dev)
+        xp, dwp = x.data_ptr(), dw.data_ptr()
+    if need_b:
+        db = _empty(n, dtype=b_dtype, device=dev)
+        dbp = db.data_ptr()
+    d = LinearBackwardDesc(dyr.data_ptr(), xp, wp, 0 if pre is None else pre.data_ptr(), dxp, dwp, dbp, m, n, k, lddy, ldx,
+                           ldw, _TYPES[dt], dy.dtype is _F32, b_dtype is _F32, act)
+    nbytes = lib.yolo_amd_linear_backward_workspace_bytes(d)
+    ws = _scratch(d, nbytes, dy) if nbytes else None      # noqa: F841
+    _call(dy.get_device(), lib.yolo_amd_linear_backward, d, "linear backward")
+    return dx, dw, db, dres, None, None
+
+
+_linear_backward_once = torch.autograd.function.once_differentiable(_linear_backward)
 
 
 class _Linear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, residual, act, out_dtype):
-        need_pre = act != 0 and any(ctx.needs_input_grad[:3])
-        y, pre = _linear_forward(x, weight, bias, residual, act, out_dtype, need_pre)
         need = ctx.needs_input_grad
+        y, pre = _linear_forward(x, weight, bias, residual, act, out_dtype, act != 0 and (need[0] or need[1] or need[2]))
         ctx.save_for_backward(x if need[1] else None, weight if need[0] else None, pre)
-        ctx.act, ctx.k = act, weight.shape[1]
-        ctx.x_shape, ctx.w_shape, ctx.type = x.shape, weight.shape, x.dtype
-        ctx.bias_dtype = bias.dtype if bias is not None else None
-        ctx.residual_dtype = residual.dtype if residual is not None else None
+        ctx.conf = (act, x.shape, weight.shape, x.dtype, None if bias is None else bias.dtype,
+                    None if residual is None else residual.dtype)
         return y
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
-        need = ctx.needs_input_grad
-        dres = None
-        if need[3]:
-            dres = dy if dy.dtype == ctx.residual_dtype else dy.to(ctx.residual_dtype)
-        if not any(need[:3]):
-            return None, None, None, dres, None, None
-        x, weight, pre = ctx.saved_tensors
-        n, k = ctx.w_shape
-        dev = dy.device
-        dyr, lddy = _rows(dy)
-        d = LinearBackwardDesc()
-        d.dy, d.lddy, d.dy_f32 = dyr.data_ptr(), lddy, dy.dtype == _F32
-        d.m, d.n, d.k = (dy.numel() // n if n else ctx.x_shape[:-1].numel()), n, k
-        d.type, d.activation = _TYPES[ctx.type], ctx.act
-        d.pre = _ptr(pre)
-        dx = dw = db = None
-        if need[0]:
-            wr, d.ldw = _rows(weight)
-            dx = torch.empty(ctx.x_shape, dtype=ctx.type, device=dev)
-            d.weight, d.dx = wr.data_ptr(), dx.data_ptr()
-        if need[1]:
-            xr, d.ldx = _rows(x)
-            dw = torch.empty(ctx.w_shape, dtype=ctx.type, device=dev)
-            d.x, d.dweight = xr.data_ptr(), dw.data_ptr()
-        if need[2]:
-            db = torch.empty(n, dtype=ctx.bias_dtype, device=dev)
-            d.dbias, d.dbias_f32 = db.data_ptr(), ctx.bias_dtype == _F32
-        ws = _scratch(d, lib.yolo_amd_linear_backward_workspace_bytes(_byref(d)), dev)     # noqa: F841
-        _call(dev, lib.yolo_amd_linear_backward, d, "linear backward")
-        return dx, dw, db, dres, None, None
+        # (the wrapper that refuses a second derivative costs as much as a launch: only where one could follow)
+        return (_linear_backward_once if torch.is_grad_enabled() else _linear_backward)(ctx, dy)
 
 
 def linear(x, weight, bias=None, *, activation=None, residual=None, out_dtype=None):
@@ -174,9 +184,9 @@ def linear(x, weight, bias=None, *, activation=None, residual=None, out_dtype=No
     Sums are fp32; the result is rounded once.  Where a gradient of x, weight or bias will be wanted and there is
     an activation, ``x @ weight.T + bias`` is kept in x's type for the backward pass; the gradients of x and
     weight round d(loss)/d(pre-activation) to that type once, as the operand of their products."""
-    dev = _on_gpu("linear", x, weight=weight, bias=bias, residual=residual)
+    _on_gpu("linear", x=x, weight=weight, bias=bias, residual=residual)
     dt = x.dtype
-    if dt not in (torch.bfloat16, torch.float16):
+    if dt is not torch.bfloat16 and dt is not torch.float16:
         raise TypeError(f"linear: x must be bfloat16 or float16, got {dt}")
     if weight.dtype != dt:
         raise TypeError(f"linear: weight is {weight.dtype}, x is {dt}")
@@ -203,87 +213,87 @@ def linear(x, weight, bias=None, *, activation=None, residual=None, out_dtype=No
 # --------------------------------------------------------------------------
 # block_norm
 # --------------------------------------------------------------------------
-def _norm_desc(x, residual, gate, after_weight, after_bias, before_weight, before_bias, conf):
-    """(descriptor without outputs, tensors to keep alive over the call)."""
+def _norm_desc(x, residual, gate, after_weight, after_bias, before_weight, before_bias, conf, stream, normed):
+    """(descriptor, tensors to keep alive over the call)."""
     norm, after, before, scale, eps, rows_per_gate = conf
-    d = BlockNormDesc()
+    dt = x.dtype
     dim = x.shape[-1]
-    xr, d.ldx = _rows(x)
-    keep = [xr]
-    d.x, d.rows, d.d = xr.data_ptr(), x.numel() // dim, dim
-    d.type, d.norm, d.after, d.before, d.eps, d.scale = _TYPES[x.dtype], norm, after, before, eps, scale
+    x, ldx = _rows(x)
+    r = g = aw = ab = bw = bb = ldr = 0
+    g32 = a32 = b32 = False
+    r32 = dt is _F32
     if residual is not None:
-        rr, d.ldr = _rows(residual)
-        keep.append(rr)
-        d.residual, d.stream_f32 = rr.data_ptr(), residual.dtype == _F32
-    else:
-        d.stream_f32 = x.dtype == _F32
+        residual, ldr = _rows(residual)
+        r, r32 = residual.data_ptr(), residual.dtype is _F32
     if gate is not None:
         gate = gate.contiguous()
-        keep.append(gate)
-        d.gate, d.gate_f32, d.rows_per_gate = gate.data_ptr(), gate.dtype == _F32, rows_per_gate
-    for name, t in (("after_weight", after_weight), ("after_bias", after_bias), ("before_weight", before_weight),
-                    ("before_bias", before_bias)):
-        if t is not None:
-            t = t.contiguous()
-            keep.append(t)
-            setattr(d, name, t.data_ptr())
-            if name[0] == "a":
-                d.after_f32 = t.dtype == _F32
-            else:
-                d.before_f32 = t.dtype == _F32
-    return d, keep
+        g, g32 = gate.data_ptr(), gate.dtype is _F32
+    if after_weight is not None:
+        after_weight = after_weight.contiguous()
+        aw, a32 = after_weight.data_ptr(), after_weight.dtype is _F32
+    if after_bias is not None:
+        after_bias = after_bias.contiguous()
+        ab, a32 = after_bias.data_ptr(), after_bias.dtype is _F32
+    if before_weight is not None:
+        before_weight = before_weight.contiguous()
+        bw, b32 = before_weight.data_ptr(), before_weight.dtype is _F32
+    if before_bias is not None:
+        before_bias = before_bias.contiguous()
+        bb, b32 = before_bias.data_ptr(), before_bias.dtype is _F32
+    d = BlockNormDesc(x.data_ptr(), r, g, aw, ab, bw, bb, stream, normed, x.numel() // dim, dim, ldx, ldr, rows_per_gate,
+                      _TYPES[dt], norm, after, before, r32, g32, a32, b32, eps, scale)
+    return d, (x, residual, gate, after_weight, after_bias, before_weight, before_bias)
 
 
 def _norm_forward(x, residual, gate, after_weight, after_bias, before_weight, before_bias, conf, own_stream):
     """(stream or None where it is x itself, normed or None)."""
-    d, keep = _norm_desc(x, residual, gate, after_weight, after_bias, before_weight, before_bias, conf)
     stream = normed = None
+    s = n = 0
     if own_stream:
-        stream = torch.empty(x.shape, dtype=x.dtype if residual is None else residual.dtype, device=x.device)
-        d.stream = stream.data_ptr()
+        stream = _empty(x.shape, dtype=x.dtype if residual is None else residual.dtype, device=x.device)
+        s = stream.data_ptr()
     if conf[2]:
-        normed = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-        d.normed = normed.data_ptr()
-    _call(x.device, lib.yolo_amd_block_norm_forward, d, "block_norm")
+        normed = _empty(x.shape, dtype=x.dtype, device=x.device)
+        n = normed.data_ptr()
+    d, keep = _norm_desc(x, residual, gate, after_weight, after_bias, before_weight, before_bias, conf, s, n)
+    _call(x.get_device(), lib.yolo_amd_block_norm_forward, d, "block_norm")
     return stream, normed
+
+
+def _norm_backward(ctx, dstream, dnormed):
+    tensors = ctx.saved_tensors
+    dev = tensors[0].device
+    d, keep = _norm_desc(*tensors, ctx.conf, 0, 0)
+    ds = dn = 0
+    if dnormed is not None:
+        dnormed = dnormed.contiguous()
+        dn = dnormed.data_ptr()
+    if dstream is not None:
+        dstream = dstream.contiguous()
+        ds = dstream.data_ptr()
+    grads = [_empty(t.shape, dtype=t.dtype, device=dev) if need else None for t, need in zip(tensors, ctx.needs_input_grad)]
+    b = BlockNormBackwardDesc(d, dn, ds, *[0 if g is None else g.data_ptr() for g in grads])
+    nbytes = lib.yolo_amd_block_norm_backward_workspace_bytes(b)
+    ws = _scratch(b, nbytes, tensors[0]) if nbytes else None     # noqa: F841
+    _call(tensors[0].get_device(), lib.yolo_amd_block_norm_backward, b, "block_norm backward")
+    return (*grads, None, None)
+
+
+_norm_backward_once = torch.autograd.function.once_differentiable(_norm_backward)
 
 
 class _BlockNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, residual, gate, after_weight, after_bias, before_weight, before_bias, conf, own_stream):
-        tensors = (x, residual, gate, after_weight, after_bias, before_weight, before_bias)
-        stream, normed = _norm_forward(*tensors, conf, own_stream)
+        out = _norm_forward(x, residual, gate, after_weight, after_bias, before_weight, before_bias, conf, own_stream)
         ctx.set_materialize_grads(False)
-        ctx.save_for_backward(*tensors)
+        ctx.save_for_backward(x, residual, gate, after_weight, after_bias, before_weight, before_bias)
         ctx.conf = conf
-        return stream, normed
+        return out
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dstream, dnormed):
-        tensors = ctx.saved_tensors
-        x = tensors[0]
-        dev = x.device
-        need = ctx.needs_input_grad
-        b = BlockNormBackwardDesc()
-        d, keep = _norm_desc(*tensors, ctx.conf)
-        b.forward = d
-        if dnormed is not None:
-            dnormed = dnormed.contiguous()
-            b.dnormed = dnormed.data_ptr()
-        if dstream is not None:
-            dstream = dstream.contiguous()
-            b.dstream = dstream.data_ptr()
-        grads = [None] * 7
-        for i, name in enumerate(("dx", "dresidual", "dgate", "dafter_weight", "dafter_bias", "dbefore_weight",
-                                  "dbefore_bias")):
-            if need[i]:
-                grads[i] = torch.empty(tensors[i].shape, dtype=tensors[i].dtype, device=dev)
-                setattr(b, name, grads[i].data_ptr())
-        ws = _scratch(b, lib.yolo_amd_block_norm_backward_workspace_bytes(_byref(b)), dev)     # noqa: F841
-        _call(dev, lib.yolo_amd_block_norm_backward, b, "block_norm backward")
-        return (*grads, None, None)
+        return (_norm_backward_once if torch.is_grad_enabled() else _norm_backward)(ctx, dstream, dnormed)
 
 
 def _gate_rows(x, gate):
@@ -302,6 +312,22 @@ def _gate_rows(x, gate):
         raise ValueError(f"block_norm: gate {tuple(gate.shape)} does not go with x {tuple(x.shape)}: one gate for all "
                          f"rows, for each row, or for each run of rows (a sequence) is taken")
     return max(1, shared if i else rows)
+
+
+def _check_norm(name, there, w, b, norm, x):
+    for kind, t in (("weight", w), ("bias", b)):
+        if t is None:
+            continue
+        if not there:
+            raise ValueError(f"block_norm: {name}_{kind} without the norm it belongs to")
+        if t.shape != x.shape[-1:] or (t.dtype is not x.dtype and t.dtype is not _F32):
+            raise ValueError(f"block_norm: {name}_{kind} must be ({x.shape[-1]},) of {x.dtype} or float32, got "
+                             f"{tuple(t.shape)} of {t.dtype}")
+    if b is not None:
+        if norm == "rms":
+            raise ValueError("block_norm: an rms norm has no bias")
+        if w is not None and w.dtype is not b.dtype:
+            raise ValueError(f"block_norm: {name}_weight is {w.dtype}, {name}_bias is {b.dtype}")
 
 
 def block_norm(x, residual=None, *, norm="rms", after=None, after_weight=None, after_bias=None, gate=None,
@@ -323,8 +349,8 @@ def block_norm(x, residual=None, *, norm="rms", after=None, after_weight=None, a
 
     Statistics are fp32; normed is taken from the stream before that is rounded.  The backward pass recomputes
     everything from x and residual (neither may be changed in place before it) and no statistics are kept."""
-    dev = _on_gpu("block_norm", x, residual=residual, gate=gate, after_weight=after_weight, after_bias=after_bias,
-                  before_weight=before_weight, before_bias=before_bias)
+    _on_gpu("block_norm", x=x, residual=residual, gate=gate, after_weight=after_weight, after_bias=after_bias,
+            before_weight=before_weight, before_bias=before_bias)
     dt = x.dtype
     if dt not in _TYPES:
         raise TypeError(f"block_norm: x must be float32, bfloat16 or float16, got {dt}")
@@ -334,19 +360,8 @@ def block_norm(x, residual=None, *, norm="rms", after=None, after_weight=None, a
         raise ValueError(f"block_norm: unknown norm {norm!r}")
     if after is None:
         after = after_weight is not None or after_bias is not None
-    for name, flag, w, b in (("after", after, after_weight, after_bias), ("before", before, before_weight, before_bias)):
-        for kind, t in (("weight", w), ("bias", b)):
-            if t is None:
-                continue
-            if not flag:
-                raise ValueError(f"block_norm: {name}_{kind} without the norm it belongs to")
-            if t.shape != x.shape[-1:] or t.dtype not in (dt, _F32):
-                raise ValueError(f"block_norm: {name}_{kind} must be ({x.shape[-1]},) of {dt} or float32, got "
-                                 f"{tuple(t.shape)} of {t.dtype}")
-        if b is not None and norm == "rms":
-            raise ValueError("block_norm: an rms norm has no bias")
-        if w is not None and b is not None and w.dtype != b.dtype:
-            raise ValueError(f"block_norm: {name}_weight is {w.dtype}, {name}_bias is {b.dtype}")
+    _check_norm("after", after, after_weight, after_bias, norm, x)
+    _check_norm("before", before, before_weight, before_bias, norm, x)
     if residual is not None and (residual.shape != x.shape or residual.dtype not in (dt, _F32)):
         raise ValueError(f"block_norm: residual must be {tuple(x.shape)} of {dt} or float32, got {tuple(residual.shape)} "
                          f"of {residual.dtype}")
