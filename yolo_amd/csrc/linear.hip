@@ -754,7 +754,9 @@ linear_finish_kernel(const Epilogue e, const float* part, int slices, int M, int
 // ---------------------------------------------------------------- few rows
 // M <= 16 * MT rows of x: the product is a read of W.  A workgroup owns 16 * NT rows of W (columns of Y) and
 // its eight waves take 64 reduction indices each in turn, straight from memory into matrix-instruction fragments;
-// the eight partial sums meet in LDS in a fixed order.  No second launch, no atomics.
+// the eight partial sums meet in LDS in a fixed order.  Every workgroup reads all of x (from L2): more rows of W per
+// workgroup save that, fewer fill the chip (one row, N 16384, K 4096: NT 1 25.5 us, 5.3 TB/s; sixteen rows: NT 1 40.6,
+// NT 4 32.2).  Where even 16 columns each leave CUs without a workgroup, K is cut into slices (blockIdx.y).
 // U steps' loads are issued before the first product: what bounds this kernel is how much of W is on its way.
 template <typename T, int MT, int NT, int U>
 __global__ void __launch_bounds__(512)
@@ -775,16 +777,17 @@ linear_rows_kernel(const TileArgs a) {
     for (int i = 0; i < MT; ++i)
 #pragma unroll
         for (int j = 0; j < NT; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-    for (int k = w * 64; k < a.K; k += 512 * U) {
+    const int k1 = min(a.K, ((int)blockIdx.y + 1) * a.ksteps * kBK);
+    for (int k = (int)blockIdx.y * a.ksteps * kBK + w * 64; k < k1; k += 512 * U) {
         v8<T> xv[U][2][MT], wv[U][2][NT];
         bool in[U][2];
 #pragma unroll
         for (int u = 0; u < U; ++u)
 #pragma unroll
             for (int s = 0; s < 2; ++s) {
-                // past K (whole chunks: K is a multiple of 8): the row's start, taken as zeros below
+                // past the slice (whole chunks: K is a multiple of 8): the row's start, taken as zeros below
                 const int at = k + u * 512 + s * 32 + kl;
-                in[u][s] = at < a.K;
+                in[u][s] = at < k1;
                 const int from = in[u][s] ? at : 0;
 #pragma unroll
                 for (int j = 0; j < NT; ++j) wv[u][s][j] = *reinterpret_cast<const v8<T>*>(wp[j] + from);
@@ -827,7 +830,8 @@ linear_rows_kernel(const TileArgs a) {
             float v[8];
 #pragma unroll
             for (int i = 0; i < 4; ++i) { v[i] = lo[i]; v[4 + i] = hi[i]; }
-            finish8<T>(a.e, mr, n, a.N, v);
+            if (a.e.part) store8<T>(a.e.part, blockIdx.y * a.e.slice_stride + mr * a.e.ld_part + n, 1, v);
+            else finish8<T>(a.e, mr, n, a.N, v);
         }
     }
 }
@@ -977,18 +981,32 @@ static const TileConfig kTileConfigs[] = {
 static TilePlan plan_product(long long M, int N, long long K, bool kc_operands, int act) {
     TilePlan p{};
     const long long steps = std::max<long long>(1, (K + kBK - 1) / kBK);
-    if (kc_operands && M <= 32) {
-        p.kernel = YOLO_AMD_LINEAR_ROWS;
-        p.bm = M <= 16 ? 16 : 32;
-        p.bn = N >= 16384 ? 32 : 16;
-        p.slices = 1;
-        p.ksteps = (int)steps;
-        return p;
-    }
     // An activation's instructions lengthen an epilogue that nothing overlaps (256: 12 us a round for erf, 4.5 for the two
     // with an exponential and a reciprocal) more than one that another workgroup's products run beside (128: 2.3 and 1).
     const double slow = act == YOLO_AMD_ACT_GELU ? 1.0 : act == YOLO_AMD_ACT_GELU_TANH || act == YOLO_AMD_ACT_SILU ? 0.4 : 0.0;
     double best = 0;
+    // Few rows: one workgroup streams 22.5 bytes a nanosecond, many 6000 (80 of them half as fast); x from L2 costs two
+    // thirds of a byte of W.  K is cut only where sixteen columns to a workgroup leave CUs without one.
+    for (int nt = 1; kc_operands && M <= 32 && nt <= 4; nt *= 2) {
+        const long long wgs = (N + 16 * nt - 1) / (16 * nt);
+        for (int s = 1; s <= 16 && s * 8 <= steps + 7; s *= 2) {
+            const long long per = (steps + s - 1) / s;
+            if ((steps + per - 1) / per != s) continue;
+            if (s > 1 && (nt > 1 || wgs * s > 512)) break;
+            const double w = (double)wgs * s, rate = std::min(22.5 * w, 6000.0 * w / (w + 80.0));
+            double t = 1.8 + 2.0 * K * (N + 0.65 * wgs * M) * 1e-3 / rate;
+            if (s > 1) t += 3.4 + 0.08 * s + (double)s * M * N * 2e-6;
+            if (p.kernel == 0 || t < best) {
+                best = t;
+                p.kernel = YOLO_AMD_LINEAR_ROWS;
+                p.bm = M <= 16 ? 16 : 32;
+                p.bn = 16 * nt;
+                p.ahead = 0;
+                p.slices = s;
+                p.ksteps = (int)per;
+            }
+        }
+    }
     for (const TileConfig& c : kTileConfigs) {
         const long long tiles = ((M + c.b - 1) / c.b) * ((N + c.b - 1) / c.b);
         const int slots = 256 * tile_occupancy(c.b, c.ahead);
@@ -999,6 +1017,7 @@ static TilePlan plan_product(long long M, int N, long long K, bool kc_operands, 
             double t = (double)(wgs / slots) * (c.start + per * c.step);
             if (s == 1) t += (double)((wgs + slots - 1) / slots) * slow * (c.b == 256 ? 12.0 : c.b == 128 ? 2.5 : 0.7);
             if (rest > 0) t += rest <= 256 ? c.start_1 + per * c.step_1 : c.start + per * c.step;
+            t = std::max(t, 2.0 + 2.0 * ((double)M * K + (double)N * K + (double)M * N) * 2e-7);   // at 5 TB/s
             if (s > 1) t += 3.4 + 0.08 * s + (double)s * M * N * 2e-6;     // one more launch; partial sums out and in at 4 TB/s
             if (p.kernel == 0 || t < best) {
                 best = t;
@@ -1051,26 +1070,6 @@ static void launch_pack(Matrix (&m)[2], const size_t (&bytes)[2], Scratch& sc, h
 
 template <typename T, bool AT, bool BT>
 static int launch_product(const TilePlan& p, TileArgs a, void* partial, hipStream_t s) {
-    if (p.kernel == YOLO_AMD_LINEAR_ROWS) {
-        if constexpr (!AT && !BT) {
-            const dim3 grid((a.N + p.bn - 1) / p.bn);
-            const bool deep = a.K > 1024;              // four steps of 512 in flight
-#define YA_ROWS(MT, NT)                                                                                              \
-    do {                                                                                                             \
-        if (deep) hipLaunchKernelGGL((linear_rows_kernel<T, MT, NT, 4>), grid, dim3(512), 0, s, a);                  \
-        else hipLaunchKernelGGL((linear_rows_kernel<T, MT, NT, 2>), grid, dim3(512), 0, s, a);                       \
-    } while (0)
-            if (p.bm == 16 && p.bn == 16) YA_ROWS(1, 1);
-            else if (p.bm == 16) YA_ROWS(1, 2);
-            else if (p.bn == 16) YA_ROWS(2, 1);
-            else YA_ROWS(2, 2);
-#undef YA_ROWS
-        }
-        YA_CHECK_HIP(hipGetLastError());
-        return YA_OK;
-    }
-    a.tiles_m = (a.M + p.bm - 1) / p.bm;
-    a.tiles_n = (a.N + p.bn - 1) / p.bn;
     a.ksteps = p.ksteps;
     const Epilogue e = a.e;
     if (p.slices > 1) {
@@ -1079,11 +1078,32 @@ static int launch_product(const TilePlan& p, TileArgs a, void* partial, hipStrea
         a.e.ld_part = (long long)align_up(a.N, 8);
         a.e.slice_stride = a.e.ld_part * a.M;
     }
+    const int kernel = p.kernel == YOLO_AMD_LINEAR_ROWS ? 0 : p.bm * 10 + p.ahead;
+    if (kernel == 0) {
+        if constexpr (!AT && !BT) {
+            const dim3 grid((a.N + p.bn - 1) / p.bn, p.slices);
+            const bool deep = p.ksteps > 16;           // four steps of 512 in flight
+#define YA_ROWS(MT, NT)                                                                                              \
+    do {                                                                                                             \
+        if (deep) hipLaunchKernelGGL((linear_rows_kernel<T, MT, NT, 4>), grid, dim3(512), 0, s, a);                  \
+        else hipLaunchKernelGGL((linear_rows_kernel<T, MT, NT, 2>), grid, dim3(512), 0, s, a);                       \
+    } while (0)
+            if (p.bm == 16 && p.bn == 16) YA_ROWS(1, 1);
+            else if (p.bm == 16 && p.bn == 32) YA_ROWS(1, 2);
+            else if (p.bm == 16) YA_ROWS(1, 4);
+            else if (p.bn == 16) YA_ROWS(2, 1);
+            else if (p.bn == 32) YA_ROWS(2, 2);
+            else YA_ROWS(2, 4);
+#undef YA_ROWS
+        }
+    }
+    a.tiles_m = (a.M + p.bm - 1) / p.bm;
+    a.tiles_n = (a.N + p.bn - 1) / p.bn;
     const dim3 grid((unsigned)((long long)a.tiles_m * a.tiles_n), (unsigned)p.slices);
-    if (p.bm == 256) hipLaunchKernelGGL((linear_tile_kernel<T, 256, 256, 2, AT, BT>), grid, dim3(256), 0, s, a);
-    else if (p.bm == 128 && p.ahead == 2) hipLaunchKernelGGL((linear_tile_kernel<T, 128, 128, 2, AT, BT>), grid, dim3(256), 0, s, a);
-    else if (p.bm == 128) hipLaunchKernelGGL((linear_tile_kernel<T, 128, 128, 4, AT, BT>), grid, dim3(256), 0, s, a);
-    else hipLaunchKernelGGL((linear_tile_kernel<T, 64, 64, 4, AT, BT>), grid, dim3(256), 0, s, a);
+    if (kernel == 2562) hipLaunchKernelGGL((linear_tile_kernel<T, 256, 256, 2, AT, BT>), grid, dim3(256), 0, s, a);
+    else if (kernel == 1282) hipLaunchKernelGGL((linear_tile_kernel<T, 128, 128, 2, AT, BT>), grid, dim3(256), 0, s, a);
+    else if (kernel == 1284) hipLaunchKernelGGL((linear_tile_kernel<T, 128, 128, 4, AT, BT>), grid, dim3(256), 0, s, a);
+    else if (kernel == 644) hipLaunchKernelGGL((linear_tile_kernel<T, 64, 64, 4, AT, BT>), grid, dim3(256), 0, s, a);
     if (p.slices > 1) {
         Epilogue f = e;
         f.ld_part = a.e.ld_part;
