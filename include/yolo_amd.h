@@ -327,7 +327,8 @@ int yolo_amd_conv_forward(const yolo_amd_conv_desc* descs, int n, const void* ze
  * fp32 where their flag says so.  Row strides (ld*) are in elements and at least the row's length; any
  * alignment to the element is accepted (rows that start on 16-byte boundaries with k a multiple of 8 are
  * read in place, others are copied into the workspace by the call).  Sums are fp32, in an order that
- * depends on the sizes only; y is rounded once.  m == 0 and n == 0 do nothing; k == 0 sums nothing. */
+ * depends on the sizes only; y is rounded once.  m == 0 and n == 0 do nothing; k == 0 sums nothing.
+ * m up to 2^30, n and k below 2^22; strides of 2^22 and more make a copy as well. */
 #define YOLO_AMD_TYPE_F32 0
 #define YOLO_AMD_TYPE_BF16 1
 #define YOLO_AMD_TYPE_F16 2
@@ -413,7 +414,7 @@ int yolo_amd_linear_backward(const yolo_amd_linear_backward_desc* desc, void* st
  * i / rows_per_gate of it (1: a gate for each row; the rows of a sequence: one for each sequence; >= rows:
  * one for all).  Weights and biases are of `type` or fp32, one flag per norm.  NULL stands for: no residual
  * (0), no gate (1), no weight (1), no bias (0).  Statistics are fp32; stream is rounded once, and normed is
- * taken from the unrounded stream.  Rows are independent of each other; 1 <= d <= 16384. */
+ * taken from the unrounded stream.  Rows are independent of each other; fewer than 2^31 rows, 1 <= d <= 16384. */
 #define YOLO_AMD_NORM_RMS 0
 #define YOLO_AMD_NORM_LAYER 1
 

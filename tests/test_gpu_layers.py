@@ -110,6 +110,45 @@ def test_linear_reads_views_and_nothing_beyond_them(m):
     assert y.shape == (4, 2, 5, 24)
 
 
+def test_linear_last_token_is_read_in_place():
+    """x[:, -1:] of a (batch, tokens, channels) tensor is rows at one stride: no copy."""
+    from yolo_amd.layers import _rows, linear
+    g = _gen(91)
+    x, w = _rand(g, 6, 50, 64, dtype=BF16), _rand(g, 40, 64, dtype=BF16)
+    for view in (x[:, -1:], x[:, 7], x[2:3, :, :], x[:, -1:].transpose(0, 1), x[::2, 3:4]):
+        assert _rows(view)[0].data_ptr() == view.data_ptr()
+        want, bound, _, _ = ref.linear_ref(view.reshape(-1, 64), w, None, None, None, BF16)
+        assert_within(linear(view, w).reshape(-1, 40), want, bound, str(tuple(view.shape)))
+    far = torch.empty(20, 1 << 23, dtype=BF16, device="cuda")[:, 5:69]        # rows 16 MiB apart
+    far.copy_(_rand(g, 20, 64))
+    for rows in (far, far[:1]):
+        want, bound, _, _ = ref.linear_ref(rows, w, None, None, None, BF16)
+        assert_within(linear(rows, w), want, bound, "far apart")
+    odd = x[:, :3]                                           # three of fifty tokens each: copied
+    want, bound, _, _ = ref.linear_ref(odd.reshape(-1, 64), w, None, None, None, BF16)
+    assert_within(linear(odd, w).reshape(-1, 40), want, bound, "copied")
+
+
+@pytest.mark.parametrize("m,n,k", [(3, 40, 64), (200, 41, 72), (64, 520, 8192), (300, 1000, 100)])
+def test_linear_residual_in_place(m, n, k):
+    """At the C entry y may be the residual itself."""
+    import ctypes
+    from yolo_amd import _lib
+    from yolo_amd._lib import lib
+    g = _gen(92)
+    x, w, r = _rand(g, m, k, dtype=BF16), _rand(g, n, k, scale=k ** -0.5, dtype=BF16), _rand(g, m, n, dtype=BF16)
+    y = r.clone()
+    d = _lib.LinearDesc()
+    d.x, d.weight, d.residual, d.y = x.data_ptr(), w.data_ptr(), y.data_ptr(), y.data_ptr()
+    d.m, d.n, d.k, d.ldx, d.ldw, d.ldr, d.ldy, d.type = m, n, k, k, k, n, n, _lib.TYPE_BF16
+    need = lib.yolo_amd_linear_workspace_bytes(ctypes.byref(d))
+    ws = torch.empty(max(need, 1), dtype=torch.uint8, device="cuda")
+    d.workspace, d.workspace_bytes = ws.data_ptr(), need
+    _lib.check(lib.yolo_amd_linear_forward(ctypes.byref(d), _lib.current_stream_ptr()), "linear")
+    want, bound, _, _ = ref.linear_ref(x, w, None, r, None, BF16)
+    assert_within(y, want, bound, "in place")
+
+
 @pytest.mark.parametrize("m", [4, 150])
 def test_linear_nan_and_inf_stay_in_their_row(m):
     from yolo_amd.layers import linear
@@ -164,10 +203,10 @@ def test_linear_offsets_past_32_bits():
 def _band_check(x, w, b, r, y, act, dtype):
     """A band of rows and a band of columns of y, both with the ragged edge: the 64-bit product of all is slow here."""
     m, n = y.shape
-    rows = torch.cat([torch.arange(0, 40), torch.arange(max(0, m - 300), m)]).cuda()
+    rows = torch.cat([torch.arange(0, min(m, 40)), torch.arange(max(0, m - 300), m)]).cuda()
     want, bound, _, _ = ref.linear_ref(x[rows], w, b, r[rows], act, dtype)
     assert_within(y[rows], want, bound, "rows")
-    cols = torch.cat([torch.arange(0, 40), torch.arange(max(0, n - 300), n)]).cuda()
+    cols = torch.cat([torch.arange(0, min(n, 40)), torch.arange(max(0, n - 300), n)]).cuda()
     want, bound, _, _ = ref.linear_ref(x, w[cols], b[cols], r[:, cols], act, dtype)
     assert_within(y[:, cols], want, bound, "columns")
 
@@ -191,6 +230,27 @@ def test_linear_tiles(shape, bm, slices, ahead, dtype):
     c = _choice(x, w)[1]
     assert (c.bm, c.k_slices > 1, c.steps_ahead) == (bm, slices > 1, ahead)
     _band_check(x, w, b, r, linear(x, w, b, activation="gelu_tanh", residual=r), "gelu_tanh", dtype)
+
+
+# (m, n, k), rows and columns of y per workgroup, and whether K is split
+ROWS = [((1, 307, 40), 16, 16, False), ((11, 130, 2152), 16, 16, False), ((5, 114, 4680), 16, 16, True),
+        ((7, 41, 11753), 16, 16, True), ((9, 15112, 72), 16, 32, False), ((7, 9080, 2544), 16, 32, False),
+        ((13, 19760, 64), 16, 64, False), ((31, 132, 72), 32, 16, False),
+        ((19, 64, 1056), 32, 16, False), ((20, 24, 3400), 32, 16, True), ((21, 16, 8216), 32, 16, True),
+        ((27, 5850, 72), 32, 32, False), ((31, 4912, 1056), 32, 32, False), ((25, 20003, 136), 32, 64, False)]
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("shape,bm,bn,split", ROWS)
+def test_linear_few_rows(shape, bm, bn, split, dtype):
+    from yolo_amd.layers import linear
+    m, n, k = shape
+    g = _gen(m + n + k)
+    x, w, b = _rand(g, m, k, dtype=dtype), _rand(g, n, k, scale=k ** -0.5, dtype=dtype), _rand(g, n, dtype=dtype)
+    r = _rand(g, m, n, dtype=dtype)
+    name, c = _choice(x, w)
+    assert (name, c.bm, c.bn, c.k_slices > 1) == ("rows", bm, bn, split)
+    _band_check(x, w, b, r, linear(x, w, b, activation="silu", residual=r), "silu", dtype)
 
 
 # ------------------------------------------------------------------ linear, backward
@@ -222,7 +282,7 @@ def test_linear_backward(m, n, k, dtype):
 
 
 @pytest.mark.parametrize("dtype", [BF16, F16])
-@pytest.mark.parametrize("m,n,k", [(4096, 2048, 4096), (4100, 2056, 4104), (2048, 2048, 2048), (4100, 1032, 2056)])
+@pytest.mark.parametrize("m,n,k", [(4096, 2048, 4096), (4100, 2056, 4104), (2048, 2048, 2048), (4100, 1032, 2056), (2048, 4096, 4096), (2060, 264, 4104)])
 def test_linear_backward_large(m, n, k, dtype):
     """The products of the backward pass on the larger tiles: bands of dx and dweight."""
     from yolo_amd.layers import linear
@@ -256,6 +316,28 @@ def test_linear_backward_one_gradient_at_a_time():
             full = got
         for a, c in zip(got, full):
             assert a is None or torch.equal(a, c)
+
+
+def test_linear_padding_is_not_written():
+    """Rows behind the last one and columns behind the row's end keep what they held (a strided y at the C entry)."""
+    import ctypes
+    from yolo_amd import _lib
+    from yolo_amd._lib import lib
+    g = _gen(93)
+    for m, n, k, ld in ((3, 40, 64, 48), (70, 41, 64, 50), (300, 250, 72, 251), (40, 24, 4680, 33)):
+        for f32 in (0, 1):
+            x, w = _rand(g, m, k, dtype=BF16), _rand(g, n, k, scale=k ** -0.5, dtype=BF16)
+            y = torch.full((m + 2, ld), 7.0, dtype=F32 if f32 else BF16, device="cuda")
+            d = _lib.LinearDesc()
+            d.x, d.weight, d.y = x.data_ptr(), w.data_ptr(), y.data_ptr()
+            d.m, d.n, d.k, d.ldx, d.ldw, d.ldy, d.type, d.y_f32 = m, n, k, k, k, ld, _lib.TYPE_BF16, f32
+            need = lib.yolo_amd_linear_workspace_bytes(ctypes.byref(d))
+            ws = torch.empty(max(need, 1), dtype=torch.uint8, device="cuda")
+            d.workspace, d.workspace_bytes = ws.data_ptr(), need
+            _lib.check(lib.yolo_amd_linear_forward(ctypes.byref(d), _lib.current_stream_ptr()), "linear")
+            want, bound, _, _ = ref.linear_ref(x, w, None, None, None, y.dtype)
+            assert_within(y[:m, :n], want, bound, "inside")
+            assert (y[m:] == 7).all() and (y[:m, n:] == 7).all()
 
 
 def test_linear_backward_views():
@@ -592,7 +674,8 @@ def test_layers_refuse_on_the_gpu():
     z = lambda *s, t=BF16: torch.zeros(*s, dtype=t, device="cuda")     # noqa: E731
     x, w = z(4, 16), z(8, 16)
     for bad in (lambda: linear(z(4, 16, t=F32), z(8, 16, t=F32)), lambda: linear(x, z(8, 16, t=F16)),
-                lambda: linear(x, w, out_dtype=F16), lambda: block_norm(x.long()), lambda: block_norm(x, gate=z(16, t=F16))):
+                lambda: linear(x, w, out_dtype=F16), lambda: block_norm(x.long()), lambda: block_norm(x, gate=z(16, t=F16)),
+                lambda: block_norm(x, residual_scale=z(1)), lambda: block_norm(x, eps=z(1))):
         with pytest.raises(TypeError):
             bad()
     for bad in (lambda: linear(x, z(8, 15)), lambda: linear(x, z(16)), lambda: linear(x, w, z(7)), lambda: linear(x, w, z(8, t=F16)),

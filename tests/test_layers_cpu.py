@@ -72,7 +72,7 @@ def test_codes_match_the_header():
     (dict(type=0), "type"), (dict(type=3), "type"), (dict(activation=6), "activation"), (dict(activation=-1), "activation"),
     (dict(m=-1), "m="), (dict(k=1 << 22, ldx=1 << 22, ldw=1 << 22), "k="), (dict(n=1 << 22, ldy=1 << 22), "n="),
     (dict(m=1 << 31), "m="), (dict(x=None), "x is null"), (dict(weight=None), "weight is null"), (dict(y=None), "y is null"),
-    (dict(ldx=15), "row stride"), (dict(ldw=0), "row stride"), (dict(ldy=7), "row stride"), (dict(ldx=1 << 23), "row stride"),
+    (dict(ldx=15), "row stride"), (dict(ldw=0), "row stride"), (dict(ldy=7), "row stride"),
     (dict(residual=0x40000, ldr=4), "residual"), (dict(x=0x10001), "aligned"), (dict(y=0x30002, y_f32=1), "aligned"),
     (dict(bias=0x40002, bias_f32=1), "bias"),
 ])
@@ -120,6 +120,8 @@ def test_linear_dispatch():
     assert (c.copies_x, c.copies_weight) == (1, 0)
     c = _query(_linear_desc(1, 60, 64, ldx=65))[1]          # one row has no stride
     assert (c.copies_x, c.copies_weight) == (0, 0)
+    c = _query(_linear_desc(300, 60, 64, ldx=1 << 23))[1]   # the last token of long sequences
+    assert (c.copies_x, c.copies_weight) == (1, 0)
     c = _query(_linear_desc(300, 60, 64, weight=0x20002))[1]
     assert (c.copies_x, c.copies_weight) == (0, 1)
     assert _query(_linear_desc(0, 8, 16, x=None, y=None))[0] == 0
@@ -200,6 +202,16 @@ def test_reference_bounds_catch_planted_mistakes():
     unbiased = (v - v.mean(-1, keepdim=True)) / v.std(-1, keepdim=True)
     with pytest.raises(AssertionError):
         ref.assert_within(unbiased, out[0], ref.rounded(*out, torch.float32), "wrong")
+
+
+def test_rows_of_views():
+    from yolo_amd.layers import _rows
+    t = torch.zeros(4, 6, 8)
+    assert _rows(t)[1] == 8 and _rows(t[:, -1:])[1] == 48 and _rows(t[:, 2])[1] == 48 and _rows(t[..., :5])[1] == 8
+    assert _rows(t[0])[1] == 8 and _rows(t[1:2, ::2])[1] == 16 and _rows(t[:, :, ::2])[1] == 4 and _rows(t[:, :2])[1] == 8
+    assert _rows(t[:, :2])[0].is_contiguous() and _rows(t[:1].expand(4, 6, 8))[0].is_contiguous()
+    assert _rows(t[0, 0].expand(3, 8))[1] == 8 and _rows(t[0, 0, ::2])[0].is_contiguous()
+    assert _rows(t[..., :1])[1] == 8 and _rows(t.transpose(0, 1))[0].is_contiguous()
 
 
 def test_gate_rows():

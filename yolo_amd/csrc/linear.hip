@@ -755,8 +755,8 @@ linear_finish_kernel(const Epilogue e, const float* part, int slices, int M, int
 // M <= 16 * MT rows of x: the product is a read of W.  A workgroup owns 16 * NT rows of W (columns of Y) and
 // its eight waves take 64 reduction indices each in turn, straight from memory into matrix-instruction fragments;
 // the eight partial sums meet in LDS in a fixed order.  Every workgroup reads all of x (from L2): more rows of W per
-// workgroup save that, fewer fill the chip (one row, N 16384, K 4096: NT 1 25.5 us, 5.3 TB/s; sixteen rows: NT 1 40.6,
-// NT 4 32.2).  Where even 16 columns each leave CUs without a workgroup, K is cut into slices (blockIdx.y).
+// workgroup save that, fewer fill the chip (one row, N 16384, K 4096: NT 1 25.5 us, 5.3 TB/s, NT 2 30.2; sixteen rows:
+// NT 1 40.6, NT 2 36.7, and the 64-wide tile 33.4).  Where even 16 columns each leave CUs without a workgroup, K is cut into slices (blockIdx.y).
 // U steps' loads are issued before the first product: what bounds this kernel is how much of W is on its way.
 template <typename T, int MT, int NT, int U>
 __global__ void __launch_bounds__(512)
@@ -948,8 +948,12 @@ struct Matrix {
     int cols;
 };
 
+// Tiles address their rows with 32-bit byte offsets: 256 rows of this many elements.
+constexpr long long kMaxLd = (1ll << 22) - 1, kMaxRows = 1ll << 30;
+
+// can be read in place: whole 16-byte chunks, no row's last one reaching into the next
 static bool packed_ok(const Matrix& m) {
-    return ((uintptr_t)m.p & 15) == 0 && m.cols % 8 == 0 && (m.ld % 8 == 0 || m.rows <= 1);
+    return ((uintptr_t)m.p & 15) == 0 && m.cols % 8 == 0 && ((m.ld % 8 == 0 && m.ld <= kMaxLd) || m.rows <= 1);
 }
 static size_t packed_bytes(const Matrix& m) {
     return packed_ok(m) ? 0 : align_up((size_t)m.rows * align_up(m.cols, 8) * 2, 256);
@@ -1090,16 +1094,18 @@ static int launch_product(const TilePlan& p, TileArgs a, void* partial, hipStrea
     } while (0)
             if (p.bm == 16 && p.bn == 16) YA_ROWS(1, 1);
             else if (p.bm == 16 && p.bn == 32) YA_ROWS(1, 2);
-            else if (p.bm == 16) YA_ROWS(1, 4);
+            else if (p.bm == 16) hipLaunchKernelGGL((linear_rows_kernel<T, 1, 4, 2>), grid, dim3(512), 0, s, a);
             else if (p.bn == 16) YA_ROWS(2, 1);
             else if (p.bn == 32) YA_ROWS(2, 2);
-            else YA_ROWS(2, 4);
+            else hipLaunchKernelGGL((linear_rows_kernel<T, 2, 4, 2>), grid, dim3(512), 0, s, a);
 #undef YA_ROWS
         }
     }
     a.tiles_m = (a.M + p.bm - 1) / p.bm;
     a.tiles_n = (a.N + p.bn - 1) / p.bn;
-    const dim3 grid((unsigned)((long long)a.tiles_m * a.tiles_n), (unsigned)p.slices);
+    const long long tiles = (long long)a.tiles_m * a.tiles_n;
+    YA_REQUIRE(kernel == 0 || tiles < 1 << 24, "linear: %d x %d takes %lld tiles, more than a launch holds", a.M, a.N, tiles);
+    const dim3 grid((unsigned)tiles, (unsigned)p.slices);
     if (kernel == 2562) hipLaunchKernelGGL((linear_tile_kernel<T, 256, 256, 2, AT, BT>), grid, dim3(256), 0, s, a);
     else if (kernel == 1282) hipLaunchKernelGGL((linear_tile_kernel<T, 128, 128, 2, AT, BT>), grid, dim3(256), 0, s, a);
     else if (kernel == 1284) hipLaunchKernelGGL((linear_tile_kernel<T, 128, 128, 4, AT, BT>), grid, dim3(256), 0, s, a);
@@ -1115,7 +1121,6 @@ static int launch_product(const TilePlan& p, TileArgs a, void* partial, hipStrea
     return YA_OK;
 }
 
-constexpr long long kMaxLd = (1ll << 22) - 1, kMaxRows = (1ll << 31) - 1024;
 
 static int check_common(const char* what, int64_t m, int64_t n, int64_t k, int type, int act) {
     YA_REQUIRE(m >= 0 && n >= 0 && k >= 0 && m <= kMaxRows && n <= kMaxLd && k <= kMaxLd,
@@ -1130,8 +1135,7 @@ static int check_matrix(const char* what, const char* name, const void* p, long 
     if (rows == 0 || cols == 0) return YA_OK;
     YA_REQUIRE(p, "%s: %s is null", what, name);
     YA_REQUIRE(((uintptr_t)p & (esize - 1)) == 0, "%s: %s is not aligned to its elements", what, name);
-    YA_REQUIRE(rows <= 1 || (ld >= cols && ld <= kMaxLd), "%s: %s has row stride %lld for %d columns (at most %lld)", what, name, ld,
-               cols, kMaxLd);
+    YA_REQUIRE(rows <= 1 || ld >= cols, "%s: %s has row stride %lld for %d columns", what, name, ld, cols);
     return YA_OK;
 }
 static int check_forward(const yolo_amd_linear_desc* d) {

@@ -9,7 +9,8 @@ before a block fused with the block's gate, residual scale and residual add.
 
 Both are differentiable in every tensor argument (once; a second derivative raises), take inputs on any GPU and
 run on torch's current stream of that GPU.  They allocate outputs and scratch with torch's allocator, so they
-can be captured into a HIP graph, keep nothing between calls and never synchronise.  Results depend on the
+can be captured into a HIP graph, keep nothing between calls and never synchronise.  (As anywhere in torch, a
+backward pass is captured only while no eager graph of the same leaves is alive.)  Results depend on the
 inputs alone: every sum has a fixed order.  Row views (``x[:, :k]``) are read in place; other strides are copied.
 There is no CPU implementation: tensors on the CPU raise YoloAmdError.
 
@@ -61,13 +62,20 @@ def _rows(t):
     shape = t.shape
     if t.is_contiguous():
         return t, shape[-1]
-    if t.dim() >= 2 and t.stride(-1) == 1 and t.stride(-2) >= shape[-1]:
-        step = t.stride(-2)
-        for i in range(t.dim() - 3, -1, -1):
-            if shape[i] != 1 and t.stride(i) != t.stride(i + 1) * shape[i + 1]:
+    if shape[-1] == 1 or t.stride(-1) == 1:
+        step = rows = 0                              # dimensions of size 1 have no stride to speak of
+        for i in range(t.dim() - 2, -1, -1):
+            if shape[i] == 1:
+                continue
+            if rows == 0:
+                step = t.stride(i)
+                rows = 1
+            elif t.stride(i) != step * rows:
                 break
+            rows *= shape[i]
         else:
-            return t, step
+            if step >= shape[-1]:
+                return t, step
     t = t.contiguous()
     return t, shape[-1]
 
@@ -367,6 +375,9 @@ def block_norm(x, residual=None, *, norm="rms", after=None, after_weight=None, a
                          f"of {residual.dtype}")
     if gate is not None and gate.dtype not in (dt, _F32):
         raise TypeError(f"block_norm: gate must be {dt} or float32, got {gate.dtype}")
+    if torch.is_tensor(residual_scale) or torch.is_tensor(eps):
+        raise TypeError("block_norm: residual_scale and eps are numbers (reading one from a tensor would wait for the GPU); a "
+                        "learned scale goes in as the gate")
     rows_per_gate = _gate_rows(x, gate) if gate is not None else 1
     scale = float(residual_scale)
     conf = (_lib.NORM_CODES[norm], bool(after), bool(before), scale, float(eps), rows_per_gate)
