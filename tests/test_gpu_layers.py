@@ -162,6 +162,26 @@ def test_linear_nan_and_inf_stay_in_their_row(m):
     assert torch.equal(y[keep], clean[keep])
 
 
+@pytest.mark.parametrize("act", ["leaky", "relu", "gelu", "gelu_tanh", "silu"])
+def test_linear_slopes_past_the_type(act):
+    """Pre-activations beyond fp16's range, with an fp32 result: kept as infinities, where every slope has its limit."""
+    from yolo_amd.layers import linear
+    x = torch.full((3, 8), 200.0, dtype=F16, device="cuda")
+    w = torch.stack([torch.full((8,), 200.0), torch.full((8,), -200.0), torch.full((8,), 100.0)]).to(F16).cuda()
+    w[2, :4] *= -1                                          # 320000, -320000, 0
+    b = torch.zeros(3, device="cuda")
+    leaves = [t.requires_grad_() for t in (x, w, b)]
+    y = linear(x, w, b, activation=act, out_dtype=F32)
+    dx, dw, db = torch.autograd.grad(y, leaves, torch.ones_like(y))
+    low, zero = (0.1, 0.1) if act == "leaky" else (0.0, 0.0 if act == "relu" else 0.5)
+    # rows of three: sums of at most three roundings of a slope to fp16
+    want = torch.tensor([1.0, low, zero], device="cuda")
+    torch.testing.assert_close(db, 3 * want, rtol=2.0 ** -22, atol=2.0 ** -22)
+    torch.testing.assert_close(dw.float(), 3 * 200 * want.to(F16).float()[:, None].expand(3, 8), rtol=2.0 ** -10, atol=1e-6)
+    assert torch.isfinite(dx).all()
+    assert torch.equal(y[:, 0].detach(), torch.full((3,), 320000.0, device="cuda"))
+
+
 def test_linear_empty():
     from yolo_amd.layers import linear
     g = _gen(11)

@@ -138,10 +138,13 @@ __device__ __forceinline__ float act_value(float p, int act) {
     }
 }
 
+// act'(p).  From 100 on the curved ones have slope 1 and below -100 slope 0 in fp32: p is held there, so that no product
+// of an infinity (a pre-activation past fp16's range is kept as one) and a zero arises.  NaN stays NaN.
 template <int ACT>
 __device__ __forceinline__ float act_slope(float p) {
     if constexpr (ACT == YOLO_AMD_ACT_LEAKY) return p > 0.f ? 1.f : 0.1f;
     if constexpr (ACT == YOLO_AMD_ACT_RELU) return p > 0.f ? 1.f : 0.f;
+    if constexpr (ACT != YOLO_AMD_ACT_NONE) p = fabsf(p) > 100.f ? copysignf(100.f, p) : p;
     if constexpr (ACT == YOLO_AMD_ACT_GELU) {
         float e;
         const float q = 0.5f * erfc_scaled(p, e);
