@@ -549,6 +549,19 @@ def test_block_norm_empty():
     assert dx.shape == (0, 32) and not dw.any()
 
 
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_block_norm_empty_gate_gradient(dtype):
+    """No rows at all: the gradient of a gate that outlives them (one row, one for each sequence) is zero."""
+    from yolo_amd.layers import block_norm
+    for shape, gate_shape in (((0, 32), (32,)), ((4, 0, 32), (32,)), ((4, 0, 32), (4, 1, 32)), ((0, 7, 32), (0, 1, 32))):
+        x = torch.empty(shape, dtype=dtype, device="cuda")
+        gate = torch.full(gate_shape, 2.0, dtype=dtype, device="cuda", requires_grad=True)
+        torch.full(gate_shape, float("nan"), dtype=dtype, device="cuda")     # what freed memory may hold
+        s, y = block_norm(x, x, gate=gate, before_weight=torch.ones(32, device="cuda"))
+        dg, = torch.autograd.grad((s, y), gate, (torch.empty_like(s), torch.empty_like(y)))
+        assert dg.shape == gate.shape and torch.equal(dg, torch.zeros_like(dg)), (shape, gate_shape)
+
+
 def test_block_norm_gradient_against_differences():
     from yolo_amd.layers import block_norm
     g = _gen(33)

@@ -280,6 +280,8 @@ def _norm_backward(ctx, dstream, dnormed):
         dstream = dstream.contiguous()
         ds = dstream.data_ptr()
     grads = [_empty(t.shape, dtype=t.dtype, device=dev) if need else None for t, need in zip(tensors, ctx.needs_input_grad)]
+    if grads[2] is not None and tensors[0].numel() == 0:         # no row has a share in a gate's row
+        grads[2].zero_()
     b = BlockNormBackwardDesc(d, dn, ds, *[0 if g is None else g.data_ptr() for g in grads])
     nbytes = lib.yolo_amd_block_norm_backward_workspace_bytes(b)
     ws = _scratch(b, nbytes, tensors[0]) if nbytes else None     # noqa: F841
