@@ -322,37 +322,40 @@ block_norm_forward_kernel(const NormArgs a) {
     }
 }
 
-// The column sums of a workgroup: N vectors, each thread's eight columns of each.  In LDS while a thread has eight columns
-// (a thread only ever touches its own words, in order): the registers they would take hide more of memory's latency as
-// further waves.  Sixteen columns would not fit there and stay in registers.
+// The column sums of a workgroup: N vectors, each thread's columns of each.  As many of them in LDS as fit (a thread only
+// ever touches its own words, in order): the registers they would take hide more of memory's latency as further waves,
+// and with sixteen columns to a thread there are none to spare (2048 rows of 8192, layer, bf16 with an fp32 stream: in
+// registers 150 us, in LDS 90).
 template <typename C, int TPR, int GROUPS, int N>
 struct Sums {
-    static constexpr bool LDS = C::E == 8;
-    static constexpr int NT = TPR * GROUPS, WORDS = LDS ? N * 2 * NT : GROUPS > 1 ? GROUPS * C::E * TPR / 4 : 1;
+    static constexpr int NT = TPR * GROUPS, Q = C::E / 4, FIT = (160 * 1024 - 1024) / (C::E * NT * 4), IN_LDS = FIT < N ? FIT : N;
+    static constexpr int WORDS = IN_LDS * Q * NT;
+    static_assert(IN_LDS == N || GROUPS == 1, "rows this long have a workgroup each");
     f32x4* lds;                                        // WORDS of them
-    float v[LDS ? 1 : N][C::E];
+    float v[IN_LDS < N ? N - IN_LDS : 1][C::E];
 
     __device__ __forceinline__ void clear(int k) {
-        if constexpr (LDS) {
-            lds[(k * 2) * NT + threadIdx.x] = lds[(k * 2 + 1) * NT + threadIdx.x] = f32x4{0.f, 0.f, 0.f, 0.f};
+        if (k < IN_LDS) {
+#pragma unroll
+            for (int q = 0; q < Q; ++q) lds[(k * Q + q) * NT + threadIdx.x] = f32x4{0.f, 0.f, 0.f, 0.f};
         } else {
 #pragma unroll
-            for (int e = 0; e < C::E; ++e) v[k][e] = 0.f;
+            for (int e = 0; e < C::E; ++e) v[k - IN_LDS][e] = 0.f;
         }
     }
     // sums[k] += x * y
     __device__ __forceinline__ void add(int k, const float (&x)[C::E], const float (&y)[C::E]) {
-        if constexpr (LDS) {
+        if (k < IN_LDS) {
 #pragma unroll
-            for (int q = 0; q < 2; ++q) {
-                f32x4 s = lds[(k * 2 + q) * NT + threadIdx.x];
+            for (int q = 0; q < Q; ++q) {
+                f32x4 s = lds[(k * Q + q) * NT + threadIdx.x];
 #pragma unroll
                 for (int i = 0; i < 4; ++i) s[i] = fmaf(x[q * 4 + i], y[q * 4 + i], s[i]);
-                lds[(k * 2 + q) * NT + threadIdx.x] = s;
+                lds[(k * Q + q) * NT + threadIdx.x] = s;
             }
         } else {
 #pragma unroll
-            for (int e = 0; e < C::E; ++e) v[k][e] = fmaf(x[e], y[e], v[k][e]);
+            for (int e = 0; e < C::E; ++e) v[k - IN_LDS][e] = fmaf(x[e], y[e], v[k - IN_LDS][e]);
         }
     }
     __device__ __forceinline__ void add(int k, const float (&x)[C::E]) {
@@ -363,14 +366,14 @@ struct Sums {
     }
     // the groups' sums in group order -> out[0 .. D); every thread calls it
     __device__ __forceinline__ void write(int k, int t, int group, int D, float* out) {
-        if constexpr (LDS) {
+        if (k < IN_LDS) {
             __syncthreads();
             if (group == 0) {
 #pragma unroll
-                for (int q = 0; q < 2; ++q) {
-                    f32x4 s = lds[(k * 2 + q) * NT + t];
+                for (int q = 0; q < Q; ++q) {
+                    f32x4 s = lds[(k * Q + q) * NT + t];
 #pragma unroll
-                    for (int g = 1; g < GROUPS; ++g) s += lds[(k * 2 + q) * NT + g * TPR + t];
+                    for (int g = 1; g < GROUPS; ++g) s += lds[(k * Q + q) * NT + g * TPR + t];
 #pragma unroll
                     for (int i = 0; i < 4; ++i)
                         if (C::in(t, q * 4 + i, D)) out[C::col(t, q * 4 + i)] = s[i];
@@ -378,20 +381,21 @@ struct Sums {
             }
             __syncthreads();
         } else {
-            static_assert(LDS || GROUPS == 1, "rows this long have a workgroup each");
 #pragma unroll
             for (int e = 0; e < C::E; ++e)
-                if (C::in(t, e, D)) out[C::col(t, e)] = v[k][e];
+                if (C::in(t, e, D)) out[C::col(t, e)] = v[k - IN_LDS][e];
         }
     }
 };
 
 // The next row of each group is on its way (as it is in memory) while one is worked on; parameters that all rows share
-// stay in registers.
+// stay in registers.  1024 threads of sixteen columns have 128 registers each, too few for either: they read a row where
+// it is used, and the parameters (from L2) again with every row (2048 bf16 rows of 16384, rms: 149 us, otherwise 331).
 template <typename T, typename R, int TPR, int CH, bool FULL, bool LAYER>
 __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR)
 block_norm_backward_kernel(const NormArgs a) {
     constexpr int NT = TPR < 256 ? 256 : TPR, GROUPS = NT / TPR, E = CH * 8;
+    constexpr bool AHEAD = TPR * CH < 2048;
     typedef Cols<TPR, CH, FULL> C;
     __shared__ float slots[2][2][NT / 64];
     enum { WB, WA, WG, BB, BA };
@@ -406,39 +410,65 @@ block_norm_backward_kernel(const NormArgs a) {
     const long long s1 = min(a.sequences, s0 + a.seq_per_block);
 #pragma unroll
     for (int k = 0; k < (LAYER ? 5 : 3); ++k) sums.clear(k);
-    float pa[E], pb[E], pg[E];
-#pragma unroll
-    for (int e = 0; e < E; ++e) pa[e] = pb[e] = pg[e] = 1.f;
-    if (a.aw) C::template param<T>(a.aw, a.after_f32, 0, a.D, t, pa);
-    if (a.bw) C::template param<T>(a.bw, a.before_f32, 0, a.D, t, pb);
-    if (a.gate && a.gate_shared) C::template param<T>(a.gate, a.gate_f32, 0, a.D, t, pg);
     const bool row_gate = a.gate && !a.gate_shared;
+    float pa[E], pb[E], pg[E];
+    auto parameter = [&](const void* p, int f32, long long at, float (&v)[E]) {
+        if constexpr (!AHEAD) asm volatile("" : "+s"(at));     // not to be read ahead of the loop and kept after all
+        if (p) {
+            C::template param<T>(p, f32, at, a.D, t, v);
+        } else {
+#pragma unroll
+            for (int e = 0; e < E; ++e) v[e] = 1.f;
+        }
+    };
+    auto after_weight = [&] { parameter(a.aw, a.after_f32, 0, pa); };
+    auto before_weight = [&] { parameter(a.bw, a.before_f32, 0, pb); };
+    auto gate_of = [&](long long row) { parameter(a.gate, a.gate_f32, a.gate ? gate_row(a, row) * a.D : 0, pg); };
+    if constexpr (AHEAD) {
+        after_weight();
+        before_weight();
+        gate_of(0);                                    // of all rows, or none
+    }
     typename C::template Raw<T> ru, ry;
     typename C::template Raw<R> rh, rd;
     typename C::template Param<T> rg;
-    auto fetch = [&](long long row) {
+    auto fetch_values = [&](long long row) {
         ru.load((const T*)a.x + row * a.ldx, a.D, t);
         if (a.res) rh.load((const R*)a.res + row * a.ldr, a.D, t);
+        if (AHEAD && row_gate) rg.load(a.gate, a.gate_f32, gate_row(a, row) * a.D, a.D, t);
+    };
+    auto fetch_gradients = [&](long long row) {
         if (a.dy) ry.load((const T*)a.dy + row * a.D, a.D, t);
         if (a.dh) rd.load((const R*)a.dh + row * a.D, a.D, t);
-        if (row_gate) rg.load(a.gate, a.gate_f32, gate_row(a, row) * a.D, a.D, t);
     };
     for (long long seq = s0; seq < s1; ++seq) {
         const long long r0 = seq * a.length + chunk * a.chunk_rows;
         const long long r1 = min(seq * a.length + a.length, r0 + a.chunk_rows);
-        fetch(min(r0 + group, r1 - 1));
+        if constexpr (AHEAD) {
+            fetch_values(min(r0 + group, r1 - 1));
+            fetch_gradients(min(r0 + group, r1 - 1));
+        }
         for (long long base = r0; base < r1; base += GROUPS) {
             const bool valid = base + group < r1;
             const long long row = valid ? base + group : r1 - 1;
+            const long long next = min(base + GROUPS + group, r1 - 1);
+            const bool more = AHEAD && base + GROUPS < r1;
             float u[E], h[E], d[E], dy[E], p[E];
+            if constexpr (!AHEAD) fetch_values(row);
             ru.get(a.D, t, u);
 #pragma unroll
             for (int e = 0; e < E; ++e) h[e] = d[e] = 0.f;
             if (a.res) rh.get(a.D, t, h);
-            if (a.dy) ry.get(a.D, t, dy);
-            if (a.dh) rd.get(a.D, t, d);
-            if (row_gate) rg.get(a.gate_f32, a.D, t, pg);
-            if (base + GROUPS < r1) fetch(min(base + GROUPS + group, r1 - 1));
+            if (AHEAD && row_gate) rg.get(a.gate_f32, a.D, t, pg);
+            auto gradients = [&] {
+                if constexpr (!AHEAD) fetch_gradients(row);
+                if (a.dy) ry.get(a.D, t, dy);
+                if (a.dh) rd.get(a.D, t, d);
+            };
+            // sixteen columns to a thread: the gradients later, when fewer registers are taken
+            if constexpr (CH == 1) gradients();
+            if (more) fetch_values(next);
+            if (CH == 1 && more) fetch_gradients(next);
             // forward again: u becomes u^ (its norm without weights), h the stream
             float fu = 1.f;
             if (a.after) {
@@ -447,6 +477,7 @@ block_norm_backward_kernel(const NormArgs a) {
 #pragma unroll
                 for (int e = 0; e < E; ++e) u[e] = C::in(t, e, a.D) ? (u[e] - mean) * fu : 0.f;
             }
+            if constexpr (!AHEAD) after_weight();
 #pragma unroll
             for (int e = 0; e < E; ++e) p[e] = u[e] * pa[e];
             if (LAYER && a.ab) {
@@ -455,17 +486,23 @@ block_norm_backward_kernel(const NormArgs a) {
 #pragma unroll
                 for (int e = 0; e < E; ++e) p[e] += w[e];
             }
+            float mean_h = 0.f, fh = 0.f;
             if (a.dy) {
-                float mean, f;
+                if constexpr (!AHEAD) gate_of(row);
 #pragma unroll
                 for (int e = 0; e < E; ++e) h[e] = fmaf(a.scale, pg[e] * p[e], h[e]);
-                row_stats<C>(h, a, t, sum, mean, f);
+                row_stats<C>(h, a, t, sum, mean_h, fh);
+            }
+            if constexpr (CH > 1) gradients();
+            if (CH > 1 && more) fetch_gradients(next);
+            if (a.dy) {
 #pragma unroll
-                for (int e = 0; e < E; ++e) h[e] = C::in(t, e, a.D) ? (h[e] - mean) * f : 0.f;
+                for (int e = 0; e < E; ++e) h[e] = C::in(t, e, a.D) ? (h[e] - mean_h) * fh : 0.f;
                 if (valid) {
                     if (a.at_wb >= 0) sums.add(WB, dy, h);
                     if (LAYER && a.at_bb >= 0) sums.add(BB, dy);
                 }
+                if constexpr (!AHEAD) before_weight();
                 float c0 = 0.f, c1 = 0.f;
 #pragma unroll
                 for (int e = 0; e < E; ++e) {
@@ -478,10 +515,11 @@ block_norm_backward_kernel(const NormArgs a) {
                 c0 *= a.inv_d;
                 c1 *= a.inv_d;
 #pragma unroll
-                for (int e = 0; e < E; ++e) d[e] = C::in(t, e, a.D) ? d[e] + f * (dy[e] - c0 - h[e] * c1) : 0.f;
+                for (int e = 0; e < E; ++e) d[e] = C::in(t, e, a.D) ? d[e] + fh * (dy[e] - c0 - h[e] * c1) : 0.f;
             }
             if (a.dres && valid) C::store((R*)a.dres + row * a.D, a.D, t, d);
             // gate
+            if constexpr (!AHEAD) gate_of(row);
 #pragma unroll
             for (int e = 0; e < E; ++e) {
                 p[e] *= a.scale * d[e];
@@ -497,6 +535,7 @@ block_norm_backward_kernel(const NormArgs a) {
                 if (LAYER && a.at_ba >= 0) sums.add(BA, d);
             }
             if (a.after && a.dx) {
+                if constexpr (!AHEAD) after_weight();
                 float c0 = 0.f, c1 = 0.f;
 #pragma unroll
                 for (int e = 0; e < E; ++e) {

@@ -91,8 +91,9 @@ static int launch(const yolo_amd_block_norm_desc* d, const NormArgs& a, int bloc
 
 // How the backward pass cuts its rows: runs that share a gate row (one run where none does), each run in chunks or
 // several runs to a block.  A block for every CU, and up to three (what the registers of rows to 2048 allow) where each
-// still has eight rows or more for each of its groups: every block adds a row of partial sums per parameter.  8192 bf16
-// rows of 2048: 256 blocks 69 us, 768 blocks 63; 1239 rows of 1021: 17 against 23.
+// still has four rows or more for each of its groups: every block adds a row of partial sums per parameter.  8192 bf16
+// rows of 2048: 256 blocks 69 us, 768 blocks 63; 4207 fp32 rows of 769 (layer): 256 blocks 56 us, 525 45; 1239 rows of
+// 1021: 256 blocks 17 us, 768 23.
 struct BackwardPlan {
     bool sequence_gate, channel_gate, token_gate;
     long long sequences, length, chunk_rows;
@@ -112,7 +113,7 @@ static BackwardPlan plan(const yolo_amd_block_norm_backward_desc* b) {
     p.length = p.sequence_gate ? d->rows_per_gate : d->rows;
     p.sequences = (d->rows + p.length - 1) / p.length;
     const int groups = norm_backward_groups((int)d->d);
-    const long long target = std::min<long long>(d->d <= 2048 ? 768 : 256, std::max<long long>(256, d->rows / (8 * groups)));
+    const long long target = std::min<long long>(d->d <= 2048 ? 768 : 256, std::max<long long>(256, d->rows / (4 * groups)));
     if (p.sequences >= target) {
         p.chunks = 1;
         p.chunk_rows = p.length;
