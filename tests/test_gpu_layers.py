@@ -462,6 +462,16 @@ def test_block_norm_widths(dim, dtype, stream, par):
         _check_norm(_norm_case(g, lead, dim, dtype, stream, norm, after, gate, par), norm, after, 0.5)
 
 
+@pytest.mark.parametrize("dim", [2, 7, 9, 511, 1025, 1528, 1536, 2056, 2560, 2561, 3584, 4104, 5504, 6144, 6145, 6501, 7168, 8184, 8191, 8200])
+def test_block_norm_widths_between(dim):
+    """Rows that fill some of a workgroup's waves, whole or not, and that end anywhere in a run of eight."""
+    g = _gen(dim + 1)
+    _check_norm(_norm_case(g, (2, 3), dim, BF16, BF16, "rms", True, "token", F32), "rms", True, 0.5)
+    _check_norm(_norm_case(g, (3, 2), dim, F16, F32, "rms", False, "channel", F16), "rms", False, 2.0)
+    if dim >= 8:
+        _check_norm(_norm_case(g, (2, 5), dim, F32, F32, "layer", True, "sequence", F32), "layer", True, 0.5)
+
+
 @pytest.mark.parametrize("dim", [16384, 12001])
 def test_block_norm_widest(dim):
     g = _gen(5)

@@ -55,76 +55,87 @@ struct Eight {
     typedef S vecu __attribute__((ext_vector_type(8), aligned(sizeof(S))));
 };
 
-// The columns thread t of a group owns: CH runs of eight, TPR * 8 apart.  D may be any number: the thread whose run
-// holds a row's last one to seven values (D % 8) reads the row's last eight and moves them down, and stores by element.
-// FULL: D is exactly TPR * CH * 8 and no column needs a check.
-template <int TPR, int CH, bool FULL>
+// The columns thread t of a group owns: CH runs of eight, TPR * 8 apart.  D may be any number: a run that would pass the
+// row's end holds the row's last eight values instead, and those of them that are not its own (the run before it owns
+// them, or it owns none) are left out of sums and stores.
+//   FULL: the threads there are hold exactly D columns and none needs a check.
+//   EIGHTS: D is a multiple of 8: a run is the row's or it is not.
+//   ANY: element by element, in the waves that hold a row's end.
+// (rms, bf16, forward, 67 MB in and out: rows of 1536, FULL, 25 us; of 1528, EIGHTS, 30; of 1500, ANY, 38, with
+// every other row starting between 16-byte boundaries.)
+enum { ANY, EIGHTS, FULL };
+template <int TPR, int CH, int MODE>
 struct Cols {
     static constexpr int E = CH * 8;
-    __device__ static __forceinline__ int col(int t, int e) { return ((e >> 3) * TPR + t) * 8 + (e & 7); }
-    __device__ static __forceinline__ bool in(int t, int e, int D) { return FULL || col(t, e) < D; }
+    // run c's first column as counted, and as held
+    __device__ static __forceinline__ int run(int t, int c) { return (c * TPR + t) * 8; }
+    __device__ static __forceinline__ int held(int t, int c, int D) { return MODE == FULL ? run(t, c) : min(run(t, c), max(D - 8, 0)); }
+    __device__ static __forceinline__ int col(int t, int e, int D) { return held(t, e >> 3, D) + (e & 7); }
+    // is element e a column of its own
+    __device__ static __forceinline__ bool in(int t, int e, int D) {
+        const int c = col(t, e, D);
+        return MODE == FULL || (MODE == EIGHTS ? run(t, e >> 3) < D : c >= run(t, e >> 3) && c < D);
+    }
+    // has this wave (ANY) a run that is not whole
+    __device__ static __forceinline__ bool edge(int t, int c, int D) { return __builtin_amdgcn_ballot_w64(run(t, c) + 8 > D) != 0; }
+    // sum over the thread's columns; add(e, s): s and element e's share
+    template <typename F>
+    __device__ static __forceinline__ float total(int t, int D, F add) {
+        float s = 0.f;
+#pragma unroll
+        for (int c = 0; c < CH; ++c) {
+            float r = 0.f;
+            if (MODE == ANY && edge(t, c, D)) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const float n = add(c * 8 + i, r);
+                    r = in(t, c * 8 + i, D) ? n : r;
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) r = add(c * 8 + i, r);
+            }
+            if (MODE == EIGHTS) r = in(t, c * 8, D) ? r : 0.f;
+            s = c ? s + r : r;
+        }
+        return s;
+    }
 
     // a row's values as they are in memory, so that a row can be on its way while another is worked on
     template <typename S>
     struct Raw {
         typename Eight<S>::vec v[CH];
         __device__ __forceinline__ void load(const S* row, int D, int t) {
-            if constexpr (FULL) {
+            if (MODE != ANY || D >= 8) {
 #pragma unroll
                 for (int c = 0; c < CH; ++c) {
-                    const typename Eight<S>::vecu x = *reinterpret_cast<const typename Eight<S>::vecu*>(row + (c * TPR + t) * 8);
+                    const typename Eight<S>::vecu x = *reinterpret_cast<const typename Eight<S>::vecu*>(row + held(t, c, D));
                     v[c] = x;
                 }
-            } else if (D >= 8) {
-#pragma unroll
-                for (int c = 0; c < CH; ++c) {
-                    const typename Eight<S>::vecu x = *reinterpret_cast<const typename Eight<S>::vecu*>(row + min((c * TPR + t) * 8, D - 8));
-                    v[c] = x;
-                }
-            } else {                                   // a row shorter than eight: by element, thread 0
+            } else {                                   // a row shorter than eight: by element
 #pragma unroll
                 for (int i = 0; i < 8; ++i) v[0][i] = row[min(i, D - 1)];
             }
         }
-        // columns past D as 0
-        __device__ __forceinline__ void get(int D, int t, float (&f)[E]) const {
+        __device__ __forceinline__ void get(float (&f)[E]) const {
 #pragma unroll
             for (int e = 0; e < E; ++e) f[e] = (float)v[e >> 3][e & 7];
-            if constexpr (!FULL) finish(D, t, f);
         }
     };
-    __device__ static __forceinline__ void finish(int D, int t, float (&f)[E]) {
-#pragma unroll
-        for (int c = 0; c < CH; ++c) {
-            const int at = (c * TPR + t) * 8;
-            if ((D & 7) && D >= 8) {
-                const bool last = at < D && at + 8 > D;
-                const int s = 8 - (D & 7);             // places to move down (the same for all rows)
-#pragma unroll
-                for (int bit = 1; bit < 8; bit *= 2)
-                    if (s & bit) {
-#pragma unroll
-                        for (int i = 0; i < 8; ++i) f[c * 8 + i] = last ? (i + bit < 8 ? f[c * 8 + i + bit] : 0.f) : f[c * 8 + i];
-                    }
-            }
-#pragma unroll
-            for (int i = 0; i < 8; ++i) f[c * 8 + i] = at + i < D ? f[c * 8 + i] : 0.f;
-        }
-    }
     template <typename S>
     __device__ static __forceinline__ void store(S* row, int D, int t, const float (&v)[E]) {
 #pragma unroll
         for (int c = 0; c < CH; ++c) {
-            const int at = (c * TPR + t) * 8;
-            if (FULL || at + 8 <= D) {
+            const int at = run(t, c);
+            if (MODE == FULL || at + 8 <= D) {
                 typename Eight<S>::vecu x;
 #pragma unroll
                 for (int i = 0; i < 8; ++i) x[i] = (S)v[c * 8 + i];
                 *reinterpret_cast<typename Eight<S>::vecu*>(row + at) = x;
-            } else if (at < D) {
+            } else if (MODE == ANY && at < D) {
 #pragma unroll
-                for (int i = 0; i < 7; ++i)
-                    if (at + i < D) row[at + i] = (S)v[c * 8 + i];
+                for (int i = 0; i < 8; ++i)
+                    if (in(t, c * 8 + i, D)) row[col(t, c * 8 + i, D)] = (S)v[c * 8 + i];
             }
         }
     }
@@ -148,7 +159,7 @@ struct Cols {
                 for (int c = 0; c < CH; ++c) w[c][0] = __builtin_bit_cast(u32x4, r.v[c]);
             }
         }
-        __device__ __forceinline__ void get(int f32, int D, int t, float (&f)[E]) const {
+        __device__ __forceinline__ void get(int f32, float (&f)[E]) const {
             if (f32) {
 #pragma unroll
                 for (int e = 0; e < E; ++e) f[e] = __uint_as_float(w[e >> 3][(e >> 2) & 1][e & 3]);
@@ -160,14 +171,13 @@ struct Cols {
                     for (int i = 0; i < 8; ++i) f[c * 8 + i] = (float)v[i];
                 }
             }
-            if constexpr (!FULL) finish(D, t, f);
         }
     };
     template <typename T>
     __device__ static __forceinline__ void param(const void* p, int f32, long long at, int D, int t, float (&v)[E]) {
         Param<T> r;
         r.load(p, f32, at, D, t);
-        r.get(f32, D, t, v);
+        r.get(f32, v);
     }
 };
 
@@ -185,12 +195,19 @@ __device__ __forceinline__ float wave_sum(float v) {
            (__int_as_float(__builtin_amdgcn_readlane(b, 32)) + __int_as_float(__builtin_amdgcn_readlane(b, 48)));
 }
 
-// Sums over a group of TPR threads; every thread of the workgroup makes the same calls.  Two slot sets in turn:
-// a set is written again only after the barrier of the call in between, which its readers reach after reading.
+// Sums over a group of TPR threads (or of the first so many waves of them: see threads_of); every thread of the
+// workgroup makes the same calls.  Two slot sets in turn: a set is written again only after the barrier of the call in
+// between, which its readers reach after reading.
 template <int TPR, int NT>
 struct GroupSum {
     float (*slots)[2][NT / 64];
     int parity;
+    // waves that are not there add zeros (their slots are written here alone, ahead of the first call's barrier)
+    __device__ __forceinline__ void init() {
+        parity = 0;
+        const int w = threadIdx.x % (NT / 64);
+        if (threadIdx.x < 4 * (NT / 64) && w >= (int)(blockDim.x >> 6)) (&slots[0][0][0])[threadIdx.x] = 0.f;
+    }
     __device__ __forceinline__ void two(float& a, float& b) {
         a = wave_sum(a);
         b = wave_sum(b);
@@ -232,32 +249,29 @@ __device__ __forceinline__ long long gate_row(const NormArgs& a, long long row) 
     return a.gate_shared ? 0 : (long long)((uint32_t)row / (uint32_t)a.rows_per_gate);
 }
 
-// mean (0 for rms) and factor of a row; columns past D hold 0
+// mean (0 for rms) and factor of a row
 template <typename C, typename G>
 __device__ __forceinline__ void row_stats(const float (&v)[C::E], const NormArgs& a, int t, G& sum, float& mean, float& f) {
     mean = 0.f;
     if (a.layer) {
-        float s = 0.f;
-#pragma unroll
-        for (int e = 0; e < C::E; ++e) s += v[e];
+        const float s = C::total(t, a.D, [&](int e, float r) { return r + v[e]; });
         mean = sum.one(s) * a.inv_d;
     }
-    float q = 0.f;
-#pragma unroll
-    for (int e = 0; e < C::E; ++e) {
-        const float d = C::in(t, e, a.D) ? v[e] - mean : 0.f;
-        q = fmaf(d, d, q);
-    }
+    const float q = C::total(t, a.D, [&](int e, float r) {
+        const float d = v[e] - mean;
+        return fmaf(d, d, r);
+    });
     f = rsqrtf(sum.one(q) * a.inv_d + a.eps);
 }
 
-template <typename T, typename R, int TPR, int CH, bool FULL>
+template <typename T, typename R, int TPR, int CH, int MODE>
 __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR)
 block_norm_forward_kernel(const NormArgs a) {
     constexpr int NT = TPR < 256 ? 256 : TPR, GROUPS = NT / TPR, E = CH * 8;
-    typedef Cols<TPR, CH, FULL> C;
+    typedef Cols<TPR, CH, MODE> C;
     __shared__ float slots[2][2][NT / 64];
-    GroupSum<TPR, NT> sum{slots, 0};
+    GroupSum<TPR, NT> sum{slots};
+    sum.init();
     const int t = threadIdx.x % TPR, group = threadIdx.x / TPR;
     for (long long base = (long long)blockIdx.x * GROUPS; base < a.rows; base += (long long)gridDim.x * GROUPS) {
         const bool valid = base + group < a.rows;
@@ -270,14 +284,14 @@ block_norm_forward_kernel(const NormArgs a) {
         if (a.res) rh.load((const R*)a.res + row * a.ldr, a.D, t);
         if (a.gate) rg.load(a.gate, a.gate_f32, gate_row(a, row) * a.D, a.D, t);
         if (a.aw) rw.load(a.aw, a.after_f32, 0, a.D, t);
-        ru.get(a.D, t, u);
+        ru.get(u);
         if (a.after) {
             float mean, f;
             row_stats<C>(u, a, t, sum, mean, f);
 #pragma unroll
-            for (int e = 0; e < E; ++e) u[e] = C::in(t, e, a.D) ? (u[e] - mean) * f : 0.f;
+            for (int e = 0; e < E; ++e) u[e] = (u[e] - mean) * f;
             if (a.aw) {
-                rw.get(a.after_f32, a.D, t, w);
+                rw.get(a.after_f32, w);
 #pragma unroll
                 for (int e = 0; e < E; ++e) u[e] *= w[e];
             }
@@ -289,12 +303,12 @@ block_norm_forward_kernel(const NormArgs a) {
         }
         if (a.bw) rw.load(a.bw, a.before_f32, 0, a.D, t);
         if (a.gate) {
-            rg.get(a.gate_f32, a.D, t, w);
+            rg.get(a.gate_f32, w);
 #pragma unroll
             for (int e = 0; e < E; ++e) u[e] *= w[e];
         }
         if (a.res) {
-            rh.get(a.D, t, h);
+            rh.get(h);
 #pragma unroll
             for (int e = 0; e < E; ++e) h[e] = fmaf(a.scale, u[e], h[e]);
         } else {
@@ -308,7 +322,7 @@ block_norm_forward_kernel(const NormArgs a) {
 #pragma unroll
             for (int e = 0; e < E; ++e) h[e] = (h[e] - mean) * f;
             if (a.bw) {
-                rw.get(a.before_f32, a.D, t, w);
+                rw.get(a.before_f32, w);
 #pragma unroll
                 for (int e = 0; e < E; ++e) h[e] *= w[e];
             }
@@ -328,7 +342,8 @@ block_norm_forward_kernel(const NormArgs a) {
 // registers 150 us, in LDS 90).
 template <typename C, int TPR, int GROUPS, int N>
 struct Sums {
-    static constexpr int NT = TPR * GROUPS, Q = C::E / 4, FIT = (160 * 1024 - 1024) / (C::E * NT * 4), IN_LDS = FIT < N ? FIT : N;
+    static constexpr int NT = TPR * GROUPS, Q = C::E / 4;
+    static constexpr int FIT = ((C::E == 8 ? 80 : 160) * 1024 - 1024) / (C::E * NT * 4), IN_LDS = FIT < N ? FIT : N;
     static constexpr int WORDS = IN_LDS * Q * NT;
     static_assert(IN_LDS == N || GROUPS == 1, "rows this long have a workgroup each");
     f32x4* lds;                                        // WORDS of them
@@ -376,14 +391,14 @@ struct Sums {
                     for (int g = 1; g < GROUPS; ++g) s += lds[(k * Q + q) * NT + g * TPR + t];
 #pragma unroll
                     for (int i = 0; i < 4; ++i)
-                        if (C::in(t, q * 4 + i, D)) out[C::col(t, q * 4 + i)] = s[i];
+                        if (C::in(t, q * 4 + i, D)) out[C::col(t, q * 4 + i, D)] = s[i];
                 }
             }
             __syncthreads();
         } else {
 #pragma unroll
             for (int e = 0; e < C::E; ++e)
-                if (C::in(t, e, D)) out[C::col(t, e)] = v[k - IN_LDS][e];
+                if (C::in(t, e, D)) out[C::col(t, e, D)] = v[k - IN_LDS][e];
         }
     }
 };
@@ -391,19 +406,20 @@ struct Sums {
 // The next row of each group is on its way (as it is in memory) while one is worked on; parameters that all rows share
 // stay in registers.  1024 threads of sixteen columns have 128 registers each, too few for either: they read a row where
 // it is used, and the parameters (from L2) again with every row (2048 bf16 rows of 16384, rms: 149 us, otherwise 331).
-template <typename T, typename R, int TPR, int CH, bool FULL, bool LAYER>
+template <typename T, typename R, int TPR, int CH, int MODE, bool LAYER>
 __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR)
 block_norm_backward_kernel(const NormArgs a) {
     constexpr int NT = TPR < 256 ? 256 : TPR, GROUPS = NT / TPR, E = CH * 8;
     constexpr bool AHEAD = TPR * CH < 2048;
-    typedef Cols<TPR, CH, FULL> C;
+    typedef Cols<TPR, CH, MODE> C;
     __shared__ float slots[2][2][NT / 64];
     enum { WB, WA, WG, BB, BA };
     typedef Sums<C, TPR, GROUPS, LAYER ? 5 : 3> S;
     __shared__ f32x4 words[S::WORDS];
     S sums;
     sums.lds = words;
-    GroupSum<TPR, NT> sum{slots, 0};
+    GroupSum<TPR, NT> sum{slots};
+    sum.init();
     const int t = threadIdx.x % TPR, group = threadIdx.x / TPR;
     const int chunk = blockIdx.x % a.chunks;
     const long long s0 = (long long)(blockIdx.x / a.chunks) * a.seq_per_block;
@@ -455,15 +471,15 @@ block_norm_backward_kernel(const NormArgs a) {
             const bool more = AHEAD && base + GROUPS < r1;
             float u[E], h[E], d[E], dy[E], p[E];
             if constexpr (!AHEAD) fetch_values(row);
-            ru.get(a.D, t, u);
+            ru.get(u);
 #pragma unroll
             for (int e = 0; e < E; ++e) h[e] = d[e] = 0.f;
-            if (a.res) rh.get(a.D, t, h);
-            if (AHEAD && row_gate) rg.get(a.gate_f32, a.D, t, pg);
+            if (a.res) rh.get(h);
+            if (AHEAD && row_gate) rg.get(a.gate_f32, pg);
             auto gradients = [&] {
                 if constexpr (!AHEAD) fetch_gradients(row);
-                if (a.dy) ry.get(a.D, t, dy);
-                if (a.dh) rd.get(a.D, t, d);
+                if (a.dy) ry.get(dy);
+                if (a.dh) rd.get(d);
             };
             // sixteen columns to a thread: the gradients later, when fewer registers are taken
             if constexpr (CH == 1) gradients();
@@ -475,7 +491,7 @@ block_norm_backward_kernel(const NormArgs a) {
                 float mean;
                 row_stats<C>(u, a, t, sum, mean, fu);
 #pragma unroll
-                for (int e = 0; e < E; ++e) u[e] = C::in(t, e, a.D) ? (u[e] - mean) * fu : 0.f;
+                for (int e = 0; e < E; ++e) u[e] = (u[e] - mean) * fu;
             }
             if constexpr (!AHEAD) after_weight();
 #pragma unroll
@@ -497,25 +513,22 @@ block_norm_backward_kernel(const NormArgs a) {
             if (CH > 1 && more) fetch_gradients(next);
             if (a.dy) {
 #pragma unroll
-                for (int e = 0; e < E; ++e) h[e] = C::in(t, e, a.D) ? (h[e] - mean_h) * fh : 0.f;
+                for (int e = 0; e < E; ++e) h[e] = (h[e] - mean_h) * fh;
                 if (valid) {
                     if (a.at_wb >= 0) sums.add(WB, dy, h);
                     if (LAYER && a.at_bb >= 0) sums.add(BB, dy);
                 }
                 if constexpr (!AHEAD) before_weight();
-                float c0 = 0.f, c1 = 0.f;
 #pragma unroll
-                for (int e = 0; e < E; ++e) {
-                    dy[e] *= pb[e];
-                    c0 += dy[e];
-                    c1 = fmaf(dy[e], h[e], c1);
-                }
+                for (int e = 0; e < E; ++e) dy[e] *= pb[e];
+                float c0 = C::total(t, a.D, [&](int e, float r) { return r + dy[e]; });
+                float c1 = C::total(t, a.D, [&](int e, float r) { return fmaf(dy[e], h[e], r); });
                 if (LAYER) sum.two(c0, c1);
                 else { c1 = sum.one(c1); c0 = 0.f; }
                 c0 *= a.inv_d;
                 c1 *= a.inv_d;
 #pragma unroll
-                for (int e = 0; e < E; ++e) d[e] = C::in(t, e, a.D) ? d[e] + fh * (dy[e] - c0 - h[e] * c1) : 0.f;
+                for (int e = 0; e < E; ++e) d[e] = d[e] + fh * (dy[e] - c0 - h[e] * c1);
             }
             if (a.dres && valid) C::store((R*)a.dres + row * a.D, a.D, t, d);
             // gate
@@ -536,13 +549,10 @@ block_norm_backward_kernel(const NormArgs a) {
             }
             if (a.after && a.dx) {
                 if constexpr (!AHEAD) after_weight();
-                float c0 = 0.f, c1 = 0.f;
 #pragma unroll
-                for (int e = 0; e < E; ++e) {
-                    d[e] *= pa[e];
-                    c0 += d[e];
-                    c1 = fmaf(d[e], u[e], c1);
-                }
+                for (int e = 0; e < E; ++e) d[e] *= pa[e];
+                float c0 = C::total(t, a.D, [&](int e, float r) { return r + d[e]; });
+                float c1 = C::total(t, a.D, [&](int e, float r) { return fmaf(d[e], u[e], r); });
                 if (LAYER) sum.two(c0, c1);
                 else { c1 = sum.one(c1); c0 = 0.f; }
                 c0 *= a.inv_d;
@@ -566,30 +576,46 @@ block_norm_backward_kernel(const NormArgs a) {
 }
 
 // ---------------------------------------------------------------- launch, one translation unit per element type
-// Threads per row by its length: eight values each, sixteen beyond what 1024 (forward) and 512 (backward, whose row,
-// parameters and column sums share the registers) threads hold.
+// Threads per row by its length: eight values each; sixteen where twelve waves of eight (forward: two rows to a CU;
+// 2048 bf16 rows of 8192, rms: 16 waves 29.9 us, 8 of sixteen 26.5) or 512 threads (backward, whose row, parameters and
+// column sums share the registers) do not hold it.
+// A row with a workgroup of its own has as many waves as it fills: the registers of those that would only wait hold
+// another row's (forward, 3048 rows of 5504: 16 waves 61 us, 11 waves 47, and 30 with EIGHTS).
+template <int TPR, int CH>
+static inline int threads_of(int D) {
+    return TPR < 256 ? 256 : CH > 1 ? TPR : (D + 511) / 512 * 64;
+}
+template <int TPR, int CH>
+static inline int mode_of(int D) {
+    return (TPR < 256 || CH > 1 ? D == TPR * CH * 8 : D % 512 == 0) ? FULL : D % 8 == 0 ? EIGHTS : ANY;
+}
 template <typename T, typename R, int TPR, int CH>
 static void norm_launch_forward(const NormArgs& a, int blocks, hipStream_t s) {
-    constexpr int NT = TPR < 256 ? 256 : TPR;
-    if (a.D == TPR * CH * 8) hipLaunchKernelGGL((block_norm_forward_kernel<T, R, TPR, CH, true>), dim3(blocks), dim3(NT), 0, s, a);
-    else hipLaunchKernelGGL((block_norm_forward_kernel<T, R, TPR, CH, false>), dim3(blocks), dim3(NT), 0, s, a);
+    const dim3 threads(threads_of<TPR, CH>(a.D));
+    switch (mode_of<TPR, CH>(a.D)) {
+        case FULL: hipLaunchKernelGGL((block_norm_forward_kernel<T, R, TPR, CH, FULL>), dim3(blocks), threads, 0, s, a); break;
+        case EIGHTS: hipLaunchKernelGGL((block_norm_forward_kernel<T, R, TPR, CH, EIGHTS>), dim3(blocks), threads, 0, s, a); break;
+        default: hipLaunchKernelGGL((block_norm_forward_kernel<T, R, TPR, CH, ANY>), dim3(blocks), threads, 0, s, a);
+    }
 }
-template <typename T, typename R, int TPR, int CH, bool FULL>
+template <typename T, typename R, int TPR, int CH, int MODE>
 static void norm_launch_backward(const NormArgs& a, int blocks, hipStream_t s) {
-    constexpr int NT = TPR < 256 ? 256 : TPR;
-    if (a.layer) hipLaunchKernelGGL((block_norm_backward_kernel<T, R, TPR, CH, FULL, true>), dim3(blocks), dim3(NT), 0, s, a);
-    else hipLaunchKernelGGL((block_norm_backward_kernel<T, R, TPR, CH, FULL, false>), dim3(blocks), dim3(NT), 0, s, a);
+    const dim3 threads(threads_of<TPR, CH>(a.D));
+    if (a.layer) hipLaunchKernelGGL((block_norm_backward_kernel<T, R, TPR, CH, MODE, true>), dim3(blocks), threads, 0, s, a);
+    else hipLaunchKernelGGL((block_norm_backward_kernel<T, R, TPR, CH, MODE, false>), dim3(blocks), threads, 0, s, a);
 }
 template <typename T, typename R, int TPR, int CH>
 static void norm_launch_backward(const NormArgs& a, int blocks, hipStream_t s) {
-    if (a.D == TPR * CH * 8) norm_launch_backward<T, R, TPR, CH, true>(a, blocks, s);
-    else norm_launch_backward<T, R, TPR, CH, false>(a, blocks, s);
+    switch (mode_of<TPR, CH>(a.D)) {
+        case FULL: norm_launch_backward<T, R, TPR, CH, FULL>(a, blocks, s); break;
+        case EIGHTS: norm_launch_backward<T, R, TPR, CH, EIGHTS>(a, blocks, s); break;
+        default: norm_launch_backward<T, R, TPR, CH, ANY>(a, blocks, s);
+    }
 }
 
 // rows a workgroup has in hand at a time
 static inline int norm_forward_groups(int D) { return D <= 512 ? 4 : D <= 1024 ? 2 : 1; }
 static inline int norm_backward_groups(int D) { return D <= 512 ? 4 : D <= 1024 ? 2 : 1; }
-
 template <typename T, typename R>
 static void norm_launch(const NormArgs& a, int blocks, bool backward, hipStream_t s) {
     if (!backward) {
@@ -597,7 +623,8 @@ static void norm_launch(const NormArgs& a, int blocks, bool backward, hipStream_
         else if (a.D <= 1024) norm_launch_forward<T, R, 128, 1>(a, blocks, s);
         else if (a.D <= 2048) norm_launch_forward<T, R, 256, 1>(a, blocks, s);
         else if (a.D <= 4096) norm_launch_forward<T, R, 512, 1>(a, blocks, s);
-        else if (a.D <= 8192) norm_launch_forward<T, R, 1024, 1>(a, blocks, s);
+        else if (a.D <= 6144) norm_launch_forward<T, R, 1024, 1>(a, blocks, s);
+        else if (a.D <= 8192) norm_launch_forward<T, R, 512, 2>(a, blocks, s);
         else norm_launch_forward<T, R, 1024, 2>(a, blocks, s);
     } else {
         if (a.D <= 512) norm_launch_backward<T, R, 64, 1>(a, blocks, s);
