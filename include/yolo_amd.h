@@ -444,7 +444,8 @@ int yolo_amd_block_norm_forward(const yolo_amd_block_norm_desc* desc, void* stre
  * everything is recomputed from x and residual).  dnormed and dstream: gradients of the two outputs, [rows][d]
  * without gaps, of `type` and of the stream's type; NULL: zero.  Of the gradients below each may be NULL:
  * dx and dresidual [rows][d] of x's and the stream's type, the others shaped and typed like what they belong
- * to.  With a gate, rows must be whole runs of rows_per_gate (or one run).  All sums have a fixed order. */
+ * to.  With a gate, rows must be whole runs of rows_per_gate (or one run); with rows = 0 there is no run
+ * and dgate is not written, the parameters' gradients are zero.  All sums have a fixed order. */
 typedef struct {
     yolo_amd_block_norm_desc forward;
     const void* dnormed;

@@ -7,6 +7,7 @@ Submodules
   yolo_amd.yolo_v3  drop-in for the reference's yolo_v3.py
   yolo_amd.cfg      generator for the cfg text / params dict the reference expects
   yolo_amd.engine   fused execution plan (descriptors for libyolo_amd.so)
+  yolo_amd.layers   linear (product with epilogue) and block_norm (norms around a residual add), with gradients
   yolo_amd.dist     batch sharding and the detection gather for multi-GPU runs
 
 Importing yolo_amd.utilis / yolo_amd.yolo_v3 loads libyolo_amd.so and fails

@@ -8,7 +8,7 @@ void block_norm_launch_f32(const NormArgs& a, int blocks, bool backward, hipStre
 }
 
 // Sums of partial column sums: out[o][c] = sum over b of part[(o * blocks + b) * stride + c], b ascending within
-// each of the workgroup's 16 waves, the waves in order.
+// each of the workgroup's 16 waves, the waves in order.  745 blocks x 3 vectors of 2048: 6.0 us, 18 MB; else latency.
 struct SumArgs {
     const float* part[5];
     void* out[5];
