@@ -548,6 +548,53 @@ def test_block_norm_views_and_far_values():
         assert torch.equal(z[[0, 1, 2, 5]], y[[0, 1, 2, 5]])
 
 
+@pytest.mark.parametrize("dim", [5, 256, 520, 769, 1024, 1500, 2050, 7168, 8193])
+def test_block_norm_rows_do_not_meet(dim):
+    """NaN and infinities in one row leave every other row's values and gradients alone, whole rows or not."""
+    from yolo_amd.layers import block_norm
+    g = _gen(dim + 7)
+    x, r, ds, dy = (_rand(g, 11, dim, dtype=BF16) for _ in range(4))
+    w, b = _rand(g, dim), _rand(g, dim)
+    for norm in ("rms", "layer"):
+        def run(x, r):
+            leaves = [x.clone().requires_grad_(), r.clone().requires_grad_()]
+            out = block_norm(*leaves, norm=norm, after_weight=w, after_bias=b if norm == "layer" else None,
+                             gate=w, before_weight=b)
+            return [*out, *torch.autograd.grad(out, leaves, (ds, dy))]
+        clean = run(x, r)
+        bad_x, bad_r = x.clone(), r.clone()
+        bad_x[3, dim - 1], bad_x[6, 0], bad_r[8, dim // 2] = float("nan"), float("inf"), float("nan")
+        keep = [i for i in range(11) if i not in (3, 6, 8)]
+        for got, want in zip(run(bad_x, bad_r), clean):
+            assert torch.equal(got[keep], want[keep]), (norm, dim)
+
+
+def test_block_norm_offsets_past_32_bits():
+    from yolo_amd.layers import block_norm
+    rows, dim = 2 ** 20 + 333, 2056                          # 2.16e9 values
+    g = _gen(13)
+    ends = torch.cat([torch.arange(100), torch.arange(rows - 100, rows)]).cuda()
+    def filled(value):
+        t = torch.empty(rows, dim, dtype=BF16, device="cuda").fill_(value)
+        t[ends] = _rand(g, 200, dim, dtype=BF16)
+        return t
+    x, r, ds, dy = filled(0.5).requires_grad_(), filled(-0.25).requires_grad_(), filled(1.0), filled(0.125)
+    params = {"after_weight": 1 + _rand(g, dim, scale=0.3), "before_weight": 1 + _rand(g, dim, scale=0.3), "gate": _rand(g, dim)}
+    s, y = block_norm(x, r, after=True, **params)
+    dx, dr = torch.autograd.grad((s, y), (x, r), (ds, dy))
+    conf = ("rms", True, True, 1.0, 1e-6)
+    small = [t.detach()[ends] for t in (x, r, ds, dy)]
+    all_params = {"gate": params["gate"], "after_weight": params["after_weight"], "after_bias": None,
+                  "before_weight": params["before_weight"], "before_bias": None}
+    out = ref.norm_ref(small[0], small[1], conf, all_params, (small[2], small[3]))
+    assert_within(s[ends], out["stream"][0], rounded(*out["stream"], BF16), "stream")
+    assert_within(y[ends], out["normed"][0], rounded(*out["normed"], BF16), "normed")
+    assert_within(dx[ends], out["x"][0], rounded(*out["x"], BF16), "dx")
+    assert_within(dr[ends], out["residual"][0], rounded(*out["residual"], BF16), "dresidual")
+    for t in (s, y, dx, dr):                                 # the rows in between are all alike
+        assert torch.equal(t[5000], t[rows - 5000])
+
+
 def test_block_norm_empty():
     from yolo_amd.layers import block_norm
     x = torch.empty(0, 32, dtype=BF16, device="cuda", requires_grad=True)
