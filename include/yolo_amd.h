@@ -347,12 +347,14 @@ typedef struct {
     const void* residual; /* or NULL; may be y itself (same stride and type)            */
     void* y;
     void* pre;            /* or NULL: x weight^T + bias [m][n] (no gaps between rows),   */
-                          /* rounded to `type`: what yolo_amd_linear_backward wants      */
+                          /* what yolo_amd_linear_backward wants: as summed, in fp32, with */
+                          /* pre_f32, else rounded to `type`                             */
     int64_t m, n, k;
     int64_t ldx, ldw, ldr, ldy;
     int type;             /* YOLO_AMD_TYPE_BF16 or YOLO_AMD_TYPE_F16                     */
     int bias_f32, residual_f32, y_f32;
     int activation;       /* YOLO_AMD_ACT_*                                             */
+    int pre_f32;
     void* workspace;      /* 256-byte aligned, yolo_amd_linear_workspace_bytes bytes     */
     size_t workspace_bytes;
 } yolo_amd_linear_desc;
@@ -393,6 +395,7 @@ typedef struct {
     int type;
     int dy_f32, dbias_f32;
     int activation;
+    int pre_f32;          /* as in the forward call that wrote pre                       */
     void* workspace;      /* 256-byte aligned                                            */
     size_t workspace_bytes;
 } yolo_amd_linear_backward_desc;

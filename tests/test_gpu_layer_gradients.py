@@ -1,0 +1,77 @@
+"""Gradients of yolo_amd.layers.linear held to what a computation in 32 bits with one rounding at its end gives: neither
+the pre-activation nor its gradient loses bits on the way that the caller's types would have kept."""
+import ctypes
+
+import pytest
+import torch
+
+import layer_reference as ref
+from layer_reference import EPS32, assert_within, d, rounded, slope64
+
+pytestmark = pytest.mark.gpu
+
+BF16, F16, F32 = torch.bfloat16, torch.float16, torch.float32
+
+
+def _rand(g, *shape, scale=1.0, dtype=F32):
+    return (torch.randn(*shape, generator=g) * scale).to(dtype).cuda()
+
+
+# few rows, whole tiles, ragged ends and odd rows, split reductions in the forward product
+KEPT = [(1, 40, 64), (3, 984, 64), (5, 114, 4680), (64, 128, 64), (130, 75, 261), (333, 761, 4104), (200, 1030, 520), (1990, 2048, 264)]
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("m,n,k", KEPT)
+def test_linear_slopes_are_of_the_unrounded_preactivation(m, n, k, dtype):
+    """The bias gradient sums dy * act'(p) without any rounding to x's type; the slope is off by |act''| times what the fp32
+    sum p is off (its bound, 0.8 for all three) and EPS32 of its own size."""
+    from yolo_amd.layers import linear
+    g = torch.Generator().manual_seed(m + 3 * n + 5 * k)
+    x, w = _rand(g, m, k, dtype=dtype), _rand(g, n, k, scale=k ** -0.5, dtype=dtype)
+    for act in ("gelu", "gelu_tanh", "silu"):
+        b = _rand(g, n, scale=0.3).requires_grad_()
+        dy = _rand(g, m, n, dtype=dtype)
+        db, = torch.autograd.grad(linear(x, w, b, activation=act), b, dy)
+        _, _, p, ep = ref.linear_ref(x, w, b, None, act, dtype)
+        s, dy = slope64(p, act), d(dy)
+        edp = dy.abs() * (0.8 * ep + EPS32 * (1 + s.abs())) + 2.0 ** -23 * (dy * s).abs()
+        want = (dy * s).sum(0)
+        assert_within(db, want, rounded(want, edp.sum(0) + 512 * 2.0 ** -24 * (dy * s).abs().sum(0), F32), f"db {act}")
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("m,n,k", KEPT)
+def test_linear_entry_keeps_either_preactivation(m, n, k, dtype):
+    """At the C entry: in fp32 as summed, or rounded to x's type; either way nothing behind it is written, and the
+    backward entry reads what it is told that it is."""
+    from yolo_amd import _lib
+    from yolo_amd._lib import lib
+    g = torch.Generator().manual_seed(m + n + k)
+    x, w, b = _rand(g, m, k, dtype=dtype), _rand(g, n, k, scale=k ** -0.5, dtype=dtype), _rand(g, n, dtype=dtype)
+    dy = _rand(g, m, n, dtype=dtype)
+    _, _, p, ep = ref.linear_ref(x, w, b, None, None, dtype)
+    stream, code = _lib.current_stream_ptr(), {BF16: _lib.TYPE_BF16, F16: _lib.TYPE_F16}[dtype]
+
+    def scratch(desc, nbytes):
+        ws = torch.empty(max(nbytes, 1), dtype=torch.uint8, device="cuda")
+        desc.workspace, desc.workspace_bytes = ws.data_ptr(), nbytes
+        return ws
+    for f32 in (0, 1):
+        kept = torch.full((m * n + 16,), 7.0, dtype=F32 if f32 else dtype, device="cuda")
+        y, db = torch.empty(m, n, dtype=dtype, device="cuda"), torch.empty(n, device="cuda")
+        f = _lib.LinearDesc()
+        f.x, f.weight, f.bias, f.y, f.pre = x.data_ptr(), w.data_ptr(), b.data_ptr(), y.data_ptr(), kept.data_ptr()
+        f.m, f.n, f.k, f.ldx, f.ldw, f.ldy, f.type, f.activation, f.pre_f32 = m, n, k, k, k, n, code, _lib.ACT_CODES["silu"], f32
+        ws = scratch(f, lib.yolo_amd_linear_workspace_bytes(ctypes.byref(f)))          # noqa: F841
+        _lib.check(lib.yolo_amd_linear_forward(ctypes.byref(f), stream), "forward")
+        assert_within(kept[:m * n].reshape(m, n), p, rounded(p, ep, kept.dtype), "pre")
+        assert (kept[m * n:] == 7).all()
+        r = _lib.LinearBackwardDesc()
+        r.dy, r.pre, r.dbias, r.m, r.n, r.k, r.lddy = dy.data_ptr(), kept.data_ptr(), db.data_ptr(), m, n, k, n
+        r.type, r.dbias_f32, r.activation, r.pre_f32 = code, 1, _lib.ACT_CODES["silu"], f32
+        ws = scratch(r, lib.yolo_amd_linear_backward_workspace_bytes(ctypes.byref(r)))
+        _lib.check(lib.yolo_amd_linear_backward(ctypes.byref(r), stream), "backward")
+        own = d(kept[:m * n].reshape(m, n))                  # the slope of what was kept
+        want = (d(dy) * slope64(own, "silu")).sum(0)
+        assert_within(db, want, rounded(want, (EPS32 * 2 + 512 * 2.0 ** -24) * d(dy).abs().sum(0) * 1.1, F32), "db")

@@ -109,7 +109,7 @@ class LinearDesc(ctypes.Structure):
         ("ldx", ctypes.c_int64), ("ldw", ctypes.c_int64), ("ldr", ctypes.c_int64), ("ldy", ctypes.c_int64),
         ("type", ctypes.c_int),
         ("bias_f32", ctypes.c_int), ("residual_f32", ctypes.c_int), ("y_f32", ctypes.c_int),
-        ("activation", ctypes.c_int),
+        ("activation", ctypes.c_int), ("pre_f32", ctypes.c_int),
         ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_size_t),
     ]
 
@@ -128,6 +128,7 @@ class LinearBackwardDesc(ctypes.Structure):
         ("m", ctypes.c_int64), ("n", ctypes.c_int64), ("k", ctypes.c_int64),
         ("lddy", ctypes.c_int64), ("ldx", ctypes.c_int64), ("ldw", ctypes.c_int64),
         ("type", ctypes.c_int), ("dy_f32", ctypes.c_int), ("dbias_f32", ctypes.c_int), ("activation", ctypes.c_int),
+        ("pre_f32", ctypes.c_int),
         ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_size_t),
     ]
 

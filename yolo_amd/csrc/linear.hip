@@ -139,7 +139,7 @@ __device__ __forceinline__ float act_value(float p, int act) {
 }
 
 // act'(p).  From 100 on the curved ones have slope 1 and below -100 slope 0 in fp32: p is held there, so that no product
-// of an infinity (a pre-activation past fp16's range is kept as one) and a zero arises.  NaN stays NaN.
+// of an infinity (of the sum itself, or of one past fp16's range kept in that type) and a zero arises.  NaN stays NaN.
 template <int ACT>
 __device__ __forceinline__ float act_slope(float p) {
     if constexpr (ACT == YOLO_AMD_ACT_LEAKY) return p > 0.f ? 1.f : 0.1f;
@@ -183,9 +183,9 @@ struct Epilogue {
     const void* bias;      // [N] or null
     const void* res;       // [M][ldr] or null
     void* y;               // [M][ldy]
-    void* pre;             // [M][ldp] or null: P, rounded to T, for the backward pass
+    void* pre;             // [M][ldp] or null: P for the backward pass
     long long ldr, ldy, ldp;
-    int bias_f32, res_f32, y_f32, act;
+    int bias_f32, res_f32, y_f32, pre_f32, act;
     float* part;           // not null: the raw sums of one K slice go to [slice][M][ld_part] instead
     long long ld_part, slice_stride;
 };
@@ -236,7 +236,7 @@ __device__ __forceinline__ void store1(void* p, long long at, int f32, float v) 
 template <typename T>
 __device__ __forceinline__ void finish1(const Epilogue& e, long long m, int n, float s) {
     if (e.bias) s += load1<T>(e.bias, n, e.bias_f32);
-    if (e.pre) store1<T>(e.pre, m * e.ldp + n, 0, s);
+    if (e.pre) store1<T>(e.pre, m * e.ldp + n, e.pre_f32, s);
     s = act_value(s, e.act);
     if (e.res) s += load1<T>(e.res, m * e.ldr + n, e.res_f32);
     store1<T>(e.y, m * e.ldy + n, e.y_f32, s);
@@ -253,7 +253,7 @@ __device__ __forceinline__ void finish8(const Epilogue& e, long long m, int n, i
 #pragma unroll
             for (int i = 0; i < 8; ++i) v[i] += b[i];
         }
-        if (e.pre) store8<T>(e.pre, m * e.ldp + n, 0, v);
+        if (e.pre) store8<T>(e.pre, m * e.ldp + n, e.pre_f32, v);
         if (e.act) {
 #pragma unroll
             for (int i = 0; i < 8; ++i) v[i] = act_value(v[i], e.act);
@@ -390,10 +390,20 @@ __device__ __forceinline__ void finish_direct(const Epilogue& e, f32x4 (&acc)[TM
                     if (c >= 0 && c < 8) *reinterpret_cast<f32x4*>(t + (i * 16 + row) * 8 + c) = f32x4{v[h][0], v[h][1], v[h][2], v[h][3]};
                 }
             };
+            auto out = [&](void* p, long long ld, int f32) {
+                if (f32) {
+#pragma unroll
+                    for (int h = 0; h < 2; ++h)
+                        if (m < M && n + h * 16 + c4 < NV)
+                            *reinterpret_cast<f32x4u*>((float*)p + m * ld + n + h * 16 + c4) = f32x4{v[h][0], v[h][1], v[h][2], v[h][3]};
+                } else {
+                    const u32x4 o = pair_out<T>(v);
+                    if (in8) *reinterpret_cast<u32x4u*>((T*)p + m * ld + n + c8) = o;
+                }
+            };
             if (e.pre) {
                 if (ends) to_tail(tail + TM * 16 * 8);
-                const u32x4 o = pair_out<T>(v);
-                if (in8) *reinterpret_cast<u32x4u*>((T*)e.pre + m * e.ldp + n + c8) = o;
+                out(e.pre, e.ldp, e.pre_f32);
             }
             act_values<ACT>(v);
             if (ends) to_tail(tail);
@@ -413,15 +423,7 @@ __device__ __forceinline__ void finish_direct(const Epilogue& e, f32x4 (&acc)[TM
                         for (int k = 0; k < 4; ++k) v[h][k] += r[k];
                     }
             }
-            if (e.y_f32) {
-#pragma unroll
-                for (int h = 0; h < 2; ++h)
-                    if (m < M && n + h * 16 + c4 < NV)
-                        *reinterpret_cast<f32x4u*>((float*)e.y + m * e.ldy + n + h * 16 + c4) = f32x4{v[h][0], v[h][1], v[h][2], v[h][3]};
-            } else {
-                const u32x4 o = pair_out<T>(v);
-                if (in8) *reinterpret_cast<u32x4u*>((T*)e.y + m * e.ldy + n + c8) = o;
-            }
+            out(e.y, e.ldy, e.y_f32);
         }
     }
     if (!tail || n0 > NV || NV >= n0 + TN * 16) return;
@@ -434,7 +436,7 @@ __device__ __forceinline__ void finish_direct(const Epilogue& e, f32x4 (&acc)[TM
         if (m < M) {
             float s = tail[r * 8 + c];
             if (e.res) s += load1<T>(e.res, m * e.ldr + NV + c, e.res_f32);
-            if (e.pre) store1<T>(e.pre, m * e.ldp + NV + c, 0, tail[TM * 16 * 8 + r * 8 + c]);
+            if (e.pre) store1<T>(e.pre, m * e.ldp + NV + c, e.pre_f32, tail[TM * 16 * 8 + r * 8 + c]);
             store1<T>(e.y, m * e.ldy + NV + c, e.y_f32, s);
         }
     }
@@ -877,7 +879,7 @@ linear_pack_kernel(const PackArgs a) {
 struct DpreArgs {
     const void *dy, *pre;
     long long lddy, ldpre;
-    int dy_f32, act;
+    int dy_f32, pre_f32, act;
     void* dp;               // [M][ldp], zero filled past N; null: only the column sums are wanted
     long long ldp;
     float* part;            // [row block][N] column sums, or null
@@ -911,7 +913,7 @@ linear_dpre_kernel(const DpreArgs a) {
             float d[8], p[8];
             fetch(a.dy, m * a.lddy + n, a.dy_f32, d);
             if (a.pre) {
-                fetch(a.pre, m * a.ldpre + n, 0, p);
+                fetch(a.pre, m * a.ldpre + n, a.pre_f32, p);
                 times_slopes<8>(d, p, a.act);
             }
 #pragma unroll
@@ -1160,7 +1162,7 @@ static int check_forward(const yolo_amd_linear_desc* d) {
     YA_TRY(check_matrix("linear_forward", "y", d->y, d->ldy, d->m, (int)d->n, d->y_f32 ? 4 : 2));
     if (d->residual) YA_TRY(check_matrix("linear_forward", "residual", d->residual, d->ldr, d->m, (int)d->n, d->residual_f32 ? 4 : 2));
     if (d->bias) YA_TRY(check_matrix("linear_forward", "bias", d->bias, d->n, 1, (int)d->n, d->bias_f32 ? 4 : 2));
-    if (d->pre) YA_TRY(check_matrix("linear_forward", "pre", d->pre, d->n, d->m, (int)d->n, 2));
+    if (d->pre) YA_TRY(check_matrix("linear_forward", "pre", d->pre, d->n, d->m, (int)d->n, d->pre_f32 ? 4 : 2));
     return YA_OK;
 }
 
@@ -1206,7 +1208,8 @@ static int forward(const yolo_amd_linear_desc* d, const ForwardPlan& f, hipStrea
     Epilogue& e = a.e;
     e.bias = d->bias; e.res = d->residual; e.y = d->y; e.pre = d->pre;
     e.ldr = d->ldr; e.ldy = d->ldy; e.ldp = d->n;
-    e.bias_f32 = d->bias_f32; e.res_f32 = d->residual_f32; e.y_f32 = d->y_f32; e.act = d->activation;
+    e.bias_f32 = d->bias_f32; e.res_f32 = d->residual_f32; e.y_f32 = d->y_f32; e.pre_f32 = d->pre_f32;
+    e.act = d->activation;
     return launch_product<T, false, false>(f.tile, a, sc.take(f.part_bytes), s);
 }
 
@@ -1218,7 +1221,7 @@ static int check_backward(const yolo_amd_linear_backward_desc* d) {
     YA_TRY(check_matrix(me, "dy", d->dy, d->lddy, d->m, (int)d->n, d->dy_f32 ? 4 : 2));
     if (d->dweight) YA_TRY(check_matrix(me, "x", d->x, d->ldx, d->m, (int)d->k, 2));
     if (d->dx) YA_TRY(check_matrix(me, "weight", d->weight, d->ldw, d->n, (int)d->k, 2));
-    if (d->activation != YOLO_AMD_ACT_NONE) YA_TRY(check_matrix(me, "pre", d->pre, d->n, d->m, (int)d->n, 2));
+    if (d->activation != YOLO_AMD_ACT_NONE) YA_TRY(check_matrix(me, "pre", d->pre, d->n, d->m, (int)d->n, d->pre_f32 ? 4 : 2));
     if (d->dx) YA_TRY(check_matrix(me, "dx", d->dx, d->k, d->m, (int)d->k, 2));
     if (d->dweight) YA_TRY(check_matrix(me, "dweight", d->dweight, d->k, d->n, (int)d->k, 2));
     if (d->dbias) YA_TRY(check_matrix(me, "dbias", d->dbias, d->n, 1, (int)d->n, d->dbias_f32 ? 4 : 2));
@@ -1288,7 +1291,7 @@ static int backward(const yolo_amd_linear_backward_desc* d, const BackwardPlan& 
     if (b.own_dp || d->dbias) {
         DpreArgs g{};
         g.dy = d->dy; g.lddy = d->lddy; g.dy_f32 = d->dy_f32;
-        g.act = d->activation;
+        g.act = d->activation; g.pre_f32 = d->pre_f32;
         g.pre = g.act == YOLO_AMD_ACT_NONE ? nullptr : d->pre;
         g.ldpre = N;
         g.dp = b.own_dp ? dp : nullptr;

@@ -126,10 +126,10 @@ def _linear_forward(x, weight, bias, residual, act, out_dtype, keep_pre):
         residual, ldr = _rows(residual)
         r, r32 = residual.data_ptr(), residual.dtype is _F32
     if keep_pre:
-        pre = x.new_empty(shape)
+        pre = x.new_empty(shape, dtype=_F32)
         p = pre.data_ptr()
     d = LinearDesc(x.data_ptr(), weight.data_ptr(), b, r, y.data_ptr(), p, m, n, k, ldx, ldw, ldr, n, _TYPES[dt], b32, r32,
-                   out_dtype is _F32, act)
+                   out_dtype is _F32, act, True)
     nbytes = lib.yolo_amd_linear_workspace_bytes(d)
     ws = _scratch(d, nbytes, y) if nbytes else None      # noqa: F841  (alive over the call)
     _call(x.get_device(), lib.yolo_amd_linear_forward, d, "linear")
@@ -160,7 +160,7 @@ def _linear_backward(ctx, dy):
         db = dy.new_empty(n, dtype=b_dtype)
         dbp = db.data_ptr()
     d = LinearBackwardDesc(dyr.data_ptr(), xp, wp, 0 if pre is None else pre.data_ptr(), dxp, dwp, dbp, m, n, k, lddy, ldx,
-                           ldw, _TYPES[dt], dy.dtype is _F32, b_dtype is _F32, act)
+                           ldw, _TYPES[dt], dy.dtype is _F32, b_dtype is _F32, act, True)
     nbytes = lib.yolo_amd_linear_backward_workspace_bytes(d)
     ws = _scratch(d, nbytes, dy) if nbytes else None      # noqa: F841
     _call(dy.get_device(), lib.yolo_amd_linear_backward, d, "linear backward")
@@ -194,7 +194,7 @@ def linear(x, weight, bias=None, *, activation=None, residual=None, out_dtype=No
     "gelu_tanh" or "silu".  The result has ``out_dtype`` (x's type by default, or torch.float32).
 
     Sums are fp32; the result is rounded once.  Where a gradient of x, weight or bias will be wanted and there is
-    an activation, ``x @ weight.T + bias`` is kept in x's type for the backward pass; the gradients of x and
+    an activation, ``x @ weight.T + bias`` is kept in fp32 for the backward pass; the gradients of x and
     weight round d(loss)/d(pre-activation) to that type once, as the operand of their products."""
     _on_gpu("linear", x=x, weight=weight, bias=bias, residual=residual)
     dt = x.dtype
