@@ -6,7 +6,7 @@ import pytest
 import torch
 
 import layer_reference as ref
-from layer_reference import EPS32, assert_within, d, rounded, slope64
+from layer_reference import EPS32, TINY, U, assert_within, d, rounded, slope64
 
 pytestmark = pytest.mark.gpu
 
@@ -75,3 +75,57 @@ def test_linear_entry_keeps_either_preactivation(m, n, k, dtype):
         own = d(kept[:m * n].reshape(m, n))                  # the slope of what was kept
         want = (d(dy) * slope64(own, "silu")).sum(0)
         assert_within(db, want, rounded(want, (EPS32 * 2 + 512 * 2.0 ** -24) * d(dy).abs().sum(0) * 1.1, F32), "db")
+
+
+def _gradients(x, w, p, ep, dy, kind, bias_dtype):
+    """((dx, bound), (dw, bound), (db, bound)) with p kept in 32 bits (ep: its bound) and d(loss)/dp given to the products in
+    two parts of x's type t.
+
+    Bounds.  The slope is off by |act''| ep <= 0.8 ep and EPS32 of its own size; leaky and relu take the other slope only
+    where the sum's own rounding can change p's sign.  The first part is off by U[t] relative, the second part, which
+    holds the rest, by U[t] of that: U[t]^2 in all.  Below their normal range the parts of bf16 are off by TINY; those of fp16
+    are scaled by a power of two that puts the largest of them at 2^14 or above, so that their steps of 2^-24 are at most
+    2^-38 of it, and a rounding half of that.  A product of r terms in two parts adds 2 r of them."""
+    t = x.dtype
+    x, w, dy = d(x), d(w), d(dy)
+    s = slope64(p, kind)
+    if kind is None:
+        es = torch.zeros_like(p)
+    elif kind in ("leaky", "relu"):
+        es = (p.abs() <= ep).to(p.dtype) + EPS32 * s
+    else:
+        es = 0.8 * ep + EPS32 * (1 + s.abs())
+    dp = dy * s
+    edp = dy.abs() * es + 2.0 ** -23 * dp.abs()
+    largest = float(dp.abs().max()) if dp.numel() else 0.0
+    eop = edp + U[t] ** 2 * (dp.abs() + edp) + (largest * 2.0 ** -39 if t is F16 else TINY[t])
+    m, n = dp.shape
+    dx, dw, db = dp @ w, dp.t() @ x, dp.sum(0)
+    edx = eop @ w.abs() + 1.01 * (2 * n + 4) * 2.0 ** -23 * (dp.abs() @ w.abs())
+    edw = eop.t() @ x.abs() + 1.01 * (2 * m + 4) * 2.0 ** -23 * (dp.abs().t() @ x.abs())
+    edb = edp.sum(0) + 512 * 2.0 ** -24 * dp.abs().sum(0)
+    return ((dx, rounded(dx, edx, t)), (dw, rounded(dw, edw, t)), (db, rounded(db, edb, bias_dtype)))
+
+
+def _check(x, w, b, act, dy, out):
+    from yolo_amd.layers import linear
+    leaves = [t.detach().requires_grad_() for t in (x, w, b)]
+    got = torch.autograd.grad(linear(*leaves, activation=act, out_dtype=out), leaves, dy)
+    _, _, p, ep = ref.linear_ref(x, w, b, None, act, out)
+    for name, a, want in zip(("dx", "dw", "db"), got, _gradients(x, w, p, ep, dy, act, b.dtype)):
+        assert_within(a, *want, f"{name} {act}")
+
+
+# few rows, whole tiles, ragged ends and odd rows of every tile, a split reduction in dX and in dW
+SHAPES = [(1, 40, 64), (3, 984, 64), (64, 128, 64), (130, 75, 261), (333, 136, 1021), (200, 1030, 520), (16, 4096, 1024), (2500, 40, 48),
+          (1990, 2048, 264)]
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("m,n,k", SHAPES)
+def test_linear_gradients_lose_no_bits(m, n, k, dtype):
+    g = torch.Generator().manual_seed(m + 3 * n + 5 * k)
+    x, w = _rand(g, m, k, dtype=dtype), _rand(g, n, k, scale=k ** -0.5, dtype=dtype)
+    b = _rand(g, n, scale=0.3)
+    for act, out in ((None, F32), ("gelu", dtype), ("gelu_tanh", F32), ("silu", dtype), ("leaky", dtype), ("relu", dtype)):
+        _check(x, w, b, act, _rand(g, m, n, dtype=out), out)

@@ -4,6 +4,10 @@
 //   Y = act(P) + r
 //   dP = dY * act'(P);  dX = dP W;  dW = dP^T x;  db = sum over rows of dP;  dr = dY
 //
+// The matrix units take 16-bit operands and dP is an fp32 value: where the operands' type does not hold it, it goes in as
+// two parts of that type, dP = hi + lo up to its rounding squared (2^-16 relative in bf16, 2^-22 in fp16), and the products sum
+// hi and lo of 64 reduction indices in turn into the same accumulators.
+//
 // All three products are D[m][n] = sum_k A(m, k) B(n, k) with operands that are contiguous either along k
 // (x and W in the forward product) or along their own rows' index (W in dX, dP and x in dW): one tile kernel
 // takes both, the second kind through the transposing LDS read (ds_read_b64_tr_b16).
@@ -449,6 +453,7 @@ struct TileArgs {
     int M, N, K;
     int tiles_m, tiles_n;
     int ksteps;             // units of 64 reduction indices per slice (blockIdx.y = slice)
+    long long lo;           // bytes from A to its second part (AT or BT only), 0: it has one
     Epilogue e;
 };
 
@@ -593,7 +598,9 @@ linear_tile_kernel(const TileArgs a) {
     const int m0 = tile_m * BM, n0 = tile_n * BN;
     const int kbeg = (int)blockIdx.y * a.ksteps * kBK;
     const int kend = min(a.K, kbeg + a.ksteps * kBK);
-    const int nt = kend > kbeg ? (kend - kbeg + kBK - 1) / kBK : 0;
+    // steps of 64 reduction indices; A's two parts take one each
+    const bool two = (AT || BT) && a.lo != 0;
+    const int nt = kend > kbeg ? (kend - kbeg + kBK - 1) / kBK << (two ? 1 : 0) : 0;
 
     OpA opa;
     OpB opb;
@@ -632,14 +639,19 @@ linear_tile_kernel(const TileArgs a) {
     auto limit_b = [&]() {
         if (left_b < kBK) opb.limit(left_b);
     };
+    bool lo_a = false, lo_b = false;                   // at A's second part; B's tile for it is the same again
     auto next_a = [&]() {
-        opa.base += opa.step;
-        left_a -= kBK;
+        const bool stay = two && !lo_a;
+        opa.base += stay ? a.lo : two ? opa.step - a.lo : opa.step;
+        left_a -= stay ? 0 : kBK;
+        lo_a = stay;
         limit_a();
     };
     auto next_b = [&]() {
-        opb.base += opb.step;
-        left_b -= kBK;
+        const bool stay = two && !lo_b;
+        opb.base += stay ? 0 : opb.step;
+        left_b -= stay ? 0 : kBK;
+        lo_b = stay;
         limit_b();
     };
     // the slot two on (one step), as byte offsets
@@ -881,6 +893,7 @@ struct DpreArgs {
     long long lddy, ldpre;
     int dy_f32, pre_f32, act;
     void* dp;               // [M][ldp], zero filled past N; null: only the column sums are wanted
+    void* dp_lo;            // dP - dp, the same way; null: dp holds dP as it is
     long long ldp;
     float* part;            // [row block][N] column sums, or null
     int M, N, rows;         // rows per block
@@ -919,6 +932,14 @@ linear_dpre_kernel(const DpreArgs a) {
 #pragma unroll
             for (int i = 0; i < 8; ++i) sum[i] += d[i];
             if (a.dp) store8<T>(a.dp, m * a.ldp + n, 0, d);          // padded rows: zeros behind the last column
+            if (a.dp_lo) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const float r = d[i] - (float)(T)d[i];           // exact; no part of a value past the type's range
+                    d[i] = fabsf(r) < __builtin_inff() ? r : 0.f;
+                }
+                store8<T>(a.dp_lo, m * a.ldp + n, 0, d);
+            }
         }
     }
     if (!a.part) return;
@@ -998,7 +1019,8 @@ static const TileConfig kTileConfigs[] = {
     {64, 4, 3.2, 0.436, 3.1, 0.274},
 };
 
-static TilePlan plan_product(long long M, int N, long long K, bool kc_operands, int act) {
+// `parts` of the first operand: each step of 64 reduction indices is so many.
+static TilePlan plan_product(long long M, int N, long long K, bool kc_operands, int act, int parts = 1) {
     TilePlan p{};
     const long long steps = std::max<long long>(1, (K + kBK - 1) / kBK);
     // An activation's instructions lengthen an epilogue that nothing overlaps (256: 12 us a round for erf, 4.5 for the two
@@ -1034,10 +1056,10 @@ static TilePlan plan_product(long long M, int N, long long K, bool kc_operands, 
             const long long per = (steps + s - 1) / s, wgs = tiles * s, rest = wgs % slots;
             if ((steps + per - 1) / per != s) continue;
             if (s > 1 && wgs > slots) break;           // a split only fills a round that is not full
-            double t = (double)(wgs / slots) * (c.start + per * c.step);
+            double t = (double)(wgs / slots) * (c.start + parts * per * c.step);
             if (s == 1) t += (double)((wgs + slots - 1) / slots) * slow * (c.b == 256 ? 12.0 : c.b == 128 ? 2.5 : 0.7);
-            if (rest > 0) t += rest <= 256 ? c.start_1 + per * c.step_1 : c.start + per * c.step;
-            t = std::max(t, 2.0 + 2.0 * ((double)M * K + (double)N * K + (double)M * N) * 2e-7);   // at 5 TB/s
+            if (rest > 0) t += rest <= 256 ? c.start_1 + parts * per * c.step_1 : c.start + parts * per * c.step;
+            t = std::max(t, 2.0 + 2.0 * ((double)parts * M * K + (double)N * K + (double)M * N) * 2e-7);   // at 5 TB/s
             if (s > 1) t += 3.4 + 0.08 * s + (double)s * M * N * 2e-6;     // one more launch; partial sums out and in at 4 TB/s
             if (p.kernel == 0 || t < best) {
                 best = t;
@@ -1232,6 +1254,7 @@ struct BackwardPlan {
     TilePlan dx, dw;
     Matrix x, w;
     bool own_dp;            // dP is a tensor of its own (else dY is dP)
+    int parts;              // of dP
     int blocks, rows;       // row blocks of the column sums
     size_t dp_bytes, db_bytes, x_bytes, w_bytes, part_bytes;
     size_t bytes() const { return dp_bytes + db_bytes + x_bytes + w_bytes + part_bytes; }
@@ -1245,7 +1268,9 @@ static BackwardPlan plan_backward(const yolo_amd_linear_backward_desc* d) {
     b.w = Matrix{d->weight, d->ldw, d->n, (int)d->k};
     const bool products = (d->dx || d->dweight) && d->k > 0 && !empty;
     b.own_dp = products && (d->activation != YOLO_AMD_ACT_NONE || d->dy_f32 || !packed_ok(dy));
-    if (b.own_dp) b.dp_bytes = align_up((size_t)d->m * align_up(d->n, 8) * 2, 256);
+    // dY in the operands' type times 1 or 0 is a value of that type
+    b.parts = !d->dy_f32 && (d->activation == YOLO_AMD_ACT_NONE || d->activation == YOLO_AMD_ACT_RELU) ? 1 : 2;
+    if (b.own_dp) b.dp_bytes = b.parts * align_up((size_t)d->m * align_up(d->n, 8) * 2, 256);
     // enough blocks of rows to fill the chip, at least 16 rows each
     const long long cols = std::max<long long>(1, (d->n + 255) / 256), want = std::max<long long>(1, 2048 / cols);
     b.rows = (int)std::max<long long>(16, (d->m + want - 1) / want);
@@ -1253,12 +1278,12 @@ static BackwardPlan plan_backward(const yolo_amd_linear_backward_desc* d) {
     b.blocks = (int)((d->m + b.rows - 1) / b.rows);
     if (!products) return b;
     if (d->dx) {
-        b.dx = plan_product(d->m, (int)d->k, d->n, false, YOLO_AMD_ACT_NONE);
+        b.dx = plan_product(d->m, (int)d->k, d->n, false, YOLO_AMD_ACT_NONE, b.parts);
         b.w_bytes = packed_bytes(b.w);
         b.part_bytes = partial_bytes(b.dx, d->m, (int)d->k);
     }
     if (d->dweight) {
-        b.dw = plan_product(d->n, (int)d->k, d->m, false, YOLO_AMD_ACT_NONE);
+        b.dw = plan_product(d->n, (int)d->k, d->m, false, YOLO_AMD_ACT_NONE, b.parts);
         b.x_bytes = packed_bytes(b.x);
         b.part_bytes = std::max(b.part_bytes, partial_bytes(b.dw, d->n, (int)d->k));
     }
@@ -1295,6 +1320,7 @@ static int backward(const yolo_amd_linear_backward_desc* d, const BackwardPlan& 
         g.pre = g.act == YOLO_AMD_ACT_NONE ? nullptr : d->pre;
         g.ldpre = N;
         g.dp = b.own_dp ? dp : nullptr;
+        g.dp_lo = b.own_dp && b.parts == 2 ? (char*)dp + b.dp_bytes / 2 : nullptr;
         g.ldp = (long long)align_up(N, 8);
         g.part = d->dbias ? db : nullptr;
         g.M = M; g.N = N; g.rows = b.rows;
@@ -1308,6 +1334,7 @@ static int backward(const yolo_amd_linear_backward_desc* d, const BackwardPlan& 
         TileArgs a{};
         a.e.act = YOLO_AMD_ACT_NONE;
         a.e.ldy = K;
+        a.lo = b.own_dp && b.parts == 2 ? (long long)(b.dp_bytes / 2) : 0;
         Matrix in[2] = {b.x, b.w};
         launch_pack<T>(in, {b.x_bytes, b.w_bytes}, sc, s);
         const Matrix &x = in[0], &w = in[1];

@@ -193,9 +193,9 @@ def linear(x, weight, bias=None, *, activation=None, residual=None, out_dtype=No
     shape of the result: that type or fp32.  activation: None, "leaky" (slope 0.1), "relu", "gelu" (erf),
     "gelu_tanh" or "silu".  The result has ``out_dtype`` (x's type by default, or torch.float32).
 
-    Sums are fp32; the result is rounded once.  Where a gradient of x, weight or bias will be wanted and there is
-    an activation, ``x @ weight.T + bias`` is kept in fp32 for the backward pass; the gradients of x and
-    weight round d(loss)/d(pre-activation) to that type once, as the operand of their products."""
+    Sums are fp32; the result is rounded once, and so is each gradient.  Where a gradient of x, weight or bias will be
+    wanted and there is an activation, ``x @ weight.T + bias`` is kept in fp32 for the backward pass; the products of the
+    gradients of x and weight take d(loss)/d(pre-activation) in two parts of x's type where one does not hold it."""
     _on_gpu("linear", x=x, weight=weight, bias=bias, residual=residual)
     dt = x.dtype
     if dt is not torch.bfloat16 and dt is not torch.float16:
