@@ -112,8 +112,12 @@ def _check(x, w, b, act, dy, out):
     leaves = [t.detach().requires_grad_() for t in (x, w, b)]
     got = torch.autograd.grad(linear(*leaves, activation=act, out_dtype=out), leaves, dy)
     _, _, p, ep = ref.linear_ref(x, w, b, None, act, out)
-    for name, a, want in zip(("dx", "dw", "db"), got, _gradients(x, w, p, ep, dy, act, b.dtype)):
-        assert_within(a, *want, f"{name} {act}")
+    for name, a, (want, bound) in zip(("dx", "dw", "db"), got, _gradients(x, w, p, ep, dy, act, b.dtype)):
+        # from half a step past the type's largest number on, a value rounds to an infinity
+        end = (2 - U[a.dtype]) * 2.0 ** (15 if a.dtype is F16 else 127)
+        past, may = want.abs() - bound > end, (want.abs() + bound >= end) & torch.isinf(d(a))
+        assert torch.equal(d(a)[past], want[past].sign() * float("inf")), f"{name} {act}"
+        assert_within(torch.where(past | may, 0.0, d(a)), torch.where(past | may, 0.0, want), bound, f"{name} {act}")
 
 
 # few rows, whole tiles, ragged ends and odd rows of every tile, a split reduction in dX and in dW
@@ -129,3 +133,45 @@ def test_linear_gradients_lose_no_bits(m, n, k, dtype):
     b = _rand(g, n, scale=0.3)
     for act, out in ((None, F32), ("gelu", dtype), ("gelu_tanh", F32), ("silu", dtype), ("leaky", dtype), ("relu", dtype)):
         _check(x, w, b, act, _rand(g, m, n, dtype=out), out)
+
+
+@pytest.mark.parametrize("act", [None, "gelu"])
+@pytest.mark.parametrize("size,of_x,of_w", [(1e-9, 1e3, 1e3), (1e6, 1e-2, 1e-4), (1e-30, 1e4, 1e4)])
+def test_linear_gradients_past_the_range_of_fp16(size, of_x, of_w, act):
+    """fp16 operands with an fp32 result: its gradient may lie where fp16 has no numbers (a mean loss over wide scores, a
+    scaled loss), while the gradients of x and weight do not."""
+    g = torch.Generator().manual_seed(5)
+    m, n, k = 70, 520, 64
+    x, w, b = _rand(g, m, k, scale=of_x, dtype=F16), _rand(g, n, k, scale=of_w, dtype=F16), _rand(g, n)
+    dy = _rand(g, m, n, scale=size)
+    dy[3] = 0
+    dy[5] *= 2.0 ** -20
+    _check(x, w, b, act, dy, F32)
+
+
+def test_linear_gradients_of_zeros_and_infinities():
+    """An incoming gradient of zeros gives zeros; an infinity or NaN in one row leaves the gradients of the other rows as they
+    would be without it."""
+    from yolo_amd.layers import linear
+    g = torch.Generator().manual_seed(6)
+    for dtype in (F16, BF16):
+        x, w = _rand(g, 70, 64, dtype=dtype).requires_grad_(), _rand(g, 136, 64, dtype=dtype).requires_grad_()
+        y = linear(x, w, activation="silu", out_dtype=F32)
+        zeros = torch.autograd.grad(y, (x, w), torch.zeros(70, 136, device="cuda"), retain_graph=True)
+        assert not zeros[0].any() and not zeros[1].any()
+        dy = _rand(g, 70, 136, scale=1e-3)
+        clean, = torch.autograd.grad(y, x, dy, retain_graph=True)
+        dy[4, 7], dy[9, 100] = float("inf"), float("nan")
+        dx, dw = torch.autograd.grad(y, (x, w), dy)
+        keep = [i for i in range(70) if i not in (4, 9)]
+        assert torch.equal(dx[keep], clean[keep])
+        assert not torch.isfinite(dx[[4, 9]]).any() and not torch.isfinite(dw[7]).any() and torch.isnan(dw[100]).all()
+
+
+def test_linear_gradients_of_the_largest_values():
+    """Slopes above one at the type's largest gradients."""
+    for dtype, size, weight in ((F16, 65504.0, 2.0 ** -12), (BF16, 2.0 ** 127, 2.0 ** -40)):
+        x = torch.full((5, 8), 0.5, dtype=dtype).cuda()
+        w = torch.full((24, 8), weight, dtype=dtype).cuda()
+        b = torch.full((24,), 1.4).cuda()                     # gelu's slope is 1.13 there
+        _check(x, w, b, "gelu", torch.full((5, 24), size, dtype=dtype).cuda(), dtype)

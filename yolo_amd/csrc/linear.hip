@@ -6,7 +6,8 @@
 //
 // The matrix units take 16-bit operands and dP is an fp32 value: where the operands' type does not hold it, it goes in as
 // two parts of that type, dP = hi + lo up to its rounding squared (2^-16 relative in bf16, 2^-22 in fp16), and the products sum
-// hi and lo of 64 reduction indices in turn into the same accumulators.
+// hi and lo of 64 reduction indices in turn into the same accumulators.  fp16 lacks fp32's range as well: there dP is
+// multiplied by the power of two that brings its largest finite value to 2^14 .. 2^15, and the products' sums by its inverse.
 //
 // All three products are D[m][n] = sum_k A(m, k) B(n, k) with operands that are contiguous either along k
 // (x and W in the forward product) or along their own rows' index (W in dX, dP and x in dW): one tile kernel
@@ -190,6 +191,7 @@ struct Epilogue {
     void* pre;             // [M][ldp] or null: P for the backward pass
     long long ldr, ldy, ldp;
     int bias_f32, res_f32, y_f32, pre_f32, act;
+    const float* unscale;  // not null: the sums are multiplied by this first (products of the backward pass)
     float* part;           // not null: the raw sums of one K slice go to [slice][M][ld_part] instead
     long long ld_part, slice_stride;
 };
@@ -342,9 +344,10 @@ __device__ __forceinline__ void acc_read(f32x4& c, float (&v)[4]) {
 // The wave's rows m0 .. and columns n0 ...  Whole eights of columns (below NV = N rounded down) are stored from here; the
 // last one to seven columns of a row go, with bias and activation, through `tail` (LDS of this wave, [2][16 TM][8]:
 // outputs, pre-activations) and are finished by element behind the loop, in code that is short because it is cold.
-template <typename T, int ACT, bool IN_PLACE, int TM, int TN>
+template <typename T, int ACT, bool IN_PLACE, bool SCALED, int TM, int TN>
 __device__ __forceinline__ void finish_direct(const Epilogue& e, f32x4 (&acc)[TM][TN], int m0, int n0, int M, int N, int NV,
                                               int lane, float* tail) {
+    const float factor = SCALED && e.unscale ? *e.unscale : 1.f;
     const int row = lane & 15, c4 = (lane >> 4) * 4, c8 = (lane >> 4) * 8;
     float bias[TN][4];
 #pragma unroll
@@ -385,7 +388,7 @@ __device__ __forceinline__ void finish_direct(const Epilogue& e, f32x4 (&acc)[TM
             for (int h = 0; h < 2; ++h) {
                 acc_read<IN_PLACE>(acc[i][p * 2 + h], v[h]);
 #pragma unroll
-                for (int k = 0; k < 4; ++k) v[h][k] += bias[p * 2 + h][k];
+                for (int k = 0; k < 4; ++k) v[h][k] = (SCALED ? v[h][k] * factor : v[h][k]) + bias[p * 2 + h][k];
             }
             auto to_tail = [&](float* t) {
 #pragma unroll
@@ -738,7 +741,7 @@ linear_tile_kernel(const TileArgs a) {
         __syncthreads();                               // every wave is done with the ring
         tail = reinterpret_cast<float*>(lds) + w * (2 * WTM * 8);
     }
-#define YA_FINISH(ACT) finish_direct<T, ACT, IN_PLACE>(e, acc, mw, nw, a.M, a.N, nv, lane, tail)
+#define YA_FINISH(ACT) finish_direct<T, ACT, IN_PLACE, AT || BT>(e, acc, mw, nw, a.M, a.N, nv, lane, tail)
     if constexpr (AT || BT) {
         YA_FINISH(YOLO_AMD_ACT_NONE);
     } else {
@@ -772,6 +775,11 @@ linear_finish_kernel(const Epilogue e, const float* part, int slices, int M, int
             load8<T>(p, s * e.slice_stride, 1, u);
 #pragma unroll
             for (int k = 0; k < 8; ++k) v[k] += u[k];
+        }
+        if (e.unscale) {
+            const float factor = *e.unscale;
+#pragma unroll
+            for (int k = 0; k < 8; ++k) v[k] *= factor;
         }
         finish8<T>(e, m, n, N, v);
     }
@@ -895,6 +903,8 @@ struct DpreArgs {
     void* dp;               // [M][ldp], zero filled past N; null: only the column sums are wanted
     void* dp_lo;            // dP - dp, the same way; null: dp holds dP as it is
     long long ldp;
+    const float* scale;     // null: 1; else what dP is multiplied by where it is stored
+    float* peaks;           // [row block][column block] largest finite |dP|, or null
     float* part;            // [row block][N] column sums, or null
     int M, N, rows;         // rows per block
 };
@@ -913,6 +923,8 @@ linear_dpre_kernel(const DpreArgs a) {
     const long long r1 = min((long long)a.M, r0 + a.rows);
     const bool whole = n + 8 <= a.N;
     float sum[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    float peak = 0.f;
+    const float scale = a.scale ? *a.scale : 1.f;
     auto fetch = [&](const void* p, long long at, int f32, float (&v)[8]) {
         if (whole) {
             load8<T>(p, at, f32, v);
@@ -931,6 +943,12 @@ linear_dpre_kernel(const DpreArgs a) {
             }
 #pragma unroll
             for (int i = 0; i < 8; ++i) sum[i] += d[i];
+            if (a.peaks) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) peak = fabsf(d[i]) < __builtin_inff() ? fmaxf(peak, fabsf(d[i])) : peak;
+            }
+#pragma unroll
+            for (int i = 0; i < 8; ++i) d[i] *= scale;
             if (a.dp) store8<T>(a.dp, m * a.ldp + n, 0, d);          // padded rows: zeros behind the last column
             if (a.dp_lo) {
 #pragma unroll
@@ -942,6 +960,17 @@ linear_dpre_kernel(const DpreArgs a) {
             }
         }
     }
+    if (a.peaks) {
+        red[0][threadIdx.x] = peak;
+        __syncthreads();
+        if (threadIdx.x < 64) {
+            peak = fmaxf(fmaxf(red[0][threadIdx.x], red[0][threadIdx.x + 64]), fmaxf(red[0][threadIdx.x + 128], red[0][threadIdx.x + 192]));
+#pragma unroll
+            for (int i = 32; i; i >>= 1) peak = fmaxf(peak, __shfl_xor(peak, i));
+            if (threadIdx.x == 0) a.peaks[(long long)blockIdx.y * gridDim.x + blockIdx.x] = peak;
+        }
+        __syncthreads();
+    }
     if (!a.part) return;
 #pragma unroll
     for (int i = 0; i < 8; ++i) red[lane_r][lane_c * 8 + i] = sum[i];
@@ -952,6 +981,30 @@ linear_dpre_kernel(const DpreArgs a) {
 #pragma unroll
         for (int r = 0; r < RL; ++r) s += red[r][threadIdx.x];
         a.part[(long long)blockIdx.y * a.N + c] = s;
+    }
+}
+
+// scale[0]: the power of two that brings the largest of the peaks to 2^14 .. 2^15 (1 if there is none); scale[1]: its inverse.
+// Both are normal numbers: values below 2^-112, which come out lower than that, are zeros in any result of type fp16.
+__global__ void __launch_bounds__(1024)
+linear_scale_kernel(const float* peaks, int n, float* scale) {
+    __shared__ float red[16];
+    float peak = 0.f;
+    for (int i = threadIdx.x; i < n; i += 1024) peak = fmaxf(peak, peaks[i]);
+#pragma unroll
+    for (int i = 32; i; i >>= 1) peak = fmaxf(peak, __shfl_xor(peak, i));
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = peak;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+#pragma unroll
+        for (int i = 1; i < 16; ++i) peak = fmaxf(peak, red[i]);
+        int e = 0;
+        if (peak > 0.f) {
+            frexpf(peak, &e);                          // peak = 0.5 .. 1 times 2^e
+            e = min(15 - e, 126);
+        }
+        scale[0] = ldexpf(1.f, e);
+        scale[1] = ldexpf(1.f, -e);
     }
 }
 
@@ -1255,9 +1308,10 @@ struct BackwardPlan {
     Matrix x, w;
     bool own_dp;            // dP is a tensor of its own (else dY is dP)
     int parts;              // of dP
+    bool scaled;            // by a power of two
     int blocks, rows;       // row blocks of the column sums
-    size_t dp_bytes, db_bytes, x_bytes, w_bytes, part_bytes;
-    size_t bytes() const { return dp_bytes + db_bytes + x_bytes + w_bytes + part_bytes; }
+    size_t dp_bytes, db_bytes, scale_bytes, x_bytes, w_bytes, part_bytes;
+    size_t bytes() const { return dp_bytes + db_bytes + scale_bytes + x_bytes + w_bytes + part_bytes; }
 };
 
 static BackwardPlan plan_backward(const yolo_amd_linear_backward_desc* d) {
@@ -1276,6 +1330,8 @@ static BackwardPlan plan_backward(const yolo_amd_linear_backward_desc* d) {
     b.rows = (int)std::max<long long>(16, (d->m + want - 1) / want);
     if (d->dbias && !empty) b.db_bytes = align_up((size_t)((d->m + b.rows - 1) / b.rows) * d->n * 4, 256);
     b.blocks = (int)((d->m + b.rows - 1) / b.rows);
+    b.scaled = b.own_dp && b.parts == 2 && d->type == YOLO_AMD_TYPE_F16;
+    if (b.scaled) b.scale_bytes = align_up(((size_t)b.blocks * cols + 2) * 4, 256);
     if (!products) return b;
     if (d->dx) {
         b.dx = plan_product(d->m, (int)d->k, d->n, false, YOLO_AMD_ACT_NONE, b.parts);
@@ -1313,6 +1369,7 @@ static int backward(const yolo_amd_linear_backward_desc* d, const BackwardPlan& 
     Scratch sc{(char*)d->workspace};
     void* dp = sc.take(b.dp_bytes);
     float* db = (float*)sc.take(b.db_bytes);
+    float* scale = b.scaled ? (float*)sc.take(b.scale_bytes) : nullptr;    // the two of them, then the peaks
     if (b.own_dp || d->dbias) {
         DpreArgs g{};
         g.dy = d->dy; g.lddy = d->lddy; g.dy_f32 = d->dy_f32;
@@ -1324,7 +1381,17 @@ static int backward(const yolo_amd_linear_backward_desc* d, const BackwardPlan& 
         g.ldp = (long long)align_up(N, 8);
         g.part = d->dbias ? db : nullptr;
         g.M = M; g.N = N; g.rows = b.rows;
-        hipLaunchKernelGGL((linear_dpre_kernel<T>), dim3((N + 255) / 256, b.blocks), dim3(256), 0, s, g);
+        const dim3 grid((N + 255) / 256, b.blocks);
+        if (b.scaled) {                           // the largest value first: dY and P are read twice
+            DpreArgs first = g;
+            first.dp = first.dp_lo = nullptr;
+            first.peaks = scale + 2;
+            g.part = nullptr;
+            g.scale = scale;
+            hipLaunchKernelGGL((linear_dpre_kernel<T>), grid, dim3(256), 0, s, first);
+            hipLaunchKernelGGL(linear_scale_kernel, dim3(1), dim3(1024), 0, s, scale + 2, (int)(grid.x * grid.y), scale);
+        }
+        hipLaunchKernelGGL((linear_dpre_kernel<T>), grid, dim3(256), 0, s, g);
         if (d->dbias)
             hipLaunchKernelGGL((linear_dbias_kernel<T>), dim3((N + 63) / 64), dim3(1024), 0, s, db, b.blocks, N, d->dbias, d->dbias_f32);
     }
@@ -1334,6 +1401,7 @@ static int backward(const yolo_amd_linear_backward_desc* d, const BackwardPlan& 
         TileArgs a{};
         a.e.act = YOLO_AMD_ACT_NONE;
         a.e.ldy = K;
+        a.e.unscale = b.scaled ? scale + 1 : nullptr;
         a.lo = b.own_dp && b.parts == 2 ? (long long)(b.dp_bytes / 2) : 0;
         Matrix in[2] = {b.x, b.w};
         launch_pack<T>(in, {b.x_bytes, b.w_bytes}, sc, s);
