@@ -10,8 +10,8 @@ before a block fused with the block's gate, residual scale and residual add.
 Both are differentiable in every tensor argument (once; a second derivative raises), take inputs on any GPU and
 run on torch's current stream of that GPU.  They allocate outputs and scratch with torch's allocator, so they
 can be captured into a HIP graph, keep nothing between calls and never synchronise.  (As anywhere in torch, a
-backward pass is captured only while no eager graph of the same leaves is alive.)  Results depend on the
-inputs alone: every sum has a fixed order.  Row views (``x[:, :k]``) are read in place; other strides are copied.
+backward pass is captured only while no eager graph of the same leaves is alive.)  Forward-mode derivatives and
+traces (torch.jit.trace, make_fx) are refused.  Results depend on the inputs alone: every sum has a fixed order.  Row views (``x[:, :k]``) are read in place; other strides are copied.
 There is no CPU implementation: tensors on the CPU raise YoloAmdError.
 
 The reference has no counterpart of either.
@@ -19,6 +19,7 @@ The reference has no counterpart of either.
 from __future__ import annotations
 
 import torch
+import torch.autograd.forward_ad as _forward_ad
 
 from . import _lib
 from ._lib import BlockNormBackwardDesc, BlockNormDesc, LinearBackwardDesc, LinearDesc, YoloAmdError, check, lib
@@ -38,9 +39,25 @@ def _raw_stream(index):
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", _raw_stream)
 
 
+_is_tracing = torch._C._is_tracing
+_dispatch_modes = torch._C._len_torch_dispatch_stack
+
+
+def _refuse_transforms(what, tensors):
+    """The kernels write through pointers, which torch does not see: a tangent would be dropped (a derivative of zero) and
+    a trace would hold the outputs' allocation alone, or calls without the checks of what they are given."""
+    if _forward_ad._current_level >= 0 and any(
+            t is not None and _forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise NotImplementedError(f"{what}: there is no forward-mode derivative (an argument has a tangent)")
+    if _is_tracing() or torch._C._get_dispatch_mode(torch._C._TorchDispatchModeKey.PROXY) is not None:
+        raise YoloAmdError(f"{what}: cannot be recorded in a trace (torch.jit.trace, make_fx): the kernels are not torch operators")
+
+
 def _on_gpu(what, **tensors):
     """Every argument is a tensor (or None) on one GPU, the first one's.  Returns its index."""
     index = None
+    if _forward_ad._current_level >= 0 or _is_tracing() or _dispatch_modes():
+        _refuse_transforms(what, [t for t in tensors.values() if torch.is_tensor(t)])
     for name, t in tensors.items():
         if t is None:
             continue
@@ -137,6 +154,8 @@ def _linear_forward(x, weight, bias, residual, act, out_dtype, keep_pre):
 
 
 def _linear_backward(ctx, dy):
+    if _forward_ad._current_level >= 0 or _is_tracing() or _dispatch_modes():
+        _refuse_transforms("linear backward", (dy,))
     need_x, need_w, need_b, need_r = ctx.needs_input_grad[:4]
     act, x_shape, w_shape, dt, b_dtype, r_dtype = ctx.conf
     dres = (dy if dy.dtype is r_dtype else dy.to(r_dtype)) if need_r else None
@@ -273,6 +292,8 @@ def _norm_forward(x, residual, gate, after_weight, after_bias, before_weight, be
 
 
 def _norm_backward(ctx, dstream, dnormed):
+    if _forward_ad._current_level >= 0 or _is_tracing() or _dispatch_modes():
+        _refuse_transforms("block_norm backward", (dstream, dnormed))
     tensors = ctx.saved_tensors
     d, keep = _norm_desc(*tensors, ctx.conf, 0, 0)
     ds = dn = 0
