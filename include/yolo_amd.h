@@ -328,7 +328,8 @@ int yolo_amd_conv_forward(const yolo_amd_conv_desc* descs, int n, const void* ze
  * alignment to the element is accepted (rows that start on 16-byte boundaries with k a multiple of 8 are
  * read in place, others are copied into the workspace by the call).  Sums are fp32, in an order that
  * depends on the sizes only; y is rounded once.  m == 0 and n == 0 do nothing; k == 0 sums nothing.
- * m up to 2^30, n and k below 2^22; strides of 2^22 and more make a copy as well. */
+ * m up to 2^30, n and k below 2^22, and fewer than 2^24 tiles of 256 x 256 in a product's result (y here, dx and
+ * dweight backward): more is refused.  Strides of 2^22 and more make a copy as well. */
 #define YOLO_AMD_TYPE_F32 0
 #define YOLO_AMD_TYPE_BF16 1
 #define YOLO_AMD_TYPE_F16 2

@@ -1040,6 +1040,8 @@ struct Matrix {
 
 // Tiles address their rows with 32-bit byte offsets: 256 rows of this many elements.
 constexpr long long kMaxLd = (1ll << 22) - 1, kMaxRows = 1ll << 30;
+// A launch holds fewer than 2^32 threads: so many workgroups of 256.
+constexpr long long kMaxTiles = (1ll << 24) - 1;
 
 // can be read in place: whole 16-byte chunks, no row's last one reaching into the next
 static bool packed_ok(const Matrix& m) {
@@ -1072,7 +1074,7 @@ static const TileConfig kTileConfigs[] = {
     {64, 4, 3.2, 0.436, 3.1, 0.274},
 };
 
-// `parts` of the first operand: each step of 64 reduction indices is so many.
+// `parts` of the first operand: each step of 64 reduction indices is so many.  kernel 0: more tiles than a launch holds.
 static TilePlan plan_product(long long M, int N, long long K, bool kc_operands, int act, int parts = 1) {
     TilePlan p{};
     const long long steps = std::max<long long>(1, (K + kBK - 1) / kBK);
@@ -1104,6 +1106,7 @@ static TilePlan plan_product(long long M, int N, long long K, bool kc_operands, 
     }
     for (const TileConfig& c : kTileConfigs) {
         const long long tiles = ((M + c.b - 1) / c.b) * ((N + c.b - 1) / c.b);
+        if (tiles > kMaxTiles) continue;
         const int slots = 256 * tile_occupancy(c.b, c.ahead);
         for (int s = 1; s <= 64 && s <= steps; ++s) {
             const long long per = (steps + s - 1) / s, wgs = tiles * s, rest = wgs % slots;
@@ -1194,9 +1197,7 @@ static int launch_product(const TilePlan& p, TileArgs a, void* partial, hipStrea
     }
     a.tiles_m = (a.M + p.bm - 1) / p.bm;
     a.tiles_n = (a.N + p.bn - 1) / p.bn;
-    const long long tiles = (long long)a.tiles_m * a.tiles_n;
-    YA_REQUIRE(kernel == 0 || tiles < 1 << 24, "linear: %d x %d takes %lld tiles, more than a launch holds", a.M, a.N, tiles);
-    const dim3 grid((unsigned)tiles, (unsigned)p.slices);
+    const dim3 grid((unsigned)((long long)a.tiles_m * a.tiles_n), (unsigned)p.slices);
     if (kernel == 2562) hipLaunchKernelGGL((linear_tile_kernel<T, 256, 256, 2, AT, BT>), grid, dim3(256), 0, s, a);
     else if (kernel == 1282) hipLaunchKernelGGL((linear_tile_kernel<T, 128, 128, 2, AT, BT>), grid, dim3(256), 0, s, a);
     else if (kernel == 1284) hipLaunchKernelGGL((linear_tile_kernel<T, 128, 128, 4, AT, BT>), grid, dim3(256), 0, s, a);
@@ -1258,6 +1259,14 @@ static ForwardPlan plan_forward(const yolo_amd_linear_desc* d) {
     f.w_bytes = packed_bytes(f.w);
     f.part_bytes = partial_bytes(f.tile, d->m, (int)d->n);
     return f;
+}
+
+static int check_plan(const char* what, const TilePlan& p, long long m, long long n) {
+    YA_REQUIRE(p.kernel, "%s: a product of %lld x %lld takes more tiles than a launch holds (%lld of 256 x 256)", what, m, n, kMaxTiles);
+    return YA_OK;
+}
+static int check_plan(const yolo_amd_linear_desc* d, const ForwardPlan& f) {
+    return d->m == 0 || d->n == 0 ? YA_OK : check_plan("linear_forward", f.tile, d->m, d->n);
 }
 
 static int check_workspace(const char* what, const void* ws, size_t have, size_t need) {
@@ -1346,6 +1355,13 @@ static BackwardPlan plan_backward(const yolo_amd_linear_backward_desc* d) {
     return b;
 }
 
+static int check_plan(const yolo_amd_linear_backward_desc* d, const BackwardPlan& b) {
+    if (d->m == 0 || d->n == 0 || d->k == 0) return YA_OK;
+    if (d->dx) YA_TRY(check_plan("linear_backward", b.dx, d->m, d->k));
+    if (d->dweight) YA_TRY(check_plan("linear_backward", b.dw, d->n, d->k));
+    return YA_OK;
+}
+
 template <typename T>
 __global__ void __launch_bounds__(256) linear_zero_kernel(T* p, long long n) {
     for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n; i += (long long)gridDim.x * 256) p[i] = (T)0.f;
@@ -1431,13 +1447,16 @@ static int backward(const yolo_amd_linear_backward_desc* d, const BackwardPlan& 
 using namespace yolo_amd;
 
 extern "C" size_t yolo_amd_linear_workspace_bytes(const yolo_amd_linear_desc* d) {
-    return check_forward(d) == YA_OK ? plan_forward(d).bytes() : 0;
+    if (check_forward(d) != YA_OK) return 0;
+    const ForwardPlan f = plan_forward(d);
+    return check_plan(d, f) == YA_OK ? f.bytes() : 0;
 }
 
 extern "C" int yolo_amd_linear_query(const yolo_amd_linear_desc* d, yolo_amd_linear_choice* out) {
     YA_REQUIRE(out, "linear_query: null output");
     YA_TRY(check_forward(d));
     const ForwardPlan f = plan_forward(d);
+    YA_TRY(check_plan(d, f));
     *out = yolo_amd_linear_choice{f.tile.kernel, f.tile.bm, f.tile.bn, f.tile.slices, f.x_bytes != 0, f.w_bytes != 0, f.tile.ahead};
     return YA_OK;
 }
@@ -1446,17 +1465,21 @@ extern "C" int yolo_amd_linear_forward(const yolo_amd_linear_desc* d, void* stre
     YA_TRY(check_forward(d));
     const ForwardPlan f = plan_forward(d);
     if (d->m == 0 || d->n == 0) return YA_OK;
+    YA_TRY(check_plan(d, f));
     YA_TRY(check_workspace("linear_forward", d->workspace, d->workspace_bytes, f.bytes()));
     return d->type == YOLO_AMD_TYPE_BF16 ? forward<__bf16>(d, f, (hipStream_t)stream) : forward<_Float16>(d, f, (hipStream_t)stream);
 }
 
 extern "C" size_t yolo_amd_linear_backward_workspace_bytes(const yolo_amd_linear_backward_desc* d) {
-    return check_backward(d) == YA_OK ? plan_backward(d).bytes() : 0;
+    if (check_backward(d) != YA_OK) return 0;
+    const BackwardPlan b = plan_backward(d);
+    return check_plan(d, b) == YA_OK ? b.bytes() : 0;
 }
 
 extern "C" int yolo_amd_linear_backward(const yolo_amd_linear_backward_desc* d, void* stream) {
     YA_TRY(check_backward(d));
     const BackwardPlan b = plan_backward(d);
+    YA_TRY(check_plan(d, b));
     YA_TRY(check_workspace("linear_backward", d->workspace, d->workspace_bytes, b.bytes()));
     return d->type == YOLO_AMD_TYPE_BF16 ? backward<__bf16>(d, b, (hipStream_t)stream) : backward<_Float16>(d, b, (hipStream_t)stream);
 }
