@@ -405,6 +405,9 @@ typedef struct {
 
 size_t yolo_amd_linear_backward_workspace_bytes(const yolo_amd_linear_backward_desc* desc);
 int yolo_amd_linear_backward(const yolo_amd_linear_backward_desc* desc, void* stream);
+/* What yolo_amd_linear_backward runs its two products on (all zeros: that one is not wanted or has no terms). */
+int yolo_amd_linear_backward_query(const yolo_amd_linear_backward_desc* desc, yolo_amd_linear_choice* dx,
+                                   yolo_amd_linear_choice* dweight);
 
 /* ---------------------------------------------------------------- norms around a residual add
  * What lies between two blocks of a residual network, in one pass over memory.  Per row of d values:

@@ -202,6 +202,8 @@ SYMBOLS = {
     "yolo_amd_linear_query": (ctypes.c_int, [ctypes.POINTER(LinearDesc), ctypes.POINTER(LinearChoice)]),
     "yolo_amd_linear_backward_workspace_bytes": (ctypes.c_size_t, [ctypes.POINTER(LinearBackwardDesc)]),
     "yolo_amd_linear_backward": (ctypes.c_int, [ctypes.POINTER(LinearBackwardDesc), ctypes.c_void_p]),
+    "yolo_amd_linear_backward_query": (ctypes.c_int, [ctypes.POINTER(LinearBackwardDesc), ctypes.POINTER(LinearChoice),
+                                                      ctypes.POINTER(LinearChoice)]),
     "yolo_amd_block_norm_forward": (ctypes.c_int, [ctypes.POINTER(BlockNormDesc), ctypes.c_void_p]),
     "yolo_amd_block_norm_backward_workspace_bytes": (ctypes.c_size_t, [ctypes.POINTER(BlockNormBackwardDesc)]),
     "yolo_amd_block_norm_backward": (ctypes.c_int, [ctypes.POINTER(BlockNormBackwardDesc), ctypes.c_void_p]),

@@ -1476,6 +1476,17 @@ extern "C" size_t yolo_amd_linear_backward_workspace_bytes(const yolo_amd_linear
     return check_plan(d, b) == YA_OK ? b.bytes() : 0;
 }
 
+extern "C" int yolo_amd_linear_backward_query(const yolo_amd_linear_backward_desc* d, yolo_amd_linear_choice* dx,
+                                              yolo_amd_linear_choice* dweight) {
+    YA_REQUIRE(dx && dweight, "linear_backward_query: null output");
+    YA_TRY(check_backward(d));
+    const BackwardPlan b = plan_backward(d);
+    YA_TRY(check_plan(d, b));
+    *dx = yolo_amd_linear_choice{b.dx.kernel, b.dx.bm, b.dx.bn, b.dx.slices, 0, b.w_bytes != 0, b.dx.ahead};
+    *dweight = yolo_amd_linear_choice{b.dw.kernel, b.dw.bm, b.dw.bn, b.dw.slices, b.x_bytes != 0, 0, b.dw.ahead};
+    return YA_OK;
+}
+
 extern "C" int yolo_amd_linear_backward(const yolo_amd_linear_backward_desc* d, void* stream) {
     YA_TRY(check_backward(d));
     const BackwardPlan b = plan_backward(d);
