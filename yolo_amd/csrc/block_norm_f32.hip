@@ -94,16 +94,16 @@ static int launch(const yolo_amd_block_norm_desc* d, const NormArgs& a, int bloc
 // still has four rows or more for each of its groups: every block adds a row of partial sums per parameter.  8192 bf16
 // rows of 2048: 256 blocks 69 us, 768 blocks 63; 4207 fp32 rows of 769 (layer): 256 blocks 56 us, 525 45; 1239 rows of
 // 1021: 256 blocks 17 us, 768 23.
-struct BackwardPlan {
+struct NormBackwardPlan {
     bool sequence_gate, channel_gate, token_gate;
     long long sequences, length, chunk_rows;
     int seq_per_block, chunks, blocks, vectors;
     size_t part_bytes, gate_bytes;
 };
 
-static BackwardPlan plan(const yolo_amd_block_norm_backward_desc* b) {
+static NormBackwardPlan plan(const yolo_amd_block_norm_backward_desc* b) {
     const yolo_amd_block_norm_desc* d = &b->forward;
-    BackwardPlan p{};
+    NormBackwardPlan p{};
     if (d->rows == 0) return p;
     const bool want_gate = d->gate && b->dgate;
     p.token_gate = want_gate && d->rows_per_gate == 1;
@@ -181,7 +181,7 @@ extern "C" int yolo_amd_block_norm_forward(const yolo_amd_block_norm_desc* d, vo
 
 extern "C" size_t yolo_amd_block_norm_backward_workspace_bytes(const yolo_amd_block_norm_backward_desc* b) {
     if (check_backward(b) != YA_OK) return 0;
-    const BackwardPlan p = plan(b);
+    const NormBackwardPlan p = plan(b);
     return p.part_bytes + p.gate_bytes;
 }
 
@@ -199,7 +199,7 @@ extern "C" int yolo_amd_block_norm_backward(const yolo_amd_block_norm_backward_d
         YA_CHECK_HIP(hipGetLastError());
         return YA_OK;
     }
-    const BackwardPlan p = plan(b);
+    const NormBackwardPlan p = plan(b);
     const size_t need = p.part_bytes + p.gate_bytes;
     if (need) {
         YA_REQUIRE(b->workspace && ((uintptr_t)b->workspace & 255) == 0, "%s: the workspace is null or not 256-byte aligned", me);

@@ -1312,7 +1312,7 @@ static int check_backward(const yolo_amd_linear_backward_desc* d) {
     return YA_OK;
 }
 
-struct BackwardPlan {
+struct LinearBackwardPlan {
     TilePlan dx, dw;
     Matrix x, w;
     bool own_dp;            // dP is a tensor of its own (else dY is dP)
@@ -1323,8 +1323,8 @@ struct BackwardPlan {
     size_t bytes() const { return dp_bytes + db_bytes + scale_bytes + x_bytes + w_bytes + part_bytes; }
 };
 
-static BackwardPlan plan_backward(const yolo_amd_linear_backward_desc* d) {
-    BackwardPlan b{};
+static LinearBackwardPlan plan_backward(const yolo_amd_linear_backward_desc* d) {
+    LinearBackwardPlan b{};
     const bool empty = d->m == 0 || d->n == 0;
     const Matrix dy{d->dy, d->lddy, d->m, (int)d->n};
     b.x = Matrix{d->x, d->ldx, d->m, (int)d->k};
@@ -1355,7 +1355,7 @@ static BackwardPlan plan_backward(const yolo_amd_linear_backward_desc* d) {
     return b;
 }
 
-static int check_plan(const yolo_amd_linear_backward_desc* d, const BackwardPlan& b) {
+static int check_plan(const yolo_amd_linear_backward_desc* d, const LinearBackwardPlan& b) {
     if (d->m == 0 || d->n == 0 || d->k == 0) return YA_OK;
     if (d->dx) YA_TRY(check_plan("linear_backward", b.dx, d->m, d->k));
     if (d->dweight) YA_TRY(check_plan("linear_backward", b.dw, d->n, d->k));
@@ -1372,7 +1372,7 @@ static void launch_zero(T* p, long long n, hipStream_t s) {
 }
 
 template <typename T>
-static int backward(const yolo_amd_linear_backward_desc* d, const BackwardPlan& b, hipStream_t s) {
+static int backward(const yolo_amd_linear_backward_desc* d, const LinearBackwardPlan& b, hipStream_t s) {
     const int M = (int)d->m, N = (int)d->n, K = (int)d->k;
     if (M == 0 || N == 0) {                       // sums over nothing are zero
         if (d->dx) launch_zero((T*)d->dx, (long long)M * K, s);
@@ -1472,7 +1472,7 @@ extern "C" int yolo_amd_linear_forward(const yolo_amd_linear_desc* d, void* stre
 
 extern "C" size_t yolo_amd_linear_backward_workspace_bytes(const yolo_amd_linear_backward_desc* d) {
     if (check_backward(d) != YA_OK) return 0;
-    const BackwardPlan b = plan_backward(d);
+    const LinearBackwardPlan b = plan_backward(d);
     return check_plan(d, b) == YA_OK ? b.bytes() : 0;
 }
 
@@ -1480,7 +1480,7 @@ extern "C" int yolo_amd_linear_backward_query(const yolo_amd_linear_backward_des
                                               yolo_amd_linear_choice* dweight) {
     YA_REQUIRE(dx && dweight, "linear_backward_query: null output");
     YA_TRY(check_backward(d));
-    const BackwardPlan b = plan_backward(d);
+    const LinearBackwardPlan b = plan_backward(d);
     YA_TRY(check_plan(d, b));
     *dx = yolo_amd_linear_choice{b.dx.kernel, b.dx.bm, b.dx.bn, b.dx.slices, 0, b.w_bytes != 0, b.dx.ahead};
     *dweight = yolo_amd_linear_choice{b.dw.kernel, b.dw.bm, b.dw.bn, b.dw.slices, b.x_bytes != 0, 0, b.dw.ahead};
@@ -1489,7 +1489,7 @@ extern "C" int yolo_amd_linear_backward_query(const yolo_amd_linear_backward_des
 
 extern "C" int yolo_amd_linear_backward(const yolo_amd_linear_backward_desc* d, void* stream) {
     YA_TRY(check_backward(d));
-    const BackwardPlan b = plan_backward(d);
+    const LinearBackwardPlan b = plan_backward(d);
     YA_TRY(check_plan(d, b));
     YA_TRY(check_workspace("linear_backward", d->workspace, d->workspace_bytes, b.bytes()));
     return d->type == YOLO_AMD_TYPE_BF16 ? backward<__bf16>(d, b, (hipStream_t)stream) : backward<_Float16>(d, b, (hipStream_t)stream);
