@@ -327,7 +327,7 @@ int yolo_amd_conv_forward(const yolo_amd_conv_desc* descs, int n, const void* ze
  * fp32 where their flag says so.  Row strides (ld*) are in elements and at least the row's length; any
  * alignment to the element is accepted (rows that start on 16-byte boundaries with k a multiple of 8 are
  * read in place, others are copied into the workspace by the call).  Sums are fp32, in an order that
- * depends on the sizes only; y is rounded once.  m == 0 and n == 0 do nothing; k == 0 sums nothing.
+ * depends on the sizes and the activation only; y is rounded once.  m == 0 and n == 0 do nothing; k == 0 sums nothing.
  * m up to 2^30, n and k below 2^22, and fewer than 2^24 tiles of 256 x 256 in a product's result (y here, dx and
  * dweight backward): more is refused.  Strides of 2^22 and more make a copy as well. */
 #define YOLO_AMD_TYPE_F32 0

@@ -206,7 +206,9 @@ class _Linear(torch.autograd.Function):
 
 
 def linear(x, weight, bias=None, *, activation=None, residual=None, out_dtype=None):
-    """``act(x @ weight.T + bias) + residual`` in one launch (two where few output tiles share a long reduction).
+    """``act(x @ weight.T + bias) + residual`` in one launch; a second one where few output tiles
+    share a long reduction, and one ahead of it where rows of x or weight do not start on 16-byte boundaries or are
+    no whole multiples of 8 values (they are copied).
 
     x (..., K) and weight (N, K): bf16 or fp16, the same.  bias (N,): that type or fp32.  residual (..., N), the
     shape of the result: that type or fp32.  activation: None, "leaky" (slope 0.1), "relu", "gelu" (erf),
