@@ -64,18 +64,6 @@ __device__ __forceinline__ void lds_dma16_buf(__amdgpu_buffer_rsrc_t rsrc, uint3
                  : "memory", "m0");
 #pragma clang diagnostic pop
 }
-// The same in two parts, for a stream of matrix instructions: the destination (wave-uniform), then, behind at least one
-// other instruction and nothing that uses m0, the load.
-__device__ __forceinline__ void lds_dma_to(char* lds_dst) {
-    const uint32_t base = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)lds_dst;
-#pragma clang diagnostic push
-#pragma clang diagnostic ignored "-Winline-asm"
-    asm volatile("s_mov_b32 m0, %0" : : "s"(base) : "memory", "m0");
-#pragma clang diagnostic pop
-}
-__device__ __forceinline__ void lds_dma16_buf_here(__amdgpu_buffer_rsrc_t rsrc, uint32_t voff, uint32_t soff) {
-    asm volatile("buffer_load_dwordx4 %0, %1, %2 offen lds" : : "v"(voff), "s"(rsrc), "s"(soff) : "memory");
-}
 constexpr uint32_t kRawBufferWord3 = 0x00020000u;  // untyped 32-bit raw buffer descriptor word 3
 constexpr uint32_t kBufferNowhere = 0xFFFFFF00u;   // a byte offset beyond any descriptor these kernels build
 

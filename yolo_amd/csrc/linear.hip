@@ -43,6 +43,22 @@ __device__ __forceinline__ void mfma_in_place(v8<__bf16> a, v8<__bf16> b, f32x4&
 __device__ __forceinline__ void mfma_in_place(v8<_Float16> a, v8<_Float16> b, f32x4& c) {
     asm volatile("v_mfma_f32_16x16x32_f16 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b));
 }
+// The same with a load of 16 bytes per lane to lds_dst + 16 * lane (lds_dma16_buf) behind it, in one statement: between the
+// write of m0 and the load that reads it another instruction must lie and the compiler must not (8192^3: with s_nop there
+// 745 us, with the matrix instruction 722).
+#define YA_MFMA_LOAD(T, NAME)                                                                                              \
+    __device__ __forceinline__ void mfma_in_place_load(v8<T> a, v8<T> b, f32x4& c, __amdgpu_buffer_rsrc_t rsrc, uint32_t voff, \
+                                                       char* lds_dst) {                                                    \
+        const uint32_t to = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)lds_dst;                         \
+        asm volatile("s_mov_b32 m0, %5\n\t" NAME " %0, %1, %2, %0\n\tbuffer_load_dwordx4 %3, %4, 0 offen lds"              \
+                     : "+a"(c) : "v"(a), "v"(b), "v"(voff), "s"(rsrc), "s"(to) : "memory", "m0");                          \
+    }
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
+YA_MFMA_LOAD(__bf16, "v_mfma_f32_16x16x32_bf16")
+YA_MFMA_LOAD(_Float16, "v_mfma_f32_16x16x32_f16")
+#pragma clang diagnostic pop
+#undef YA_MFMA_LOAD
 // more wait states than any matrix instruction's result takes (16 passes at most)
 __device__ __forceinline__ void mfma_drain() { asm volatile("s_nop 15\n\ts_nop 15" ::: "memory"); }
 
@@ -520,17 +536,12 @@ struct Operand {
 #pragma unroll
         for (int j = 0; j < NI; ++j) voff[j] = kfirst + j * kstride < left ? voff[j] : kBufferNowhere;
     }
-    // instruction j of the step at `base`
-    __device__ __forceinline__ void issue(int j, char* buf, int w) const {
-        const __amdgpu_buffer_rsrc_t rs =
-            __builtin_amdgcn_make_buffer_rsrc((void*)base, 0, (int)kBufferBytes, (int)kRawBufferWord3);
-        lds_dma16_buf(rs, voff[j], 0, buf + (j * W + w) * 1024);
+    // instruction j of the step at `base`: source and destination
+    __device__ __forceinline__ __amdgpu_buffer_rsrc_t source() const {
+        return __builtin_amdgcn_make_buffer_rsrc((void*)base, 0, (int)kBufferBytes, (int)kRawBufferWord3);
     }
-    // the same in two parts with other instructions between them
-    __device__ __forceinline__ void target(int j, char* buf, int w) const { lds_dma_to(buf + (j * W + w) * 1024); }
-    __device__ __forceinline__ void issue_here(int j) const {
-        lds_dma16_buf_here(__builtin_amdgcn_make_buffer_rsrc((void*)base, 0, (int)kBufferBytes, (int)kRawBufferWord3), voff[j], 0);
-    }
+    __device__ __forceinline__ static char* target(int j, char* buf, int w) { return buf + (j * W + w) * 1024; }
+    __device__ __forceinline__ void issue(int j, char* buf, int w) const { lds_dma16_buf(source(), voff[j], 0, target(j, buf, w)); }
 };
 
 // fragment reads: 16 rows x 32 reduction indices; lane l holds row (l & 15), indices (l >> 4) * 8 ..
@@ -633,8 +644,7 @@ linear_tile_kernel(const TileArgs a) {
     constexpr int PRODUCTS = TM * TN, READS = TM + TN;
     constexpr int TILE = OpA::BYTES;
     static_assert(OpA::BYTES == OpB::BYTES && PRODUCTS % OpA::NI == 0, "slots of one size, loads evenly spaced");
-    constexpr int SPACE = PRODUCTS / OpA::NI, TARGET_AT = SPACE > 2 ? SPACE - 3 : 0;
-    static_assert(TARGET_AT + 1 < SPACE, "a load's two parts lie in one interval");
+    constexpr int SPACE = PRODUCTS / OpA::NI, ISSUE_AT = SPACE > 2 ? SPACE - 2 : SPACE - 1;
     int left_a = kend - kbeg, left_b = left_a;
     auto limit_a = [&]() {
         if (left_a < kBK) opa.limit(left_a);
@@ -667,6 +677,16 @@ linear_tile_kernel(const TileArgs a) {
         if constexpr (IN_PLACE) mfma_in_place(fr[j], fr[TN + i], acc[i][j]);
         else acc[i][j] = mfma(fr[j], fr[TN + i], acc[i][j]);
     };
+    // the same and load q of an operand
+    auto product_load = [&](const v8<T> (&fr)[READS], int e, const auto& op, int q, char* buf) {
+        const int i = e / TN, j = e % TN;
+        if constexpr (IN_PLACE) {
+            mfma_in_place_load(fr[j], fr[TN + i], acc[i][j], op.source(), op.voff[q], op.target(q, buf, w));
+        } else {
+            product(fr, e);
+            op.issue(q, buf, w);
+        }
+    };
 #define YA_FENCE() __builtin_amdgcn_sched_barrier(0)
     v8<T> f0[READS], f1[READS];
     limit_a();
@@ -690,12 +710,11 @@ linear_tile_kernel(const TileArgs a) {
         // first half: the second half's fragments in the first three quarters of it
 #pragma unroll
         for (int e = 0; e < PRODUCTS; ++e) {
-            product(f0, e);
+            if (e % SPACE == ISSUE_AT) product_load(f0, e, opa, e / SPACE, lds + fill);
+            else product(f0, e);
 #pragma unroll
             for (int q = 0; q < READS; ++q)
                 if (q * PRODUCTS / (READS * 2) == e) fetch(f1, q, lds + sa, lds + sb, 1);
-            if (e % SPACE == TARGET_AT) opa.target(e / SPACE, lds + fill, w);
-            if (e % SPACE == TARGET_AT + 1) opa.issue_here(e / SPACE);
             YA_FENCE();
         }
         next_a();
@@ -710,12 +729,11 @@ linear_tile_kernel(const TileArgs a) {
         const int na = two_on(sa), nb = two_on(sb);
 #pragma unroll
         for (int e = 0; e < PRODUCTS; ++e) {
-            product(f1, e);
+            if (e % SPACE == ISSUE_AT) product_load(f1, e, opb, e / SPACE, lds + sa);
+            else product(f1, e);
 #pragma unroll
             for (int q = 0; q < READS; ++q)
                 if (q * PRODUCTS / READS == e) fetch(f0, q, lds + na, lds + nb, 0);
-            if (e % SPACE == TARGET_AT) opb.target(e / SPACE, lds + sa, w);
-            if (e % SPACE == TARGET_AT + 1) opb.issue_here(e / SPACE);
             YA_FENCE();
         }
         next_b();
