@@ -63,20 +63,24 @@ YA_MFMA_LOAD(_Float16, "v_mfma_f32_16x16x32_f16")
 __device__ __forceinline__ void mfma_drain() { asm volatile("s_nop 15\n\ts_nop 15" ::: "memory"); }
 
 // ---------------------------------------------------------------- activations
-// exp2, reciprocal: the hardware's (1 ulp each).  erfc(x) for x >= 0 after Abramowitz and Stegun, Handbook of
-// Mathematical Functions, 7.1.26 (error at most 1.5e-7 absolute): a fifth of erff's instructions, and an epilogue of
-// one activation per matrix-unit column is bound by them.
+// exp2, reciprocal: the hardware's (1 ulp each).  erfc(x) for x >= 0 is t exp(-x^2) times a polynomial in t = 1 / (1 + 0.36 x),
+// the form of Abramowitz and Stegun, Handbook of Mathematical Functions, 7.1.26, with a degree and coefficients of its own:
+// fitted to erfc(x) exp(x^2) / t over x = 0 .. 9.5 so that the largest error is least, counted in units of 2e-8 of GELU and its slope
+// or 4e-6 of erfc, whichever is larger there (it is 1.3 of them).  GELU in fp32 is off by at most 7.1e-8 (the sum
+// 1 + erf loses 8.3e-8) and keeps five digits in its negative tail.  A quarter of erff's instructions, and an epilogue of one
+// activation per matrix-unit column is bound by them.
 constexpr float kLog2e = 1.44269504088896340736f;
+constexpr float kErfcT = 0.36f * 0.70710678118654752f;            // of |p|, x = |p| / sqrt 2
+constexpr float kErfc[7] = {0.202154681f, 0.217184246f, 0.105075903f, 0.434264660f, -0.362271845f, 0.568214238f, -0.164621860f};
 constexpr float kGeluC = 0.7978845608028654f, kGeluA = 0.044715f;
 
 // erfc(|p| / sqrt 2) and exp(-p^2 / 2); NaN for NaN, 0 and 0 for infinities
 __device__ __forceinline__ float erfc_scaled(float p, float& e) {
-    const float t = __builtin_amdgcn_rcpf(fmaf(fabsf(p), 0.3275911f * 0.70710678118654752f, 1.f));
+    const float t = __builtin_amdgcn_rcpf(fmaf(fabsf(p), kErfcT, 1.f));
     e = __builtin_amdgcn_exp2f(p * p * (-0.5f * kLog2e));
-    float q = fmaf(t, 1.061405429f, -1.453152027f);
-    q = fmaf(q, t, 1.421413741f);
-    q = fmaf(q, t, -0.284496736f);
-    q = fmaf(q, t, 0.254829592f);
+    float q = fmaf(t, kErfc[6], kErfc[5]);
+#pragma unroll
+    for (int k = 4; k >= 0; --k) q = fmaf(q, t, kErfc[k]);
     return q * t * e;
 }
 
@@ -112,20 +116,19 @@ __device__ __forceinline__ void act_values(float (&v)[2][4]) {
     float* p = &v[0][0];
     if constexpr (ACT == YOLO_AMD_ACT_GELU) {
         float t[8], e[8], q[8];
-        YA_EACH t[i] = fmaf(fabsf(p[i]), 0.3275911f * 0.70710678118654752f, 1.f);
+        YA_EACH t[i] = fmaf(fabsf(p[i]), kErfcT, 1.f);
         YA_STAGE();
         YA_EACH t[i] = __builtin_amdgcn_rcpf(t[i]);
         YA_EACH e[i] = p[i] * p[i] * (-0.5f * kLog2e);
         YA_STAGE();
         YA_EACH e[i] = __builtin_amdgcn_exp2f(e[i]);
-        YA_EACH q[i] = fmaf(t[i], 1.061405429f, -1.453152027f);
+        YA_EACH q[i] = fmaf(t[i], kErfc[6], kErfc[5]);
         YA_STAGE();
-        YA_EACH q[i] = fmaf(q[i], t[i], 1.421413741f);
-        YA_STAGE();
-        YA_EACH q[i] = fmaf(q[i], t[i], -0.284496736f);
-        YA_STAGE();
-        YA_EACH q[i] = fmaf(q[i], t[i], 0.254829592f);
-        YA_STAGE();
+#pragma unroll
+        for (int k = 4; k >= 0; --k) {
+            YA_EACH q[i] = fmaf(q[i], t[i], kErfc[k]);
+            YA_STAGE();
+        }
         YA_EACH q[i] = q[i] * t[i] * e[i];
         YA_STAGE();
         YA_EACH p[i] = fmaf(fabsf(__builtin_amdgcn_fmed3f(p[i], -100.f, 100.f)) * q[i], -0.5f, max0(p[i]));
