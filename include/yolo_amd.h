@@ -380,8 +380,8 @@ int yolo_amd_linear_query(const yolo_amd_linear_desc* desc, yolo_amd_linear_choi
 /* Gradients of yolo_amd_linear_forward for dy = d(loss)/dy (the residual's gradient is dy itself).
  * With dp = dy * act'(pre): dx = dp weight, dweight = dp^T x, dbias = column sums of dp.  Where `type` does not
  * hold dp, both products take it as two parts of that type, off by at most 2^-16 (bf16) or 2^-22 (fp16)
- * relative, fp16 scaled by a power of two so that dp may lie anywhere in fp32's range; the column sums take
- * it as it is.
+ * relative, fp16 scaled by one power of two so that dp may lie anywhere in fp32's range (what is below 2^-39 of
+ * its largest finite value counts as zero); the column sums take it as it is.
  * dx [m][k], dweight [n][k] of `type` without gaps between rows; each of dx, dweight, dbias may be NULL.
  * weight is read for dx only, x for dweight only, pre unless the activation is YOLO_AMD_ACT_NONE.
  * All sums have a fixed order. */
