@@ -14,9 +14,10 @@
 // every statistic, and written once.  The backward kernel recomputes p and h from u and r instead of reading a
 // stored h: the same bytes, and no rounding of h enters the gradients.  Statistics and sums are fp32; a variance
 // is taken around its mean in a second sweep over the registers.
-//   forward: 16384 x 4096 bf16 with an fp32 stream 153 to 163 us, 4.9 to 5.3 TB/s (a copy reaches 4.9); 8192 x 2048 bf16
-//     28 us, 4.9 TB/s
-//   backward: 16384 x 4096 as above 253 us, 4.8 TB/s; 8192 x 2048 bf16 59 us with the sums, 3.4 TB/s
+//   forward: 16384 x 4096 bf16 with an fp32 stream 150 to 164 us, 4.9 to 5.4 TB/s (a copy of that size reaches 5.5);
+//     8192 x 2048 bf16 33 to 35 us, 3.9 to 4.1 TB/s
+//   backward: 8192 x 2048 bf16 46 us, 4.4 TB/s, and 6 for the partial sums
+// (kernel times under rocprofv3; called again and again on the same inputs, partly in the caches, they are lower.)
 #pragma once
 #include <algorithm>
 

@@ -67,8 +67,8 @@ __device__ __forceinline__ void mfma_drain() { asm volatile("s_nop 15\n\ts_nop 1
 // the form of Abramowitz and Stegun, Handbook of Mathematical Functions, 7.1.26, with a degree and coefficients of its own:
 // fitted to erfc(x) exp(x^2) / t over x = 0 .. 9.5 so that the largest error is least, counted in units of 2e-8 of GELU and its slope
 // or 4e-6 of erfc, whichever is larger there (it is 1.3 of them).  GELU in fp32 is off by at most 7.1e-8 (the sum
-// 1 + erf loses 8.3e-8) and keeps five digits in its negative tail.  A quarter of erff's instructions, and an epilogue of one
-// activation per matrix-unit column is bound by them.
+// 1 + erf loses 8.3e-8) and keeps five digits in its negative tail.  An epilogue of one activation per matrix-unit column is
+// bound by the instructions of this: two terms fewer take 886 us instead of 900 at 8192 x 16384 x 4096 and leave 2.1e-7.
 constexpr float kLog2e = 1.44269504088896340736f;
 constexpr float kErfcT = 0.36f * 0.70710678118654752f;            // of |p|, x = |p| / sqrt 2
 constexpr float kErfc[7] = {0.202154681f, 0.217184246f, 0.105075903f, 0.434264660f, -0.362271845f, 0.568214238f, -0.164621860f};
@@ -582,8 +582,8 @@ constexpr int tile_occupancy(int b, int ahead) { return 163840 / ((2 * ahead + 1
 // tile whose accumulators fit (256 x 256: half of a SIMD's registers, one wave per SIMD) needs the fewest LDS reads and
 // the fewest bytes from L2, and with no second wave to fill gaps the instruction stream is laid by hand.  Smaller tiles
 // give every CU work in smaller products, with two workgroups to a CU or a deeper ring against memory's latency.
-// bf16: 8192^3 in 737 to 770 us, 1.43 to 1.49 PFLOP/s, where a library product takes 700 to 733; 8192 x 16384 x 4096 with
-// gelu_tanh 835 us, 1.32; 86528 x 128 x 256 with residual 22 us, 4.1 TB/s.
+// bf16: 8192^3 in 721 to 749 us, 1.47 to 1.52 PFLOP/s; 8192 x 16384 x 4096 with gelu_tanh 812 to 842 us, 1.31 to 1.35;
+// 86528 x 128 x 256 with residual 22 us, 4.1 TB/s.  dX of 4096 x 1024 with 4096 terms: in two parts 77 us, in one 39.
 template <typename T, int BM, int BN, int AHEAD, bool AT, bool BT>
 __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(tile_occupancy(BM, AHEAD), tile_occupancy(BM, AHEAD))))
 linear_tile_kernel(const TileArgs a) {
@@ -931,8 +931,11 @@ struct DpreArgs {
 };
 
 // Thread = eight columns of a run of rows (the last ones by element); column sums in fp32 over that run, added over the
-// runs by linear_dbias_kernel.  One row at a time: more rows in flight cost registers that hide more of memory's
-// latency as further waves (4096 x 4096 with GELU: 1 row 20.8 us, 2 rows 23.9, 4 rows 28.2; 100 MB).
+// runs by linear_dbias_kernel.  4096 x 4096 with GELU, fp32 pre-activation, two parts: 36 us, 168 MB, 4.7 TB/s.  One row at a
+// time: more rows in flight cost registers that hide more of memory's latency as further waves (the same with a 16-bit
+// pre-activation and one part, 100 MB: 1 row 20.8 us, 2 rows 23.9, 4 rows 28.2).
+// fp16 in two parts wants the largest value first: this kernel runs twice, dY and P are read twice (1531 x 1030: 8.1 + 8.2 us
+// and 1.7 between them).  Keeping fp32 dP for the second run instead would move as much.
 template <typename T>
 __global__ void __launch_bounds__(256)
 linear_dpre_kernel(const DpreArgs a) {
@@ -1078,9 +1081,10 @@ struct TilePlan {
 };
 
 // The tile kernels, with what a full round of workgroups takes (microseconds: start, prologue and epilogue; then each
-// step of 64 reduction indices), and a round that leaves at most one workgroup to a CU.  Fitted to bf16 products in
+// step of 64 reduction indices), and a round that leaves at most one workgroup to a CU.  Fitted to bf16 products y in
 // captured graphs, every kernel and split on 70 sizes from 33 x 64 x 64 to 8192^3: the choice they make is 1.0 % slower
-// than the fastest of each size (geometric mean; 22 % at the worst).  The 256-wide tile moves the fewest bytes per
+// than the fastest of each size (geometric mean; 22 % at the worst).  On 30 other sizes, geometric mean and worst: y in bf16
+// 0.9 and 17 %, in fp16 0.7 and 10; dX 0.2 and 2, 0.3 and 3; dW 0.5 and 6, 0.5 and 7.  The 256-wide tile moves the fewest bytes per
 // product but wants a tile for every CU; 128 four steps ahead hides memory's latency where a CU has one workgroup
 // (4096 x 1024 x 4096: 38.8 against 46.1 us), two ahead lets two workgroups do that for each other (2048 x 4096 x 4096:
 // 69.5 against 76.6); 64 is for what has fewer than 256 tiles of 128 (1024^3: 7.4 against 12.8).
@@ -1099,8 +1103,8 @@ static const TileConfig kTileConfigs[] = {
 static TilePlan plan_product(long long M, int N, long long K, bool kc_operands, int act, int parts = 1) {
     TilePlan p{};
     const long long steps = std::max<long long>(1, (K + kBK - 1) / kBK);
-    // An activation's instructions lengthen an epilogue that nothing overlaps (256: 12 us a round for erf, 4.5 for the two
-    // with an exponential and a reciprocal) more than one that another workgroup's products run beside (128: 2.3 and 1).
+    // An activation's instructions lengthen an epilogue that nothing overlaps (256: 12 to 13 us a round for erf, 3 to 5 for the
+    // two with an exponential and a reciprocal) more than one that another workgroup's products run beside (128: 2.3 and 1).
     const double slow = act == YOLO_AMD_ACT_GELU ? 1.0 : act == YOLO_AMD_ACT_GELU_TANH || act == YOLO_AMD_ACT_SILU ? 0.4 : 0.0;
     double best = 0;
     // Few rows: one workgroup streams 22.5 bytes a nanosecond, many 6000 (80 of them half as fast); x from L2 costs two
