@@ -175,3 +175,60 @@ def test_linear_gradients_of_the_largest_values():
         w = torch.full((24, 8), weight, dtype=dtype).cuda()
         b = torch.full((24,), 1.4).cuda()                     # gelu's slope is 1.13 there
         _check(x, w, b, "gelu", torch.full((5, 24), size, dtype=dtype).cuda(), dtype)
+
+
+def test_linear_gradients_offsets_past_32_bits():
+    """Pre-activations, their gradient and its second part of 2.4e9 values each: the last rows are where they belong."""
+    from yolo_amd.layers import linear
+    m, n, k = 2 ** 25 + 77, 72, 16
+    g = torch.Generator().manual_seed(12)
+    x, dy = (torch.full((m, c), v, dtype=BF16, device="cuda") for c, v in ((k, 0.5), (n, 0.25)))
+    x[-300:], dy[-300:] = _rand(g, 300, k, dtype=BF16), _rand(g, 300, n, dtype=BF16)
+    w = _rand(g, n, k, dtype=BF16)
+    x.requires_grad_()
+    dx, = torch.autograd.grad(linear(x, w, activation="gelu"), x, dy)
+    rows = torch.cat([torch.arange(5), torch.arange(m - 300, m)]).cuda()
+    _, _, p, ep = ref.linear_ref(x[rows], w, None, None, "gelu", BF16)
+    assert_within(dx[rows], *_gradients(x[rows], w, p, ep, dy[rows], "gelu", F32)[0], "dx")
+    assert torch.equal(dx[m - 400], dx[0])
+
+
+def test_linear_gradients_repeat_on_two_streams_and_in_a_graph():
+    """fp16 with its scale, on two streams at once and replayed from a graph with other gradients, bit for bit."""
+    from yolo_amd.layers import linear
+    g = torch.Generator().manual_seed(13)
+    w = _rand(g, 136, 72, dtype=F16).requires_grad_()
+    xs = [_rand(g, m, 72, dtype=F16).requires_grad_() for m in (90, 700)]
+    dys = [_rand(g, m, 136, scale=s) for m, s in ((90, 1e-9), (700, 1e6))]
+
+    def step(x, dy):
+        return torch.autograd.grad(linear(x, w, activation="silu", out_dtype=F32), (x, w), dy)
+    want = [step(x, dy) for x, dy in zip(xs, dys)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for _ in range(3):
+        got = []
+        for st, x, dy in zip(streams, xs, dys):
+            with torch.cuda.stream(st):
+                got.append(step(x, dy))
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for u, v in zip(got, want) for a, b in zip(u, v))
+    x, dy = xs[0].detach().clone(), dys[0].clone()
+    graph = torch.cuda.CUDAGraph()
+    leaf = w.detach().clone()
+
+    def captured():
+        a, b = x.detach().requires_grad_(), leaf.detach().requires_grad_()
+        return torch.autograd.grad(linear(a, b, activation="silu", out_dtype=F32), (a, b), dy)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        captured()
+    torch.cuda.current_stream().wait_stream(side)
+    with torch.cuda.graph(graph):
+        out = captured()
+    for size in (1.0, 1e-12, 3e7, 0.0):
+        dy.copy_(dys[0] / 1e-9 * size)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(out, captured()))
